@@ -15,11 +15,12 @@ LIB_PATH = Path(os.environ.get("EXL3_B200_LIB", PKG / "libexl3b200.so"))
 HEADER = PKG.parent / "include" / "exl3_b200.h"
 
 EXL3_OK, EXL3_ERR_ARG, EXL3_ERR_CUDA, EXL3_ERR_UNSUPPORTED, EXL3_ERR_DEVICE = range(5)
-DT_F16, DT_BF16, DT_F32 = 0, 1, 2
+DT_F16, DT_BF16, DT_F32, DT_E4M3 = 0, 1, 2, 3
 CB_3INST, CB_MCG, CB_MUL1 = 0, 1, 2
 LINEAR_CTRL_BYTES = 4096
 MOE_CTRL_BYTES = 262144
 MOE_STATIC_SCRATCH_BYTES = 8 << 20
+FP8_MOE_CTRL_BYTES = 131072
 
 _P = C.c_void_p
 _I64 = C.c_int64
@@ -59,6 +60,14 @@ _SIGS = {
     "exl3_moe_prepare": (_I, [_I]),
     "exl3_moe_info": (_I, [_I, _P]),
     "exl3_scratch_status": (_I, [_P, _I, _I, _P, _P]),
+    "exl3_fp8_quantize": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _I, _I, _P]),
+    "exl3_fp8_linear_scratch_bytes": (_I64, [_I64, _I64, _I64, _I]),
+    "exl3_fp8_linear": (_I, [_P, _I, _I64, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I, _P, _I, _I64, _I, _P, _I64, _P]),
+    "exl3_fp8_status": (_I, [_I, _P, _P]),
+    "exl3_fp8_moe_scratch_bytes": (_I64, [_I64, _I64, _I64, _I64]),
+    "exl3_fp8_moe_max_rows": (_I64, []),
+    "exl3_fp8_moe_decode": (_I, [_P, _I, _P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _I64, C.c_float, _I, _P,
+                                 _I64, _P]),
     "exl3_decode_roof_out_floats": (_I64, []),
     "exl3_decode_roof": (_I, [_I, _I, _I, _P, _I64, _P, _I64, _P, _P]),
 }

@@ -1,0 +1,170 @@
+// fp8.cuh -- device helpers shared by the e4m3 operators: the group scale, the
+// correctly rounded e4m3 quotient, activation loads, the fp8 tensor-core
+// instruction and cluster (distributed shared memory) accesses.
+#pragma once
+
+#include "tcgen05.cuh"
+
+namespace exl3 {
+
+constexpr int kFp8Block = 128;          // columns (and weight rows) that share one scale
+constexpr float kE4M3Max = 448.0f;
+constexpr int kDtE4M3 = 3;              // EXL3_DTYPE_E4M3
+constexpr uint32_t kFp8WTile = 128 * 128;   // one weight block, bytes
+
+// ---------------------------------------------------------------- quantising
+// Scale of a group from the bits of its largest magnitude (non-negative
+// floats order like their bits; a NaN orders above infinity, so it is kept):
+// max(amax / 448, 2^-126), or the smallest power of two not below that.  The
+// power of two is found on the rounded quotient: amax <= 448 * 2^e if and only
+// if RN(amax / 448) <= 2^e, because 2^e is an fp32 number and the next amax
+// above 448 * 2^e already rounds above it.
+__device__ __forceinline__ float fp8_scale(uint32_t amax_bits, bool pow2) {
+    float s = __fdiv_rn(__uint_as_float(amax_bits), kE4M3Max);
+    if (s < 0x1p-126f) s = 0x1p-126f;
+    if (pow2 && s < INFINITY) {
+        const uint32_t b = __float_as_uint(s);
+        s = __uint_as_float((b + 0x7FFFFFu) & 0xFF800000u);
+    }
+    return s;
+}
+
+// x / s to within the e4m3 rounding that follows, i.e. RN_e4m3 of the result
+// is RN_e4m3 of the real quotient.  x * (1 / s) is off by at most two units in
+// its last place (two roundings of 2^-24), which moves the e4m3 rounding only next to a midpoint of
+// two e4m3 values (low 20 bits 0x80000 for normal ones, low 19 bits 0 below
+// 2^-6); only there the quotient is taken by division and a remainder that
+// the division lost breaks the false tie.
+static __device__ __noinline__ float fp8_quotient_slow(float x, float s) {
+    const float q = __fdiv_rn(x, s);
+    const uint32_t b = __float_as_uint(q);
+    if ((b & 0x7FFFFu) != 0u || !(fabsf(q) < INFINITY) || q == 0.f) return q;
+    const float r = __fmaf_rn(-q, s, x);           // exact sign of x - q * s
+    if (r == 0.f || !(s < INFINITY)) return q;
+    const bool away = (r > 0.f) == (q > 0.f);      // |x / s| above or below |q|
+    return __uint_as_float(away ? b + 1u : b - 1u);
+}
+
+__device__ __forceinline__ float fp8_quotient(float x, float s, float inv, bool pow2) {
+    const float q = x * inv;
+    if (pow2) return q;                            // exact
+    const uint32_t b = __float_as_uint(q);
+    const bool mid = ((b + 0x80002u) & 0xFFFFFu) <= 4u;
+    const bool small = (b & 0x7FFFFFFFu) < 0x3C800000u && ((b + 2u) & 0x7FFFFu) <= 4u && (b << 1) != 0u;
+    if (mid || small) return fp8_quotient_slow(x, s);
+    return q;
+}
+
+// Two fp32 -> two e4m3 bytes (nearest, ties to even, finite values saturate),
+// `lo` in the low byte.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t fp8_quant4(const float (&v)[4], float s, float inv, bool pow2) {
+    const uint32_t a = e4m3x2(fp8_quotient(v[0], s, inv, pow2), fp8_quotient(v[1], s, inv, pow2));
+    const uint32_t b = e4m3x2(fp8_quotient(v[2], s, inv, pow2), fp8_quotient(v[3], s, inv, pow2));
+    return a | (b << 16);
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+__device__ __forceinline__ uint32_t abs_bits4(const float (&v)[4]) {
+    return max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+}
+
+// ---------------------------------------------------------------- loads
+__device__ __forceinline__ float load_f32(const void* x, int dtype, int64_t i) {
+    if (dtype == 0) return __half2float(reinterpret_cast<const __half*>(x)[i]);
+    if (dtype == 1) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[i]);
+    return reinterpret_cast<const float*>(x)[i];
+}
+
+// Four values starting at element i, as they lie in memory (8 bytes of a
+// 16-bit type in raw.x, raw.y): a load that can stay in flight.
+__device__ __forceinline__ uint4 load_raw4(const void* x, int dtype, int64_t i) {
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (dtype == 2) {
+        raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(x) + i);
+    } else if (dtype == kDtE4M3) {
+        raw.x = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(x) + i);
+    } else {
+        const uint2 h = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(x) + i);
+        raw.x = h.x; raw.y = h.y;
+    }
+    return raw;
+}
+
+// The same four values one by one, those at or past `left` as zero: rows whose
+// start or pitch is not a multiple of the vector, and the last columns.
+__device__ __forceinline__ uint4 load_raw4_tail(const void* x, int dtype, int64_t i, int left) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (q >= left) continue;
+        if (dtype == 2) w[q] = reinterpret_cast<const uint32_t*>(x)[i + q];
+        else if (dtype == kDtE4M3) w[0] |= (uint32_t) reinterpret_cast<const uint8_t*>(x)[i + q] << (8 * q);
+        else w[q >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(x)[i + q] << (16 * (q & 1));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void unpack4(const uint4& raw, int dtype, float (&v)[4]) {
+    if (dtype == 2) {
+        v[0] = __uint_as_float(raw.x); v[1] = __uint_as_float(raw.y);
+        v[2] = __uint_as_float(raw.z); v[3] = __uint_as_float(raw.w);
+    } else if (dtype == 1) {
+        v[0] = __uint_as_float(raw.x << 16); v[1] = __uint_as_float(raw.x & 0xFFFF0000u);
+        v[2] = __uint_as_float(raw.y << 16); v[3] = __uint_as_float(raw.y & 0xFFFF0000u);
+    } else {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+    }
+}
+
+// ---------------------------------------------------------------- tensor core
+// D[128 x N] (+)= A . B^T of 8-bit operands, K = 32 per instruction, fp32
+// accumulation; the instruction descriptor has the layout of kind::f16 with
+// e4m3 as format 0.
+__device__ __forceinline__ void tc_mma_f8(uint32_t dtmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(dtmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc) : "memory");
+}
+
+// Byte offset of byte k (< 128) of a row in a K-major tile with 128-byte rows
+// and the 128-byte swizzle.
+__device__ __forceinline__ uint32_t sw128_byte(int row, int k) {
+    return (uint32_t) (row * 128 + (((k >> 4) ^ (row & 7)) << 4) + (k & 15));
+}
+
+// ---------------------------------------------------------------- clusters
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// fp32 at shared-memory address `addr` (of this CTA's layout) in CTA `rank` of the cluster.
+__device__ __forceinline__ float ld_dsmem(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// Brings one tile into L2 ahead of the load that will use it.
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int c0, int c1) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];"
+                 :: "l"(tmap), "r"(c0), "r"(c1) : "memory");
+}
+
+}  // namespace exl3

@@ -90,3 +90,45 @@ class LinearEXL3:
 
     def unload(self):
         pass
+
+
+class LinearFP8:
+    """Dense linear over the checkpoint's e4m3 weight with one scale for each
+    128 x 128 block, for the modules a pack does not hold as EXL3; ``forward``
+    as LinearEXL3's.  ``weight`` float8_e4m3fn [out, in]; ``weight_scale``
+    [ceil(out / 128), ceil(in / 128)] in fp32, bf16, fp16 or float8_e8m0fnu
+    (powers of two), kept as fp32.  Inputs are quantised by row and 128 columns
+    inside the call; ``pow2_scale`` rounds their scales up to powers of two, as
+    checkpoints with power-of-two scales were trained."""
+    quant_type: str = "fp8"
+
+    def __init__(self, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                 out_dtype: torch.dtype | None = None, pow2_scale: bool = False, key: str | None = None):
+        if weight.dim() == 2 and weight.dtype == torch.float8_e4m3fn:
+            k = weight.size(1)
+            if weight.stride(1) != 1 or weight.stride(0) % 16 or weight.data_ptr() % 16:
+                # rows laid out once on 16-byte boundaries
+                padded = torch.zeros((weight.size(0), -(-k // 16) * 16), dtype=torch.uint8, device=weight.device)
+                padded[:, :k] = weight.view(torch.uint8)
+                weight = padded.view(torch.float8_e4m3fn)[:, :k]
+        self.weight = weight
+        self.weight_scale = weight_scale.to(torch.float32).contiguous()
+        _ext._fp8_weight_checks(self.weight, self.weight_scale)
+        self.out_features, self.in_features = (int(v) for v in weight.shape)
+        self.bias = bias
+        self.default_out_dtype = out_dtype or torch.half
+        self.pow2_scale = bool(pow2_scale)
+        self.key = key
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, **kw) -> "LinearFP8":
+        """From an unquantised fp16 / bf16 / fp32 weight [out, in] on the GPU."""
+        q, scale = _ext.fp8_quantize(weight, block_rows=128, pow2_scale=bool(kw.get("pow2_scale", False)))
+        return cls(q, scale, **kw)
+
+    def forward(self, x: torch.Tensor, params: dict | None = None, out_dtype: torch.dtype | None = None):
+        return _ext._fp8_linear(x, self.weight, self.weight_scale, None, self.bias,
+                                out_dtype or self.default_out_dtype, self.pow2_scale)
+
+    def unload(self):
+        pass

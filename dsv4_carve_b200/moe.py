@@ -236,11 +236,77 @@ def apply_moe_prefill(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tenso
     return out
 
 
+class Fp8MoeState:
+    """A layer's routed experts in e4m3 with one scale for each 128 x 128 block:
+    gate_up [E, 2 * intermediate, hidden] (gate rows first), down [E, hidden,
+    intermediate]; the scales in any floating type, kept as fp32.
+    ``pow2_scale``: the activations' scales are rounded up to powers of two."""
+
+    def __init__(self, gate_up: torch.Tensor, gate_up_scale: torch.Tensor, down: torch.Tensor,
+                 down_scale: torch.Tensor, pow2_scale: bool = False):
+        self.gate_up, self.down = gate_up, down
+        self.gate_up_scale = gate_up_scale.to(torch.float32).contiguous()
+        self.down_scale = down_scale.to(torch.float32).contiguous()
+        self.n_experts, self.hidden, self.inter = _ext._fp8_moe_weight_checks(
+            self.gate_up, self.gate_up_scale, self.down, self.down_scale)
+        self.pow2_scale = bool(pow2_scale)
+
+
+_FP8_SCRATCH: dict[tuple, torch.Tensor] = {}
+
+
+def _fp8_moe_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
+    """Zeroed scratch of one stream (calls on different streams may overlap).
+    A capture gets its own, from the graph's memory, so that graphs which are
+    replayed side by side share nothing."""
+    if torch.cuda.is_current_stream_capturing():
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        scratch[:_ext._lib.FP8_MOE_CTRL_BYTES].zero_()
+        return scratch
+    key = (device, _ext._stream(device))
+    buf = _FP8_SCRATCH.get(key)
+    if buf is None or buf.numel() < nbytes:
+        buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        _FP8_SCRATCH[key] = buf
+    return buf
+
+
+def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, state: Fp8MoeState,
+                  expert_map: torch.Tensor | None = None, limit: float = 10.0,
+                  out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
+    """The routed experts of an e4m3 layer: two kernels up to the row ceiling
+    of fp8_moe_decode, the rows in pieces of that size above it.  Returns the
+    [T, hidden] output, or None when the call is declined."""
+    T, topk = int(x2d.shape[0]), int(ids.shape[-1])
+    if not x2d.is_cuda or x2d.dim() != 2 or T < 1 or int(x2d.shape[1]) != state.hidden or not 1 <= topk <= 16:
+        _decline(f"fp8 geometry x={tuple(x2d.shape)} topk={topk}")
+        return None
+    ids2, route_w = _router_outputs(ids, weights, expert_map)
+    x = x2d if x2d.dtype in (torch.float16, torch.bfloat16, torch.float32) else x2d.to(torch.float16)
+    x = x.contiguous()
+    if out is None:
+        out = torch.empty(x.shape, dtype=out_dtype or (x.dtype if x.dtype != torch.float32 else torch.float16),
+                          device=x.device)
+    step = min(_ext.fp8_moe_max_rows(), 256 // topk)
+    with _ext._on_device(x.device):
+        scratch = _fp8_moe_scratch(x.device, _ext.fp8_moe_scratch_bytes(min(T, step), topk, state.hidden, state.inter))
+        for t in range(0, T, step):
+            part = slice(t, min(T, t + step))
+            _ext._fp8_moe_decode(x[part], out[part], state.gate_up, state.gate_up_scale, state.down, state.down_scale,
+                                 state.n_experts, state.hidden, state.inter, ids2[part], route_w[part], limit, scratch,
+                                 expert_map, state.pow2_scale, None)
+    _CALLS["b200"] += 1
+    return out
+
+
 def apply_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, state: MoeState,
               expert_map: torch.Tensor | None = None, limit: float = 10.0,
               out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
     """Decode kernel up to its row ceiling, tensor-core prefill above it
-    (the plugin's lna2 / fused-exl3_moe split, vllm_exl3_exl3.py.lna:1707-1779)."""
+    (the plugin's lna2 / fused-exl3_moe split, vllm_exl3_exl3.py.lna:1707-1779).
+    A layer whose experts are e4m3 (Fp8MoeState) goes to its own kernels."""
+    if isinstance(state, Fp8MoeState):
+        return apply_fp8_moe(x2d, ids, weights, state, expert_map, limit, out, out_dtype)
     if int(x2d.shape[0]) <= _ext.lna2_moe_max_rows() and int(x2d.shape[0]) * int(ids.shape[-1]) <= 256:
         return apply_moe_decode(x2d, ids, weights, state, expert_map, limit, out, out_dtype)
     return apply_moe_prefill(x2d, ids, weights, state, expert_map, limit, out, out_dtype)

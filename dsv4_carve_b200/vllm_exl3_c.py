@@ -17,6 +17,10 @@ Generalisations over the reference, all optional keyword arguments:
   * dequant_trellis / exl3_gemv / exl3_gemm(..., codebook=None): the
     reference maps mcg=True to MCG and mcg=False to MUL1 (bindings.cpp:49);
     ``codebook=0`` selects 3INST explicitly.
+
+Besides the EXL3 entries, ``fp8_quantize``, ``fp8_linear`` and
+``fp8_moe_decode`` serve the modules that a pack leaves in the checkpoint's
+e4m3 with one fp32 scale for each 128 x 128 block.
 """
 from __future__ import annotations
 
@@ -30,6 +34,7 @@ __all__ = [
     "dequant_trellis", "exl3_gemv", "exl3_gemm", "exl3_mgemm", "lna2_moe_decode", "lna2_moe_scratch_bytes",
     "lna2_moe_max_rows", "lna2_moe_prepare", "lna2_moe_info", "lna2_moe_status", "lna2_moe_status_word",
     "lna2_moe_decode_routed", "lna2_moe_prefill", "lna2_moe_prefill_scratch_bytes", "exl3_linear_scratch_bytes",
+    "fp8_quantize", "fp8_linear", "fp8_status", "fp8_moe_decode", "fp8_moe_scratch_bytes", "fp8_moe_max_rows",
 ]
 
 _DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
@@ -544,3 +549,223 @@ def exl3_moe(hidden_state, output_state, expert_count, token_sorted, weight_sort
                      ids, w, int(K_gate), float(act_limit), scratch, intermediate=inter,
                      codebook=2 if gate_mul1 else 1)
     output_state.add_(y)
+
+
+# --------------------------------------------------------------------- e4m3 with block scales
+_F8 = torch.float8_e4m3fn
+_DT_X8 = {**_DT, _F8: _lib.DT_E4M3}
+_FP8_GROUP = 128
+
+
+def _rows_of(x: torch.Tensor) -> tuple:
+    """(x as a 2-D view or copy, its leading dimension): rows may lie apart,
+    the elements of a row may not."""
+    k = x.size(-1)
+    if x.dim() != 2:
+        x = x.reshape(-1, k)
+    rows, ld = x.size(0), x.stride(0)
+    if rows <= 1:
+        ld = k
+    if (x.stride(1) != 1 and k > 1) or ld < k:
+        x = x.contiguous()
+        ld = k
+    return x, ld
+
+
+def fp8_quantize(x: torch.Tensor, *, block_rows: int = 1, pow2_scale: bool = False) -> tuple:
+    """(q, scale): x in e4m3 with one fp32 scale for each row and 128 columns
+    (``block_rows=1``: activations, x [..., cols]) or for each 128 x 128 block
+    (``block_rows=128``: a weight [rows, cols]).
+
+    scale = max(amax / 448, 2^-126); with ``pow2_scale`` the smallest power of
+    two that is not below it.  q = e4m3 nearest to x / scale, ties to even."""
+    _check(x.is_cuda, "fp8_quantize: the B200 build runs on CUDA tensors only")
+    _check(x.dtype in _DT, "fp8_quantize: x must be fp16, bf16 or fp32")
+    _check(block_rows in (1, _FP8_GROUP), "fp8_quantize: block_rows must be 1 or 128")
+    _check(x.dim() >= 1 and x.size(-1) >= 1, "fp8_quantize: x must have at least one column")
+    _check(block_rows == 1 or x.dim() == 2, "fp8_quantize: blocks of 128 rows need a 2-D x")
+    x2, ld = _rows_of(x)
+    rows, cols = x2.shape
+    q = torch.empty(x.shape, dtype=_F8, device=x.device)
+    groups = -(-cols // _FP8_GROUP)
+    shape = (*x.shape[:-1], groups) if block_rows == 1 else (-(-rows // _FP8_GROUP), groups)
+    scale = torch.empty(shape, dtype=torch.float32, device=x.device)
+    with _on_device(x.device):
+        _lib.call("exl3_fp8_quantize", x2.data_ptr(), _DT[x.dtype], rows, cols, ld, q.data_ptr(), cols,
+                  scale.data_ptr(), int(block_rows), int(bool(pow2_scale)), _stream(x.device))
+    return q, scale
+
+
+def _fp8_weight_checks(weight: torch.Tensor, weight_scale: torch.Tensor) -> None:
+    _check(weight.is_cuda and weight_scale.is_cuda and weight.device == weight_scale.device,
+           "fp8_linear: the B200 build runs on CUDA tensors of one device")
+    _check(weight.dtype == _F8 and weight.dim() == 2 and weight.size(0) >= 1 and weight.size(1) >= 1,
+           "fp8_linear: weight must be float8_e4m3fn [out_features, in_features]")
+    n, k = weight.shape
+    _check((weight.stride(1) == 1 or k == 1) and weight.data_ptr() % 16 == 0
+           and (n == 1 or (weight.stride(0) >= k and weight.stride(0) % 16 == 0)),
+           "fp8_linear: weight rows must be contiguous and 16-byte aligned (pad in_features to a multiple of 16)")
+    _check(weight_scale.dtype == torch.float32 and weight_scale.is_contiguous()
+           and weight_scale.shape == (-(-n // _FP8_GROUP), -(-k // _FP8_GROUP)),
+           "fp8_linear: weight_scale must be contiguous fp32 [ceil(out / 128), ceil(in / 128)]")
+
+
+def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
+               x_scale: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               out_dtype: torch.dtype | None = None, pow2_scale: bool = False) -> torch.Tensor:
+    """y[..., n] = x[..., k] . weight[n, k]^T (+ bias) over an e4m3 weight with
+    one fp32 scale for each 128 x 128 block.
+
+    x fp16 / bf16 / fp32 is quantised by row and 128 columns inside the call
+    (``pow2_scale`` as in fp8_quantize), or x is float8_e4m3fn with its
+    ``x_scale`` [..., ceil(k / 128)].  ``out_dtype`` defaults to x's type
+    (bf16 for an e4m3 x)."""
+    _fp8_weight_checks(weight, weight_scale)
+    return _fp8_linear(x, weight, weight_scale, x_scale, bias, out_dtype, pow2_scale)
+
+
+def _fp8_linear(x, weight, weight_scale, x_scale, bias, out_dtype, pow2_scale) -> torch.Tensor:
+    """fp8_linear behind the checks of the weight, which LinearFP8 makes once."""
+    n, k = weight.shape
+    device = weight.device
+    x_code = _DT_X8.get(x.dtype)
+    _check(x_code is not None, "fp8_linear: x must be fp16, bf16, fp32 or float8_e4m3fn")
+    _check(x.device == device, "fp8_linear: x and weight on different devices")
+    _check(x.dim() >= 1 and x.size(-1) == k, "fp8_linear: x feature dimension does not match weight")
+    x2, ld = _rows_of(x)
+    rows = x2.size(0)
+    xs_ptr = None
+    if x_code == _lib.DT_E4M3:
+        _check(x_scale is not None and x_scale.device == device and x_scale.dtype == torch.float32
+               and x_scale.shape == (*x.shape[:-1], -(-k // _FP8_GROUP)),
+               "fp8_linear: an e4m3 x needs x_scale fp32 [..., ceil(in / 128)]")
+        x_scale = x_scale.contiguous()
+        xs_ptr = x_scale.data_ptr()
+    else:
+        _check(x_scale is None, "fp8_linear: x_scale goes with an e4m3 x only")
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if x_code == _lib.DT_E4M3 else x.dtype
+    y_code = _DT.get(out_dtype)
+    _check(y_code is not None, "fp8_linear: out_dtype must be fp16, bf16 or fp32")
+    bias_ptr, bias_code = None, 0
+    if bias is not None:
+        _check(bias.device == device and bias.dtype in _DT and bias.shape == (n,) and (bias.stride(0) == 1 or n == 1),
+               "fp8_linear: bias must be contiguous fp16, bf16 or fp32 [out_features]")
+        bias_ptr, bias_code = bias.data_ptr(), _DT[bias.dtype]
+    y = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=device)
+    if rows == 0:
+        return y
+    lib = _lib.load()
+    need = lib.exl3_fp8_linear_scratch_bytes(rows, k, n, x_code)
+    scratch = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    with _on_device(device):
+        _lib.check(lib.exl3_fp8_linear(x2.data_ptr(), x_code, ld, xs_ptr, rows, k, n, weight.data_ptr(),
+                                       weight.stride(0) if n > 1 else -(-k // 16) * 16, weight_scale.data_ptr(),
+                                       bias_ptr, bias_code, y.data_ptr(), y_code, n, int(bool(pow2_scale)),
+                                       scratch.data_ptr() if scratch is not None else None, max(need, 0),
+                                       _stream(device)))
+    return y
+
+
+def fp8_status(device: torch.device | None = None, clear: bool = False) -> int:
+    """Status word of the fp8 linear kernels on a device (0 = healthy; bit 3: a
+    ring wait timed out).  Synchronizes; sticky until cleared."""
+    import ctypes
+
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    word = ctypes.c_uint32(0)
+    with _on_device(dev):
+        _lib.call("exl3_fp8_status", int(bool(clear)), ctypes.addressof(word), _stream(dev))
+    return int(word.value)
+
+
+def fp8_moe_max_rows() -> int:
+    """Row ceiling of fp8_moe_decode."""
+    return int(_lib.load().exl3_fp8_moe_max_rows())
+
+
+def fp8_moe_scratch_bytes(rows: int, topk: int = 8, hidden: int = 4096, intermediate: int = 2048) -> int:
+    """Scratch bytes of fp8_moe_decode for calls of `rows` rows (-1: not served)."""
+    return int(_lib.load().exl3_fp8_moe_scratch_bytes(int(rows), int(topk), int(hidden), int(intermediate)))
+
+
+def _fp8_moe_weight_checks(gate_up, gate_up_scale, down, down_scale) -> tuple:
+    """(experts, hidden, intermediate) of a layer's stacked e4m3 experts."""
+    ts = (gate_up, gate_up_scale, down, down_scale)
+    _check(all(t.is_cuda and t.device == gate_up.device and t.is_contiguous() for t in ts),
+           "fp8_moe_decode: weights and scales must be contiguous CUDA tensors of one device")
+    _check(gate_up.dtype == _F8 and down.dtype == _F8 and gate_up.dim() == 3 and down.dim() == 3,
+           "fp8_moe_decode: gate_up and down must be float8_e4m3fn [experts, out, in]")
+    E, I2, H = gate_up.shape
+    I = down.size(2)
+    _check(down.shape == (E, H, I) and I2 == 2 * I and E >= 1,
+           "fp8_moe_decode: gate_up must be [experts, 2 * intermediate, hidden], down [experts, hidden, intermediate]")
+    _check(H >= 128 and H % 128 == 0 and I >= 128 and I % 128 == 0,
+           "fp8_moe_decode: hidden and intermediate must be multiples of 128")
+    _check(gate_up.data_ptr() % 16 == 0 and down.data_ptr() % 16 == 0, "fp8_moe_decode: weights must be 16-byte aligned")
+    _check(gate_up_scale.dtype == torch.float32 and gate_up_scale.shape == (E, I2 // 128, H // 128)
+           and down_scale.dtype == torch.float32 and down_scale.shape == (E, H // 128, I // 128),
+           "fp8_moe_decode: scales must be fp32, one for each 128 x 128 block")
+    return E, H, I
+
+
+def fp8_moe_decode(x: torch.Tensor, out: torch.Tensor, gate_up: torch.Tensor, gate_up_scale: torch.Tensor,
+                   down: torch.Tensor, down_scale: torch.Tensor, expert_ids: torch.Tensor,
+                   routing_weights: torch.Tensor, swiglu_limit: float, scratch: torch.Tensor, *,
+                   expert_map: torch.Tensor | None = None, pow2_scale: bool = False,
+                   check_status: bool | None = None) -> torch.Tensor:
+    """Routed-expert layer for a few rows over e4m3 experts; writes and returns `out`.
+
+    gate_up [E, 2 * intermediate, hidden] (gate rows first) and down [E,
+    hidden, intermediate] with one fp32 scale for each 128 x 128 block.  The
+    router's outputs go in as lna2_moe_decode_routed takes them (int32 or int64
+    ids, fp32 / bf16 / fp16 weights, an optional expert_map); `scratch` as
+    there, of fp8_moe_scratch_bytes() bytes, zeroed before its first use."""
+    E, H, I = _fp8_moe_weight_checks(gate_up, gate_up_scale, down, down_scale)
+    return _fp8_moe_decode(x, out, gate_up, gate_up_scale, down, down_scale, E, H, I, expert_ids, routing_weights,
+                           swiglu_limit, scratch, expert_map, pow2_scale, check_status)
+
+
+def _fp8_moe_decode(x, out, gate_up, gate_up_scale, down, down_scale, E, H, I, expert_ids, routing_weights,
+                    swiglu_limit, scratch, expert_map, pow2_scale, check_status) -> torch.Tensor:
+    """fp8_moe_decode behind the checks of the weights, which Fp8MoeState makes once."""
+    import ctypes
+
+    device = gate_up.device
+    _check(x.device == device and x.dtype in _DT and x.dim() == 2 and x.size(1) == H and x.is_contiguous(),
+           "fp8_moe_decode: x must be contiguous fp16, bf16 or fp32 [m, hidden] on the weights' device")
+    m = x.size(0)
+    _check(out.device == device and out.dtype in _DT and out.shape == x.shape and out.is_contiguous(),
+           "fp8_moe_decode: out must be contiguous fp16, bf16 or fp32 of x's shape on its device")
+    _check(expert_ids.device == device and expert_ids.dtype in _IDS_DT and expert_ids.is_contiguous()
+           and expert_ids.dim() == 2 and expert_ids.size(0) == m,
+           "fp8_moe_decode: expert_ids must be contiguous int32 or int64 [m, topk]")
+    topk = expert_ids.size(1)
+    _check(routing_weights.device == device and routing_weights.dtype in _DT and routing_weights.is_contiguous()
+           and routing_weights.shape == expert_ids.shape,
+           "fp8_moe_decode: routing_weights must be contiguous fp32, bf16 or fp16 [m, topk]")
+    lib = _lib.load()
+    need = lib.exl3_fp8_moe_scratch_bytes(m, topk, H, I)
+    _check(need > 0, "fp8_moe_decode: 1..64 rows, top-k 1..16, rows * top-k up to 256, hidden up to 16384 and "
+                     "intermediate up to 8192 are served")
+    limit = float(swiglu_limit)
+    _check(limit > 0.0, "fp8_moe_decode: the SwiGLU limit must be positive")
+    _check(scratch.device == device and scratch.dtype == torch.uint8 and scratch.is_contiguous()
+           and scratch.numel() >= need, "fp8_moe_decode: scratch too small")
+    map_ptr, n_global = None, 0
+    if expert_map is not None:
+        _check(expert_map.device == device and expert_map.dtype == torch.int64 and expert_map.dim() == 1
+               and expert_map.is_contiguous() and expert_map.numel() >= 1,
+               "EXL3 expert_map must be a contiguous CUDA int64 [n_global] on the hidden-state device")
+        map_ptr, n_global = expert_map.data_ptr(), expert_map.numel()
+    route = _lib.MoeRoute(expert_ids.data_ptr(), _IDS_DT[expert_ids.dtype], routing_weights.data_ptr(),
+                          _DT[routing_weights.dtype], map_ptr, n_global)
+    with _on_device(device):
+        _lib.check(lib.exl3_fp8_moe_decode(x.data_ptr(), _DT[x.dtype], out.data_ptr(), _DT[out.dtype], m, H, I,
+                                           gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(),
+                                           down_scale.data_ptr(), E, ctypes.addressof(route), topk, limit,
+                                           int(bool(pow2_scale)), scratch.data_ptr(), scratch.numel(),
+                                           _stream(device)))
+        if check_status_default() if check_status is None else check_status:
+            _raise_on_status(scratch)
+    return out

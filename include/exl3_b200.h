@@ -17,7 +17,8 @@
  *   svh      fp16  [n]                  output sign/scale vector
  *   W = diag(suh) . H . W' . H . diag(svh) / 128, H = 128-block Sylvester Hadamard.
  * Codebooks: 0 = 3INST, 1 = MCG (the production codebook), 2 = MUL1.
- * Activation / output dtypes: 0 = fp16, 1 = bf16, 2 = fp32.
+ * Activation / output dtypes: 0 = fp16, 1 = bf16, 2 = fp32 (3 = e4m3, where a
+ * declaration says so).
  *
  * Each declaration cites the reference interface it replaces (paths relative
  * to the lna-lab/dsv4-carve project root).
@@ -39,7 +40,7 @@ typedef enum {
     EXL3_ERR_DEVICE = 4        /* the device-side status word reports a failure */
 } exl3_status;
 
-enum { EXL3_DTYPE_F16 = 0, EXL3_DTYPE_BF16 = 1, EXL3_DTYPE_F32 = 2 };
+enum { EXL3_DTYPE_F16 = 0, EXL3_DTYPE_BF16 = 1, EXL3_DTYPE_F32 = 2, EXL3_DTYPE_E4M3 = 3 };
 enum { EXL3_CB_3INST = 0, EXL3_CB_MCG = 1, EXL3_CB_MUL1 = 2 };
 
 /* Version of this ABI (bumped on any signature change). */
@@ -306,6 +307,78 @@ int exl3_moe_prefill_routed(const void* x, int x_dtype, void* out, int out_dtype
                             int64_t n_experts, const int32_t* k_table, int K, int kmax, int cb,
                             const exl3_moe_route* route, int64_t topk, float swiglu_limit,
                             void* scratch, int64_t scratch_bytes, void* stream);
+
+/* ------------------------------------------------------------------ e4m3 with block scales
+ * Modules that a pack does not hold as EXL3 stay in the checkpoint's e4m3
+ * (4 exponent bits, 3 mantissa bits, largest value 448) with one fp32 scale
+ * for each 128 x 128 block of a weight.  No counterpart in the reference,
+ * whose pack leaves such modules to the serving framework.
+ *
+ * Quantiser.  For a group g -- a row's 128 columns (block_rows = 1,
+ * activations) or a 128 x 128 block (block_rows = 128, weights); the last ones
+ * may be smaller:
+ *   scale_g = max(max|x_g| / 448, 2^-126), rounded to fp32; with pow2 != 0 the
+ *             smallest power of two that is not below it
+ *   q       = the e4m3 value nearest to x / scale_g, ties to even
+ * A group that holds a NaN or an infinity has that scale and NaN for what the
+ * quotient leaves undefined.  x fp16 / bf16 / fp32 [rows, cols] with leading
+ * dimension ldx; q [rows, cols] bytes with leading dimension ldq; scale
+ * [rows, ceil(cols / 128)] or [ceil(rows / 128), ceil(cols / 128)], contiguous.
+ * rows = 0 does nothing. */
+int exl3_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
+                      float* scale, int block_rows, int pow2, void* stream);
+
+/* Linear over an e4m3 weight:
+ *   y[r, j] = bias[j] + sum over k-groups g of 128 of
+ *             sx[r, g] * w_scale[j / 128, g] * sum_{i in g} qx[r, i] * w[j, i]
+ * w [n, k] row-major with leading dimension ldw (a multiple of 16 bytes, base
+ * 16-byte aligned), w_scale fp32 [ceil(n / 128), ceil(k / 128)] contiguous;
+ * any k, n >= 1.  x fp16 / bf16 / fp32 is quantised by row and 128 columns
+ * inside the call (pow2 as above; x_scale NULL), or x is e4m3
+ * (EXL3_DTYPE_E4M3) with x_scale fp32 [rows, ceil(k / 128)].  bias [n] (fp16 /
+ * bf16 / fp32) or NULL; y fp16 / bf16 / fp32 with leading dimension ldy >= n.
+ * Products are exact and accumulated in fp32.  `scratch`:
+ * exl3_fp8_linear_scratch_bytes(rows, k, n, x_dtype) bytes (0: may be NULL), 16-byte
+ * aligned, need not be cleared, one call at a time.  rows = 0 does nothing.
+ * Launched with programmatic stream serialization; nothing that the preceding
+ * kernel may write is read before that kernel has completed. */
+int64_t exl3_fp8_linear_scratch_bytes(int64_t rows, int64_t k, int64_t n, int x_dtype);
+int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const float* x_scale, int64_t rows, int64_t k, int64_t n,
+                    const void* w, int64_t ldw, const float* w_scale, const void* bias, int bias_dtype,
+                    void* y, int y_dtype, int64_t ldy, int pow2, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* Status word of the fp8 linear kernels on the current device (bit 3: a ring
+ * wait timed out), sticky until cleared.  Synchronizes `stream`; not for use
+ * during graph capture. */
+int exl3_fp8_status(int clear, uint32_t* status, void* stream);
+
+/* Routed-expert MoE layer for a few tokens over e4m3 experts, two kernels.
+ * For every valid (row, slot), expert e = ids[row, slot]:
+ *   g = x . Wgate_e^T, u = x . Wup_e^T      (as exl3_fp8_linear, x quantised by row)
+ *   a = silu(min(g, L)) * clamp(u, -L, L)   (fp32), quantised by 128 columns
+ *   out[row] += weights[row, slot] * (a . Wdown_e^T)   (fp32 sum), then one cast.
+ * An expert listed twice in one row counts twice; a slot whose id is invalid
+ * (as in exl3_moe_decode_routed) is skipped, its weight not read; a row without
+ * a valid slot gives zeros.  gate_up e4m3 [n_experts, 2 * inter, hidden] (gate
+ * rows first) with gate_up_scale fp32 [n_experts, 2 * inter / 128, hidden / 128];
+ * down [n_experts, hidden, inter] with down_scale [n_experts, hidden / 128,
+ * inter / 128]; all contiguous, weights 16-byte aligned.  m in
+ * 1..exl3_fp8_moe_max_rows(), topk in 1..16, m * topk <= 256, hidden (<= 16384)
+ * and inter (<= 8192) multiples of 128.  x, out fp16 / bf16 / fp32
+ * [m, hidden]; swiglu_limit > 0 (infinity: no clamp); pow2 as above for x and
+ * a.  `scratch`: >= exl3_fp8_moe_scratch_bytes(m, topk, hidden, inter) bytes
+ * whose first EXL3_FP8_MOE_CTRL_BYTES are zero before first use (calls reset
+ * what they need of them, whatever sizes follow); one call at a time per
+ * scratch.  Its status word is read by
+ * exl3_scratch_status.  No kernel waits for another CTA, so calls on different
+ * streams with scratches of their own may overlap. */
+#define EXL3_FP8_MOE_CTRL_BYTES 131072
+int64_t exl3_fp8_moe_scratch_bytes(int64_t m, int64_t topk, int64_t hidden, int64_t inter);
+int64_t exl3_fp8_moe_max_rows(void);
+int exl3_fp8_moe_decode(const void* x, int x_dtype, void* out, int out_dtype, int64_t m, int64_t hidden, int64_t inter,
+                        const void* gate_up, const float* gate_up_scale, const void* down, const float* down_scale,
+                        int64_t n_experts, const exl3_moe_route* route, int64_t topk, float swiglu_limit, int pow2,
+                        void* scratch, int64_t scratch_bytes, void* stream);
 
 /* Decode-issue roof: runs the GEMV engine's decode inner loop (window
  * extraction, codebook, split-accumulator MMAs) on 32 weight tiles held in
