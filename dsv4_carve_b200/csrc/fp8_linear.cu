@@ -13,8 +13,14 @@
 // it goes from HBM through TMA into swizzled shared memory and from there to
 // the tensor core without touching a register -- and the rows of x are N.
 // A cluster of CTAs splits k; its partial sums meet in distributed shared
-// memory in rank order, so there is no workspace, no counter and no atomic,
-// and results do not depend on timing.
+// memory in rank order, so there is no counter and no atomic, and results do
+// not depend on timing.
+//
+// Many rows (fp8_gemm_kernel): bound by the tensor cores.  x is quantised by a
+// kernel of its own (launched just before, overlapped) and its rows are the M
+// operand of a pair of CTAs (cta_group::2, 256 rows x NW weight rows), so the
+// factor s_x * s_w is one number a thread for each group of 128 columns and
+// the scaling is one packed fp32 FMA for two values.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -39,6 +45,7 @@ constexpr int kFsMaxCluster = 8;
 
 struct FsParams {
     CUtensorMap wmap;            // W [n][k] bytes, box [128 k, 128 n], 128-byte swizzle
+    CUtensorMap xmap;            // PRE: e4m3 x [rows][k], box [128 k, NT]
     const void* x;
     int64_t ldx;
     const float* xs;             // scales of an e4m3 x [rows][groups], else null
@@ -49,6 +56,7 @@ struct FsParams {
     int x_dtype, y_dtype, bias_dtype, pow2, xvec;
     int rows, n, k, groups;
     int stages, cluster;
+    int early;                   // nothing still running can write the weights
 };
 
 template <int NT>
@@ -70,7 +78,8 @@ struct FsHead {
     float fac[kFsMaxStages][NT];          // s_x * s_w of the stage's rows
 };
 
-template <int NT>
+// PRE: x comes as e4m3 through TMA; otherwise warps 4-7 quantise it into the ring.
+template <int NT, bool PRE>
 __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kernel(const __grid_constant__ FsParams p) {
     using L = FsLayout<NT>;
     extern __shared__ uint8_t fs_raw[];
@@ -85,37 +94,53 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
     const int kbeg = rank * p.groups / S, nsteps = (rank + 1) * p.groups / S - kbeg;
     uint32_t* status = &g_fp8_status;
 
-    pdl_launch_dependents();
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(&H.full[s], 1 + rows);
+            mbar_init(&H.full[s], PRE ? 2 : 1 + rows);
             mbar_init(&H.empty[s], 1 + kFsEpiWarps);
         }
         for (int b = 0; b < L::kBufs; ++b) { mbar_init(&H.tfull[b], 1); mbar_init(&H.tempty[b], kFsEpiWarps); }
         fence_barrier_init();
     }
     if (warp == kFsMmaWarp) tmem_alloc(&H.tmem, L::kTmemCols);
-    // L2 prefetch ahead of the wait for the previous kernel: it brings no value
-    // into this SM, so weights that kernel may have written are still read later.
-    if (warp == kFsProducerWarp && lane < min(nsteps, p.stages)) tma_prefetch_2d(&p.wmap, (kbeg + lane) * 128, n0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = H.tmem;
-    pdl_wait();
 
     float acc[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j] = 0.f;
 
     if (warp == kFsProducerWarp) {
+        const int ahead = min(nsteps, p.stages);
+        auto weights = [&](int s) {
+            const int st = s % p.stages;
+            mbar_arrive_expect_tx(&H.full[st], kFp8WTile + (PRE ? L::kXBytes : 0));
+            tma_load_2d(ring + st * L::kStage, &p.wmap, (kbeg + s) * 128, n0, &H.full[st]);
+        };
+        auto inputs = [&](int s) {
+            const int st = s % p.stages;
+            tma_load_2d(ring + st * L::kStage + kFp8WTile, &p.xmap, (kbeg + s) * 128, row0, &H.full[st]);
+        };
+        // Ahead of the wait for the previous kernel: the weights themselves
+        // when it is the quantiser of this call, which began after everything
+        // before it; otherwise it may write them, and only a prefetch into L2,
+        // which brings no value into this SM, is ahead.
+        if (p.early) {
+            if (lane == 0) for (int s = 0; s < ahead; ++s) weights(s);
+        } else if (lane < ahead) {
+            tma_prefetch_2d(&p.wmap, (kbeg + lane) * 128, n0);
+        }
+        pdl_wait();
         if (lane == 0) {
+            pdl_launch_dependents();
+            if (PRE) fence_proxy_async_global();
             int issued = 0;
             for (int s = 0; s < nsteps; ++s) {
-                const int st = s % p.stages;
-                if (!mbar_wait(&H.empty[st], ((s / p.stages) + 1u) & 1u, status)) break;
-                mbar_arrive_expect_tx(&H.full[st], kFp8WTile);
-                tma_load_2d(ring + st * L::kStage, &p.wmap, (kbeg + s) * 128, n0, &H.full[st]);
+                if (s >= p.stages && !mbar_wait(&H.empty[s % p.stages], ((s / p.stages) + 1u) & 1u, status)) break;
+                if (s >= ahead || !p.early) weights(s);
+                if (PRE) inputs(s);
                 ++issued;
             }
             // no copy may still be in flight when the CTA retires
@@ -123,6 +148,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
                 if (!mbar_wait(&H.full[i % p.stages], (i / p.stages) & 1u, status)) break;
         }
     } else if (warp == kFsMmaWarp) {
+        pdl_wait();
         if (lane == 0) {
             const uint32_t id = idesc_f16(128, ncols);
             const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
@@ -138,10 +164,30 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
                 tc_commit(&H.tfull[b]);
             }
         }
+    } else if (warp >= kFsEpiWarps && PRE) {
+        // the factors of a step's rows, one warp a step
+        pdl_wait();
+        for (int s = warp - kFsEpiWarps; s < nsteps; s += kFsXWarps) {
+            const int st = s % p.stages;
+            const float ws = __ldg(p.ws + (int64_t) tile * p.groups + kbeg + s);
+            float f[(NT + 31) / 32];
+#pragma unroll
+            for (int h = 0; h < (NT + 31) / 32; ++h) {
+                const int j = h * 32 + lane;
+                f[h] = j < rows ? __ldcg(p.xs + (int64_t) (row0 + j) * p.groups + kbeg + s) * ws : 0.f;
+            }
+            if (!mbar_wait_lanes(&H.empty[st], ((s / p.stages) + 1u) & 1u, status)) break;
+#pragma unroll
+            for (int h = 0; h < (NT + 31) / 32; ++h)
+                if (h * 32 + lane < NT) H.fac[st][h * 32 + lane] = f[h];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&H.full[st]);
+        }
     } else if (warp >= kFsEpiWarps) {
         // x: one warp for each (step, row), four elements a lane.  Rows of the B
         // operand behind the last one hold whatever the stage held: each is a
         // column of D of its own, and those columns are never used.
+        pdl_wait();
         const int xw = warp - kFsEpiWarps, items = nsteps * rows, k4 = lane * 4;
         auto fetch = [&](int i) {
             const int col = (kbeg + i / rows) * 128 + k4;
@@ -175,6 +221,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
         }
     } else {
         // scale and add: thread = weight row, registers = rows of x
+        pdl_wait();
         for (int s = 0; s < nsteps; ++s) {
             const int st = s % p.stages, b = s % L::kBufs;
             if (!mbar_wait_lanes(&H.tfull[b], (s / L::kBufs) & 1u, status)) break;
@@ -240,6 +287,218 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
     }
 }
 
+// ------------------------------------------------------------------ many rows
+constexpr int kFgEpiWarps = 8;       // warp w: TMEM lanes 32 (w % 4), column half w / 4
+constexpr int kFgProducerWarp = 8;
+constexpr int kFgMmaWarp = 9;
+constexpr int kFgThreads = 320;
+constexpr int kFgTmemCols = 512;
+
+struct FgParams {
+    CUtensorMap xmap;            // e4m3 x [rows][k], box [128 k, 128 rows]
+    CUtensorMap wmap;            // W [n][k], box [128 k, NW / 2]
+    const float* xs;             // [rows][groups]
+    const float* ws;             // [ceil(n / 128)][groups]
+    const void* bias;
+    void* y;
+    int64_t ldy;
+    int y_dtype, bias_dtype, yvec, early;
+    int rows, n, groups, ntiles, tiles;
+};
+
+template <int NW>
+struct FgLayout {
+    static constexpr int kA = 128 * 128, kB = NW / 2 * 128, kStage = kA + kB;
+    static constexpr int kStages = NW == 256 ? 6 : 8;
+    static constexpr int kBufs = kFgTmemCols / NW;
+    static constexpr int kCols = NW / 2;                   // columns of a thread
+    static constexpr int kSmem = 1024 + kStages * kStage + 512;
+};
+
+template <int NW>
+struct FgHead {
+    uint64_t full[FgLayout<NW>::kStages];      // in the pair's first CTA: both CTAs' bytes
+    uint64_t empty[FgLayout<NW>::kStages];
+    uint64_t tfull[FgLayout<NW>::kBufs];
+    uint64_t tempty[FgLayout<NW>::kBufs];      // in the pair's first CTA: both CTAs' epilogues
+    uint32_t tmem;
+};
+
+template <int NW>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_gemm_kernel(const __grid_constant__ FgParams p) {
+    using L = FgLayout<NW>;
+    extern __shared__ uint8_t fg_raw[];
+    uint8_t* ring = fg_raw + ((1024u - (smem_u32(fg_raw) & 1023u)) & 1023u);
+    FgHead<NW>& H = *reinterpret_cast<FgHead<NW>*>(ring + L::kStages * L::kStage);
+    static_assert(sizeof(FgHead<NW>) <= 512, "head must fit its slot");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = (int) blockIdx.x >> 1, pairs = (int) gridDim.x >> 1;
+    uint32_t* status = &g_fp8_status;
+
+    if (tid == 0) {
+        for (int s = 0; s < L::kStages; ++s) { mbar_init(&H.full[s], 1); mbar_init(&H.empty[s], 1); }
+        for (int b = 0; b < L::kBufs; ++b) { mbar_init(&H.tfull[b], 1); mbar_init(&H.tempty[b], 2 * kFgEpiWarps); }
+        fence_barrier_init();
+    }
+    if (warp == kFgMmaWarp) tmem_alloc_pair(&H.tmem, kFgTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = H.tmem;
+
+    if (warp == kFgProducerWarp) {
+        if (lane == 0) {
+            int it = 0, ahead = 0;
+            const int total = ((p.tiles - pair + pairs - 1) / pairs) * p.groups;     // steps of this pair
+            auto weights = [&](int st, int nt, int kb) {
+                if (rank == 0) mbar_arrive_expect_tx(&H.full[st], 2 * L::kStage);
+                tma_load_2d_pair(ring + st * L::kStage + L::kA, &p.wmap, kb * 128, nt * NW + (int) rank * (NW / 2),
+                                 mapa_u32(smem_u32(&H.full[st]), 0));
+            };
+            if (p.early) {
+                // weights ahead of the quantiser's end (it began after everything before this call)
+                const int nt = pair % p.ntiles;
+                for (; ahead < min(L::kStages, p.groups); ++ahead) weights(ahead, nt, ahead);
+            }
+            pdl_wait();
+            pdl_launch_dependents();
+            fence_proxy_async_global();
+            bool ok = true;
+            for (int t = pair; t < p.tiles && ok; t += pairs) {
+                const int nt = t % p.ntiles, row = t / p.ntiles * 256 + (int) rank * 128;
+                for (int kb = 0; kb < p.groups; ++kb, ++it) {
+                    const int st = it % L::kStages;
+                    if (it >= L::kStages) {
+                        ok = mbar_wait_cluster(&H.empty[st], ((it / L::kStages) + 1u) & 1u, status);
+                        if (!ok) break;
+                    }
+                    if (it >= ahead) weights(st, nt, kb);
+                    tma_load_2d_pair(ring + st * L::kStage, &p.xmap, kb * 128, row, mapa_u32(smem_u32(&H.full[st]), 0));
+                }
+            }
+            // no copy may still be in flight when the CTA retires: the pair's last MMAs have read every stage
+            for (int i = max(0, total - L::kStages); i < total && ok; ++i)
+                ok = mbar_wait_cluster(&H.empty[i % L::kStages], (i / L::kStages) & 1u, status);
+        } else {
+            pdl_wait();
+        }
+    } else if (warp == kFgMmaWarp) {
+        pdl_wait();
+        if (lane == 0 && rank == 0) {
+            const uint32_t id = idesc_f16(256, NW);
+            const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
+            int it = 0;
+            bool ok = true;
+            for (int t = pair; t < p.tiles && ok; t += pairs)
+                for (int kb = 0; kb < p.groups; ++kb, ++it) {
+                    const int st = it % L::kStages, b = it % L::kBufs;
+                    ok = mbar_wait_cluster(&H.full[st], (it / L::kStages) & 1u, status) &&
+                         mbar_wait_cluster(&H.tempty[b], ((it / L::kBufs) + 1u) & 1u, status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t ad = desc0 + (uint64_t) (st * (L::kStage >> 4)), bd = ad + (L::kA >> 4);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) tc_mma_f8_pair(tmem + b * NW, ad + 2 * q, bd + 2 * q, id, q);
+                    tc_commit_pair(&H.empty[st]);
+                    tc_commit_pair(&H.tfull[b]);
+                }
+        }
+    } else {
+        // scale and add: thread = row of x, registers = its half of the weight rows
+        pdl_wait();
+        const int half = warp >> 2, lg = warp & 3;
+        const uint32_t tcol = tmem + ((uint32_t) (lg * 32) << 16) + (uint32_t) (half * L::kCols);
+        uint32_t tempty0[L::kBufs];
+#pragma unroll
+        for (int b = 0; b < L::kBufs; ++b) tempty0[b] = mapa_u32(smem_u32(&H.tempty[b]), 0);
+        int it = 0;
+        bool ok = true;
+        for (int t = pair; t < p.tiles && ok; t += pairs) {
+            const int nt = t % p.ntiles;
+            const int row = t / p.ntiles * 256 + (int) rank * 128 + lg * 32 + lane;
+            const int col0 = nt * NW + half * L::kCols;
+            const bool live = row < p.rows, wlive = col0 < p.n;
+            const float* xs = p.xs + (int64_t) (live ? row : 0) * p.groups;
+            const float* ws = p.ws + (int64_t) (wlive ? col0 / 128 : 0) * p.groups;
+            uint64_t acc[L::kCols / 2];
+#pragma unroll
+            for (int j = 0; j < L::kCols / 2; ++j) acc[j] = 0ull;
+            float f = live && wlive ? __ldcg(xs) * __ldg(ws) : 0.f;
+            for (int kb = 0; kb < p.groups; ++kb, ++it) {
+                const int b = it % L::kBufs;
+                const uint64_t ff = pack_f32x2(f, f);
+                if (kb + 1 < p.groups) f = live && wlive ? __ldcg(xs + kb + 1) * __ldg(ws + kb + 1) : 0.f;
+                ok = mbar_wait_lanes(&H.tfull[b], (it / L::kBufs) & 1u, status);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < L::kCols / 32; ++c) {
+                    float v[32];
+                    tc_ld32(tcol + (uint32_t) (b * NW + c * 32), v);
+                    if (c + 1 == L::kCols / 32) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(tempty0[b]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) fma_f32x2(acc[c * 16 + j], v[2 * j], v[2 * j + 1], ff);
+                }
+            }
+            if (!ok || !live) continue;
+            const int64_t at = (int64_t) row * p.ldy + col0;
+#pragma unroll
+            for (int c = 0; c < L::kCols / 8; ++c) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 q = unpack_f32x2(acc[c * 4 + j]);
+                    v[2 * j] = q.x;
+                    v[2 * j + 1] = q.y;
+                }
+                const int col = col0 + c * 8;
+                if (col >= p.n) break;
+                if (p.bias != nullptr)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (col + j < p.n) v[j] += load_f32(p.bias, p.bias_dtype, col + j);
+                if (p.yvec && col + 8 <= p.n) {
+                    if (p.y_dtype == 2) {
+                        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + at + c * 8);
+                        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+                        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    } else {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (p.y_dtype == 0) {
+                                const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                            } else {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                        }
+                        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.y) + at + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (col + j < p.n) store_out(p.y, p.y_dtype, at + c * 8 + j, v[j]);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                                    // the pair's memory and barriers stay until both are done
+    if (warp == kFgMmaWarp) {
+        tc_fence_after();
+        tmem_free_pair(tmem, kFgTmemCols);
+    }
+}
+
 // ------------------------------------------------------------------ host side
 namespace {
 
@@ -277,22 +536,23 @@ int fp8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int6
 namespace {
 
 // CTAs that split k: the largest power of two (a portable cluster) that keeps
-// the grid within about two CTAs an SM and leaves every CTA two groups.
-int fs_cluster(int64_t tiles, int groups) {
+// the grid within what is resident at once and leaves every CTA two groups.
+int fs_cluster(int64_t tiles, int groups, int resident) {
     int s = 1;
-    while (s < kFsMaxCluster && tiles * s * 2 <= 296 && groups >= s * 4) s *= 2;
+    while (s < kFsMaxCluster && tiles * s * 2 <= resident && groups >= s * 4) s *= 2;
     return s;
 }
 
-template <int NT>
+template <int NT, bool PRE>
 int fs_launch(FsParams& p, cudaStream_t stream) {
     using L = FsLayout<NT>;
     const int64_t tiles = ((int64_t) p.n + 127) / 128, rtiles = ((int64_t) p.rows + NT - 1) / NT;
-    p.cluster = fs_cluster(tiles * rtiles, p.groups);
+    p.cluster = fs_cluster(tiles * rtiles, p.groups, NT <= 32 ? 296 : 148);
     const int steps = (p.groups + p.cluster - 1) / p.cluster;
-    // two CTAs share an SM: at most about 112 KB each; at least the partial sums' room
+    // two CTAs share an SM up to 32 rows: at most about 112 KB each; at least the partial sums' room
+    constexpr int kBudget = (NT <= 32 ? 112 : 200) * 1024;
     const int head = 1024 + (int) sizeof(FsHead<NT>);
-    int stages = (112 * 1024 - head) / L::kStage;
+    int stages = (kBudget - head) / L::kStage;
     if (stages > kFsMaxStages) stages = kFsMaxStages;
     const int least = (NT * 512 + L::kStage - 1) / L::kStage;
     if (stages > steps) stages = steps < least ? least : steps;
@@ -303,7 +563,7 @@ int fs_launch(FsParams& p, cudaStream_t stream) {
     EXL3_CUDA(cudaGetDevice(&dev));
     cudaError_t attr = cudaSuccess;
     std::call_once(once[dev & 63], [&] {
-        attr = cudaFuncSetAttribute(fp8_stream_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 116 * 1024);
+        attr = cudaFuncSetAttribute(fp8_stream_kernel<NT, PRE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
     });
     EXL3_CUDA(attr);
     EXL3_REQUIRE(tiles * p.cluster <= INT32_MAX && rtiles <= 65535, EXL3_ERR_UNSUPPORTED, "exl3_fp8_linear: matrix too large");
@@ -321,11 +581,52 @@ int fs_launch(FsParams& p, cudaStream_t stream) {
     at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    EXL3_CUDA(cudaLaunchKernelEx(&cfg, fp8_stream_kernel<NT>, p));
+    EXL3_CUDA(cudaLaunchKernelEx(&cfg, fp8_stream_kernel<NT, PRE>, p));
     return EXL3_OK;
 }
 
+template <int NW>
+int fg_launch(FgParams& p, int sms, cudaStream_t stream) {
+    using L = FgLayout<NW>;
+    static std::once_flag once[64];
+    int dev = 0;
+    EXL3_CUDA(cudaGetDevice(&dev));
+    cudaError_t attr = cudaSuccess;
+    std::call_once(once[dev & 63], [&] {
+        attr = cudaFuncSetAttribute(fp8_gemm_kernel<NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    });
+    EXL3_CUDA(attr);
+    const int64_t ntiles = ((int64_t) p.n + NW - 1) / NW, tiles = ntiles * (((int64_t) p.rows + 255) / 256);
+    EXL3_REQUIRE(tiles * p.groups <= INT32_MAX, EXL3_ERR_UNSUPPORTED, "exl3_fp8_linear: matrix too large");
+    p.ntiles = (int) ntiles;
+    p.tiles = (int) tiles;
+    const int pairs = (int) (tiles < sms / 2 ? tiles : sms / 2);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned) (2 * pairs));
+    cfg.blockDim = dim3(kFgThreads);
+    cfg.dynamicSmemBytes = (size_t) L::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    EXL3_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<NW>, p));
+    return EXL3_OK;
+}
+
+// Rows up to which the weights are the M operand and k is split: below, the
+// 256-row tiles of the pair kernel are too few to fill the GPU.
+constexpr int kFsInlineRows = 16;    // x quantised inside the kernel
+constexpr int kFsMaxRows = 192;
+
+int64_t fp8_ldq(int64_t k) { return (k + 15) / 16 * 16; }
+
 }  // namespace
+
+int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
+                        float* scale, int block_rows, bool pow2, cudaStream_t s);
+
 }  // namespace exl3
 
 extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const float* x_scale, int64_t rows, int64_t k,
@@ -343,25 +644,69 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
     EXL3_REQUIRE((x_dtype == EXL3_DTYPE_E4M3) == (x_scale != nullptr), EXL3_ERR_ARG,
                  "exl3_fp8_linear: x_scale goes with an e4m3 x, and only with one");
     EXL3_REQUIRE(aligned16(w) && ldw % 16 == 0, EXL3_ERR_ARG, "exl3_fp8_linear: weight rows must be 16-byte aligned");
-    (void) scratch;
-    (void) scratch_bytes;
+    auto s = static_cast<cudaStream_t>(stream);
+    const int groups = (int) ((k + 127) / 128);
+    const int es = x_dtype == 2 ? 4 : x_dtype == 3 ? 1 : 2;
+    int rc;
     FsParams p{};
-    const int rc = fp8_map(&p.wmap, w, n, k, ldw, 128, "exl3_fp8_linear");
-    if (rc != EXL3_OK) return rc;
     p.x = x; p.ldx = ldx; p.xs = x_scale; p.ws = w_scale; p.bias = bias; p.y = y; p.ldy = ldy;
     p.x_dtype = x_dtype; p.y_dtype = y_dtype; p.bias_dtype = bias_dtype; p.pow2 = pow2 != 0;
-    p.rows = (int) rows; p.n = (int) n; p.k = (int) k; p.groups = (int) ((k + 127) / 128);
-    const int es = x_dtype == 2 ? 4 : x_dtype == 3 ? 1 : 2;
+    p.rows = (int) rows; p.n = (int) n; p.k = (int) k; p.groups = groups;
     p.xvec = k % 4 == 0 && ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * es) == 0;
-    auto s = static_cast<cudaStream_t>(stream);
-    if (rows <= 16) return fs_launch<16>(p, s);
-    if (rows <= 32) return fs_launch<32>(p, s);
-    return fs_launch<64>(p, s);
+    if (rows <= kFsMaxRows && (rc = fp8_map(&p.wmap, w, n, k, ldw, 128, "exl3_fp8_linear")) != EXL3_OK) return rc;
+    if (rows <= kFsInlineRows) return fs_launch<16, false>(p, s);
+
+    // e4m3 rows that TMA can load: the caller's, or a copy / the quantised rows in the scratch
+    const void* xq = x;
+    int64_t ldq = ldx;
+    const float* xs = x_scale;
+    int early = 0;
+    if (x_dtype != EXL3_DTYPE_E4M3 || !aligned16(x) || ldx % 16 != 0) {
+        const int64_t need = exl3_fp8_linear_scratch_bytes(rows, k, n, x_dtype);
+        EXL3_REQUIRE(scratch && aligned16(scratch) && scratch_bytes >= need, EXL3_ERR_ARG,
+                     "exl3_fp8_linear: scratch must be 16-byte aligned and hold %lld bytes", (long long) need);
+        ldq = fp8_ldq(k);
+        xq = scratch;
+        if (x_dtype == EXL3_DTYPE_E4M3) {
+            EXL3_CUDA(cudaMemcpy2DAsync(scratch, (size_t) ldq, x, (size_t) ldx, (size_t) k, (size_t) rows, cudaMemcpyDeviceToDevice, s));
+        } else {
+            float* sc = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + align_up(rows * ldq, 256));
+            if ((rc = fp8_quantize_launch(x, x_dtype, rows, k, ldx, scratch, ldq, sc, 1, pow2 != 0, s)) != EXL3_OK) return rc;
+            xs = sc;
+            early = 1;
+        }
+    }
+    if (rows <= kFsMaxRows) {
+        const int nt = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+        if ((rc = fp8_map(&p.xmap, xq, rows, k, ldq, nt, "exl3_fp8_linear")) != EXL3_OK) return rc;
+        p.xs = xs;
+        p.early = early;
+        return nt == 32 ? fs_launch<32, true>(p, s) : nt == 64 ? fs_launch<64, true>(p, s) : fs_launch<128, true>(p, s);
+    }
+    int dev = 0;
+    EXL3_CUDA(cudaGetDevice(&dev));
+    DeviceInfo di;
+    if ((rc = device_info(dev, &di)) != EXL3_OK) return rc;
+    // Weight rows of a tile: 256 unless tiles of 128 fill the pairs of SMs enough
+    // better to pay for loading x twice as often.
+    const int64_t pairs = di.sms / 2, mt = (rows + 255) / 256;
+    const int64_t c256 = (mt * ((n + 255) / 256) + pairs - 1) / pairs * 20, c128 = (mt * ((n + 127) / 128) + pairs - 1) / pairs * 13;
+    const int nw = c128 < c256 ? 128 : 256;
+    FgParams g{};
+    if ((rc = fp8_map(&g.xmap, xq, rows, k, ldq, 128, "exl3_fp8_linear")) != EXL3_OK) return rc;
+    if ((rc = fp8_map(&g.wmap, w, n, k, ldw, nw / 2, "exl3_fp8_linear")) != EXL3_OK) return rc;
+    g.xs = xs; g.ws = w_scale; g.bias = bias; g.y = y; g.ldy = ldy;
+    g.y_dtype = y_dtype; g.bias_dtype = bias_dtype; g.early = early;
+    g.yvec = aligned16(y) && ldy % (y_dtype == 2 ? 4 : 8) == 0;
+    g.rows = (int) rows; g.n = (int) n; g.groups = groups;
+    return nw == 128 ? fg_launch<128>(g, di.sms, s) : fg_launch<256>(g, di.sms, s);
 }
 
 extern "C" int64_t exl3_fp8_linear_scratch_bytes(int64_t rows, int64_t k, int64_t n, int x_dtype) {
+    using namespace exl3;
     if (rows < 0 || k < 1 || n < 1 || x_dtype < 0 || x_dtype > 3) return -1;
-    return 0;
+    if (rows <= kFsInlineRows) return 0;
+    return align_up(rows * fp8_ldq(k), 256) + (x_dtype == EXL3_DTYPE_E4M3 ? 0 : rows * ((k + 127) / 128) * 4);
 }
 
 extern "C" int exl3_fp8_status(int clear, uint32_t* status, void* stream) {

@@ -74,6 +74,7 @@ template <int DT>
 __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(
     const void* x, int64_t ldx, int64_t rows, int cols, uint8_t* q, int64_t ldq, float* scale, bool pow2, bool fast) {
     using V = QuantVec<DT>;
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int groups = (cols + kFp8Block - 1) / kFp8Block;
     constexpr int GP = 32 / V::LANES;                      // groups in an item
