@@ -125,7 +125,45 @@ __device__ __forceinline__ void unpack4(const uint4& raw, int dtype, float (&v)[
     }
 }
 
+// ---------------------------------------------------------------- waits
+// mbar_wait (2 s, then the ring-timeout bit) for pipelines whose steps take a
+// fraction of a microsecond: the clock is read once in 256 polls only, because
+// a read of %globaltimer takes about as long as such a step.
+static __device__ __noinline__ bool poll_expired(uint64_t& t0) {
+    const uint64_t t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    return t - t0 > kWaitLimitNs;
+}
+
+__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, uint32_t* status) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 0; i < kSpinCap; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255u) == 255u && poll_expired(t0)) break;
+    }
+    set_error(status, ERR_RING_TIMEOUT);
+    return false;
+}
+
+// Polled by every lane of a warp, with one verdict for the warp.
+__device__ __forceinline__ bool mbar_poll_lanes(uint64_t* bar, uint32_t parity, uint32_t* status) {
+    return __all_sync(0xffffffffu, mbar_poll(bar, parity, status));
+}
+
 // ---------------------------------------------------------------- tensor core
+// The MMA loop runs in all lanes of its warp and one elected lane issues: the
+// descriptors then stay in uniform registers.  Issued from inside `if (lane ==
+// 0)`, four MMAs and two commits took 870 clocks, more than the MMAs
+// themselves (256 x 256 x 32 each: 128 clocks).
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+
+// Warp index as the compiler sees it: the same in all lanes.
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int) (threadIdx.x >> 5), 0); }
+
 // D[128 x N] (+)= A . B^T of 8-bit operands, K = 32 per instruction, fp32
 // accumulation; the instruction descriptor has the layout of kind::f16 with
 // e4m3 as format 0.
@@ -164,6 +202,33 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, in
         :: "r"(smem_u32(dst)), "l"(tmap), "r"(c0), "r"(c1), "r"(bar) : "memory");
 }
 
+// 32 lanes x 32-bit, 32 consecutive columns per thread: the load, and the wait
+// for all of this thread's loads, which owns the registers until then.
+__device__ __forceinline__ void tc_ld32_issue(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
+}
+
+__device__ __forceinline__ void tc_ld32_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
+}
+
+// Register split of a launch of 384 threads at 168 registers (64,512): two
+// warpgroups raised to 232, one lowered to 40 -- 256 * 232 + 128 * 40 = 64,512.
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 232;"); }
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 40;"); }
+
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_dst, uint32_t cols) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                  :: "r"(smem_u32(smem_dst)), "r"(cols) : "memory");
@@ -172,23 +237,6 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_dst, uint32_t col
 
 __device__ __forceinline__ void tmem_free_pair(uint32_t taddr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(taddr), "r"(cols) : "memory");
-}
-
-// Packed fp32: (a.x * f + c.x, a.y * f + c.y).
-__device__ __forceinline__ void fma_f32x2(uint64_t& c, float ax, float ay, uint64_t ff) {
-    asm("{\n\t.reg .b64 a;\n\tmov.b64 a, {%1, %2};\n\tfma.rn.f32x2 %0, a, %3, %0;\n\t}" : "+l"(c) : "f"(ax), "f"(ay), "l"(ff));
-}
-
-__device__ __forceinline__ uint64_t pack_f32x2(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-
-__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
 }
 
 // ---------------------------------------------------------------- clusters
@@ -209,24 +257,13 @@ __device__ __forceinline__ uint32_t mapa_u32(uint32_t addr, uint32_t rank) {
     return a;
 }
 
+// Arrival on a barrier of any CTA of the cluster.  It hands over TMEM columns
+// that have been read into registers (tcgen05.fence::before_thread_sync comes
+// before it) and no memory, so it has CTA scope: a release at cluster scope
+// waits for every load in flight and was the largest stall of the pair kernel
+// (2048 x 4096 x 4096: 107 us with it).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(addr) : "memory");
-}
-
-// mbar_wait that also acquires what other CTAs of the cluster released.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* status) {
-    const uint64_t t0 = globaltimer_ns();
-    for (uint32_t i = 0; i < kSpinCap; ++i) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\t"
-                     "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 20000;\n\t"
-                     "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-        if (ok) return true;
-        if (globaltimer_ns() - t0 > kWaitLimitNs) break;
-    }
-    set_error(status, ERR_RING_TIMEOUT);
-    return false;
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(addr) : "memory");
 }
 
 // fp32 at shared-memory address `addr` (of this CTA's layout) in CTA `rank` of the cluster.

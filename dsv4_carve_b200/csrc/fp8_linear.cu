@@ -20,7 +20,7 @@
 // kernel of its own (launched just before, overlapped) and its rows are the M
 // operand of a pair of CTAs (cta_group::2, 256 rows x NW weight rows), so the
 // factor s_x * s_w is one number a thread for each group of 128 columns and
-// the scaling is one packed fp32 FMA for two values.
+// the scaling is one FMA a value.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
     extern __shared__ uint8_t fs_raw[];
     uint8_t* ring = fs_raw + ((1024u - (smem_u32(fs_raw) & 1023u)) & 1023u);
     FsHead<NT>& H = *reinterpret_cast<FsHead<NT>*>(ring + p.stages * L::kStage);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const int S = p.cluster, rank = S > 1 ? (int) cluster_rank() : 0;
     const int tile = (int) blockIdx.x / S;
     const int n0 = tile * 128, row0 = (int) blockIdx.y * NT;
@@ -149,15 +149,15 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
         }
     } else if (warp == kFsMmaWarp) {
         pdl_wait();
-        if (lane == 0) {
-            const uint32_t id = idesc_f16(128, ncols);
-            const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
-            for (int s = 0; s < nsteps; ++s) {
-                const int st = s % p.stages, b = s % L::kBufs;
-                if (!mbar_wait(&H.full[st], (s / p.stages) & 1u, status)) break;
-                if (!mbar_wait(&H.tempty[b], ((s / L::kBufs) + 1u) & 1u, status)) break;
-                tc_fence_after();
-                const uint64_t wd = desc0 + (uint64_t) (st * (L::kStage >> 4)), xd = wd + (kFp8WTile >> 4);
+        const uint32_t id = idesc_f16(128, ncols);
+        const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
+        for (int s = 0; s < nsteps; ++s) {
+            const int st = s % p.stages, b = s % L::kBufs;
+            if (!mbar_wait_lanes(&H.full[st], (s / p.stages) & 1u, status)) break;
+            if (!mbar_wait_lanes(&H.tempty[b], ((s / L::kBufs) + 1u) & 1u, status)) break;
+            tc_fence_after();
+            const uint64_t wd = desc0 + (uint64_t) (st * (L::kStage >> 4)), xd = wd + (kFp8WTile >> 4);
+            if (elect_lane()) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) tc_mma_f8(tmem + b * NT, wd + 2 * q, xd + 2 * q, id, q);
                 tc_commit(&H.empty[st]);
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
 constexpr int kFgEpiWarps = 8;       // warp w: TMEM lanes 32 (w % 4), column half w / 4
 constexpr int kFgProducerWarp = 8;
 constexpr int kFgMmaWarp = 9;
-constexpr int kFgThreads = 320;
+constexpr int kFgThreads = 384;      // warps 10, 11 fill the third warpgroup
 constexpr int kFgTmemCols = 512;
 
 struct FgParams {
@@ -331,7 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
     uint8_t* ring = fg_raw + ((1024u - (smem_u32(fg_raw) & 1023u)) & 1023u);
     FgHead<NW>& H = *reinterpret_cast<FgHead<NW>*>(ring + L::kStages * L::kStage);
     static_assert(sizeof(FgHead<NW>) <= 512, "head must fit its slot");
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const uint32_t rank = cluster_rank();
     const int pair = (int) blockIdx.x >> 1, pairs = (int) gridDim.x >> 1;
     uint32_t* status = &g_fp8_status;
@@ -349,6 +349,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
     const uint32_t tmem = H.tmem;
 
     if (warp == kFgProducerWarp) {
+        regs_down();
         if (lane == 0) {
             int it = 0, ahead = 0;
             const int total = ((p.tiles - pair + pairs - 1) / pairs) * p.groups;     // steps of this pair
@@ -371,7 +372,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
                 for (int kb = 0; kb < p.groups; ++kb, ++it) {
                     const int st = it % L::kStages;
                     if (it >= L::kStages) {
-                        ok = mbar_wait_cluster(&H.empty[st], ((it / L::kStages) + 1u) & 1u, status);
+                        ok = mbar_poll(&H.empty[st], ((it / L::kStages) + 1u) & 1u, status);
                         if (!ok) break;
                     }
                     if (it >= ahead) weights(st, nt, kb);
@@ -380,13 +381,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
             }
             // no copy may still be in flight when the CTA retires: the pair's last MMAs have read every stage
             for (int i = max(0, total - L::kStages); i < total && ok; ++i)
-                ok = mbar_wait_cluster(&H.empty[i % L::kStages], (i / L::kStages) & 1u, status);
+                ok = mbar_poll(&H.empty[i % L::kStages], (i / L::kStages) & 1u, status);
         } else {
             pdl_wait();
         }
     } else if (warp == kFgMmaWarp) {
+        regs_down();
         pdl_wait();
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             const uint32_t id = idesc_f16(256, NW);
             const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
             int it = 0;
@@ -394,25 +396,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
             for (int t = pair; t < p.tiles && ok; t += pairs)
                 for (int kb = 0; kb < p.groups; ++kb, ++it) {
                     const int st = it % L::kStages, b = it % L::kBufs;
-                    ok = mbar_wait_cluster(&H.full[st], (it / L::kStages) & 1u, status) &&
-                         mbar_wait_cluster(&H.tempty[b], ((it / L::kBufs) + 1u) & 1u, status);
+                    ok = mbar_poll_lanes(&H.full[st], (it / L::kStages) & 1u, status) &&
+                         mbar_poll_lanes(&H.tempty[b], ((it / L::kBufs) + 1u) & 1u, status);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t ad = desc0 + (uint64_t) (st * (L::kStage >> 4)), bd = ad + (L::kA >> 4);
+                    if (elect_lane()) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) tc_mma_f8_pair(tmem + b * NW, ad + 2 * q, bd + 2 * q, id, q);
-                    tc_commit_pair(&H.empty[st]);
-                    tc_commit_pair(&H.tfull[b]);
+                        for (int q = 0; q < 4; ++q) tc_mma_f8_pair(tmem + b * NW, ad + 2 * q, bd + 2 * q, id, q);
+                        tc_commit_pair(&H.empty[st]);
+                        tc_commit_pair(&H.tfull[b]);
+                    }
                 }
         }
+    } else if (warp > kFgMmaWarp) {
+        regs_down();
     } else {
         // scale and add: thread = row of x, registers = its half of the weight rows
+        regs_up();
         pdl_wait();
         const int half = warp >> 2, lg = warp & 3;
         const uint32_t tcol = tmem + ((uint32_t) (lg * 32) << 16) + (uint32_t) (half * L::kCols);
-        uint32_t tempty0[L::kBufs];
-#pragma unroll
-        for (int b = 0; b < L::kBufs; ++b) tempty0[b] = mapa_u32(smem_u32(&H.tempty[b]), 0);
+        const uint32_t tempty0 = mapa_u32(smem_u32(&H.tempty[0]), 0);
         int it = 0;
         bool ok = true;
         for (int t = pair; t < p.tiles && ok; t += pairs) {
@@ -422,28 +427,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
             const bool live = row < p.rows, wlive = col0 < p.n;
             const float* xs = p.xs + (int64_t) (live ? row : 0) * p.groups;
             const float* ws = p.ws + (int64_t) (wlive ? col0 / 128 : 0) * p.groups;
-            uint64_t acc[L::kCols / 2];
+            float acc[L::kCols];
 #pragma unroll
-            for (int j = 0; j < L::kCols / 2; ++j) acc[j] = 0ull;
-            float f = live && wlive ? __ldcg(xs) * __ldg(ws) : 0.f;
+            for (int j = 0; j < L::kCols; ++j) acc[j] = 0.f;
+            // scales two steps ahead: a step is shorter than a load from L2
+            auto scales = [&](int kb) { return live && wlive && kb < p.groups ? make_float2(__ldcg(xs + kb), __ldg(ws + kb)) : make_float2(0.f, 0.f); };
+            float2 s0 = scales(0), s1 = scales(1);
             for (int kb = 0; kb < p.groups; ++kb, ++it) {
                 const int b = it % L::kBufs;
-                const uint64_t ff = pack_f32x2(f, f);
-                if (kb + 1 < p.groups) f = live && wlive ? __ldcg(xs + kb + 1) * __ldg(ws + kb + 1) : 0.f;
-                ok = mbar_wait_lanes(&H.tfull[b], (it / L::kBufs) & 1u, status);
+                const float f = s0.x * s0.y;
+                s0 = s1;
+                s1 = scales(kb + 2);
+                ok = mbar_poll_lanes(&H.tfull[b], (it / L::kBufs) & 1u, status);
                 if (!ok) break;
                 tc_fence_after();
+                // the next 32 columns are on their way while these are scaled
+                constexpr int NC = L::kCols / 32;
+                uint32_t v[2][32];
+                tc_ld32_issue(tcol + (uint32_t) (b * NW), v[0]);
 #pragma unroll
-                for (int c = 0; c < L::kCols / 32; ++c) {
-                    float v[32];
-                    tc_ld32(tcol + (uint32_t) (b * NW + c * 32), v);
-                    if (c + 1 == L::kCols / 32) {
+                for (int c = 0; c < NC; ++c) {
+                    tc_ld32_wait(v[c & 1]);
+                    if (c + 1 < NC) {
+                        tc_ld32_issue(tcol + (uint32_t) (b * NW + (c + 1) * 32), v[(c + 1) & 1]);
+                    } else {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(tempty0[b]);
+                        if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * (uint32_t) b);
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) fma_f32x2(acc[c * 16 + j], v[2 * j], v[2 * j + 1], ff);
+                    for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[c & 1][j]), f, acc[c * 32 + j]);
                 }
             }
             if (!ok || !live) continue;
@@ -452,11 +465,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
             for (int c = 0; c < L::kCols / 8; ++c) {
                 float v[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 q = unpack_f32x2(acc[c * 4 + j]);
-                    v[2 * j] = q.x;
-                    v[2 * j + 1] = q.y;
-                }
+                for (int j = 0; j < 8; ++j) v[j] = acc[c * 8 + j];
                 const int col = col0 + c * 8;
                 if (col >= p.n) break;
                 if (p.bias != nullptr)

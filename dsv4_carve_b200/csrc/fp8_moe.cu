@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
     uint8_t* ring = fm_raw + ((1024u - (smem_u32(fm_raw) & 1023u)) & 1023u);
     FmHead<NT>& S = *reinterpret_cast<FmHead<NT>*>(ring + p.stages * L::kStage);
     float* oacc = reinterpret_cast<float*>(ring + p.stages * L::kStage + sizeof(FmHead<NT>));    // PH 1: [m][128]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const int C = (int) gridDim.x, cta = (int) blockIdx.x;
     const int NBI = p.I / 128, NBH = p.H / 128, KB = PH == 0 ? NBH : NBI;
     uint32_t* status = p.ctrl + 2;
@@ -252,17 +252,17 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
             pdl_wait();
         }
     } else if (warp == kFmMmaWarp) {
-        if (lane == 0) {
-            const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
-            FmAt<PH> a(beg, max(G, 1), NBI, KB);
-            for (int s = 0; s < nsteps; ++s, a.next()) {
-                const int st = s % sm, b = s % L::kBufs;
-                const int n = P.gstart[a.g + 1] - P.gstart[a.g];
-                const uint32_t id = idesc_f16(128, (n + 15) & ~15);
-                if (!mbar_wait(&S.full[st], (s / sm) & 1u, status)) break;
-                if (!mbar_wait(&S.tempty[b], ((s / L::kBufs) + 1u) & 1u, status)) break;
-                tc_fence_after();
-                const uint64_t wd = desc0 + (uint64_t) (st * (L::kStage >> 4)), xd = wd + (L::kW >> 4);
+        const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
+        FmAt<PH> a(beg, max(G, 1), NBI, KB);
+        for (int s = 0; s < nsteps; ++s, a.next()) {
+            const int st = s % sm, b = s % L::kBufs;
+            const int n = P.gstart[a.g + 1] - P.gstart[a.g];
+            const uint32_t id = __shfl_sync(0xffffffffu, idesc_f16(128, (n + 15) & ~15), 0);
+            if (!mbar_wait_lanes(&S.full[st], (s / sm) & 1u, status)) break;
+            if (!mbar_wait_lanes(&S.tempty[b], ((s / L::kBufs) + 1u) & 1u, status)) break;
+            tc_fence_after();
+            const uint64_t wd = desc0 + (uint64_t) (st * (L::kStage >> 4)), xd = wd + (L::kW >> 4);
+            if (elect_lane()) {
 #pragma unroll
                 for (int mat = 0; mat < kMats; ++mat)
 #pragma unroll
