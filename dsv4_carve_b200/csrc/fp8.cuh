@@ -150,6 +150,14 @@ __device__ __forceinline__ bool mbar_poll_lanes(uint64_t* bar, uint32_t parity, 
     return __all_sync(0xffffffffu, mbar_poll(bar, parity, status));
 }
 
+// Two phases at once: both looks are in flight together, so that a loop whose
+// barriers have completed pays for one of them.
+__device__ __forceinline__ bool mbar_poll2_lanes(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, uint32_t* status) {
+    const bool ra = mbar_try_wait(a, pa), rb = mbar_try_wait(b, pb);
+    if (__all_sync(0xffffffffu, ra && rb)) return true;
+    return mbar_poll_lanes(a, pa, status) && mbar_poll_lanes(b, pb, status);
+}
+
 // ---------------------------------------------------------------- tensor core
 // The MMA loop runs in all lanes of its warp and one elected lane issues: the
 // descriptors then stay in uniform registers.  Issued from inside `if (lane ==

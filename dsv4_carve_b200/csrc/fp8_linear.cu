@@ -48,7 +48,8 @@ struct FsParams {
     CUtensorMap xmap;            // PRE: e4m3 x [rows][k], box [128 k, NT]
     const void* x;
     int64_t ldx;
-    const float* xs;             // scales of an e4m3 x [rows][groups], else null
+    const float* xs;             // scales of an e4m3 x: xs[row * xsr + group * xsg], else null
+    int64_t xsr, xsg;
     const float* ws;             // [ceil(n / 128)][groups]
     const void* bias;
     void* y;
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
 #pragma unroll
             for (int h = 0; h < (NT + 31) / 32; ++h) {
                 const int j = h * 32 + lane;
-                f[h] = j < rows ? __ldcg(p.xs + (int64_t) (row0 + j) * p.groups + kbeg + s) * ws : 0.f;
+                f[h] = j < rows ? __ldcg(p.xs + (row0 + j) * p.xsr + (kbeg + s) * p.xsg) * ws : 0.f;
             }
             if (!mbar_wait_lanes(&H.empty[st], ((s / p.stages) + 1u) & 1u, status)) break;
 #pragma unroll
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
             uint32_t q;
             if (p.x_dtype == kDtE4M3) {
                 q = raw.x;
-                sx = __ldg(p.xs + (int64_t) (row0 + r) * p.groups + kbeg + s);
+                sx = __ldg(p.xs + (row0 + r) * p.xsr + (kbeg + s) * p.xsg);
             } else {
                 float v[4];
                 unpack4(raw, p.x_dtype, v);
@@ -297,11 +298,11 @@ constexpr int kFgTmemCols = 512;
 struct FgParams {
     CUtensorMap xmap;            // e4m3 x [rows][k], box [128 k, 128 rows]
     CUtensorMap wmap;            // W [n][k], box [128 k, NW / 2]
-    const float* xs;             // [rows][groups]
+    const float* xs;             // xs[row * xsr + group * xsg]
     const float* ws;             // [ceil(n / 128)][groups]
     const void* bias;
     void* y;
-    int64_t ldy;
+    int64_t ldy, xsr, xsg;
     int y_dtype, bias_dtype, yvec, early;
     int rows, n, groups, ntiles, tiles;
 };
@@ -309,17 +310,21 @@ struct FgParams {
 template <int NW>
 struct FgLayout {
     static constexpr int kA = 128 * 128, kB = NW / 2 * 128, kStage = kA + kB;
-    static constexpr int kStages = NW == 256 ? 6 : 8;
+    static constexpr int kStages = NW == 256 ? 5 : 6;
     static constexpr int kBufs = kFgTmemCols / NW;
     static constexpr int kCols = NW / 2;                   // columns of a thread
-    static constexpr int kSmem = 1024 + kStages * kStage + 512;
+    static constexpr int kOut = 32 * 256;                  // 256 bytes of a warp's rows on their way out
+    static constexpr int kSmem = 1024 + kStages * kStage + kFgEpiWarps * kOut + 512;
 };
+
+// Byte offset of 16-byte piece c of row r in a warp's output buffer: pieces are
+// permuted in each row so that neither rows nor pieces meet in a bank.
+__device__ __forceinline__ int fg_out(int r, int c) { return r * 256 + ((c ^ (r & 7)) << 4); }
 
 template <int NW>
 struct FgHead {
     uint64_t full[FgLayout<NW>::kStages];      // in the pair's first CTA: both CTAs' bytes
-    uint64_t empty[FgLayout<NW>::kStages];
-    uint64_t tfull[FgLayout<NW>::kBufs];
+    uint64_t done[FgLayout<NW>::kStages];      // the stage's MMAs: it may be refilled, and its sums be read
     uint64_t tempty[FgLayout<NW>::kBufs];      // in the pair's first CTA: both CTAs' epilogues
     uint32_t tmem;
 };
@@ -329,7 +334,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
     using L = FgLayout<NW>;
     extern __shared__ uint8_t fg_raw[];
     uint8_t* ring = fg_raw + ((1024u - (smem_u32(fg_raw) & 1023u)) & 1023u);
-    FgHead<NW>& H = *reinterpret_cast<FgHead<NW>*>(ring + L::kStages * L::kStage);
+    uint8_t* stage_out = ring + L::kStages * L::kStage;
+    FgHead<NW>& H = *reinterpret_cast<FgHead<NW>*>(stage_out + kFgEpiWarps * L::kOut);
     static_assert(sizeof(FgHead<NW>) <= 512, "head must fit its slot");
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const uint32_t rank = cluster_rank();
@@ -337,8 +343,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
     uint32_t* status = &g_fp8_status;
 
     if (tid == 0) {
-        for (int s = 0; s < L::kStages; ++s) { mbar_init(&H.full[s], 1); mbar_init(&H.empty[s], 1); }
-        for (int b = 0; b < L::kBufs; ++b) { mbar_init(&H.tfull[b], 1); mbar_init(&H.tempty[b], 2 * kFgEpiWarps); }
+        for (int s = 0; s < L::kStages; ++s) { mbar_init(&H.full[s], 1); mbar_init(&H.done[s], 1); }
+        for (int b = 0; b < L::kBufs; ++b) mbar_init(&H.tempty[b], 2 * kFgEpiWarps);
         fence_barrier_init();
     }
     if (warp == kFgMmaWarp) tmem_alloc_pair(&H.tmem, kFgTmemCols);
@@ -346,7 +352,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
     __syncthreads();
     cluster_sync_all();
     tc_fence_after();
-    const uint32_t tmem = H.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, H.tmem, 0);
 
     if (warp == kFgProducerWarp) {
         regs_down();
@@ -372,7 +378,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
                 for (int kb = 0; kb < p.groups; ++kb, ++it) {
                     const int st = it % L::kStages;
                     if (it >= L::kStages) {
-                        ok = mbar_poll(&H.empty[st], ((it / L::kStages) + 1u) & 1u, status);
+                        ok = mbar_poll(&H.done[st], ((it / L::kStages) + 1u) & 1u, status);
                         if (!ok) break;
                     }
                     if (it >= ahead) weights(st, nt, kb);
@@ -381,7 +387,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
             }
             // no copy may still be in flight when the CTA retires: the pair's last MMAs have read every stage
             for (int i = max(0, total - L::kStages); i < total && ok; ++i)
-                ok = mbar_poll(&H.empty[i % L::kStages], (i / L::kStages) & 1u, status);
+                ok = mbar_poll(&H.done[i % L::kStages], (i / L::kStages) & 1u, status);
         } else {
             pdl_wait();
         }
@@ -396,16 +402,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
             for (int t = pair; t < p.tiles && ok; t += pairs)
                 for (int kb = 0; kb < p.groups; ++kb, ++it) {
                     const int st = it % L::kStages, b = it % L::kBufs;
-                    ok = mbar_poll_lanes(&H.full[st], (it / L::kStages) & 1u, status) &&
-                         mbar_poll_lanes(&H.tempty[b], ((it / L::kBufs) + 1u) & 1u, status);
+                    ok = mbar_poll2_lanes(&H.full[st], (it / L::kStages) & 1u, &H.tempty[b], ((it / L::kBufs) + 1u) & 1u, status);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t ad = desc0 + (uint64_t) (st * (L::kStage >> 4)), bd = ad + (L::kA >> 4);
                     if (elect_lane()) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q) tc_mma_f8_pair(tmem + b * NW, ad + 2 * q, bd + 2 * q, id, q);
-                        tc_commit_pair(&H.empty[st]);
-                        tc_commit_pair(&H.tfull[b]);
+                        tc_commit_pair(&H.done[st]);
                     }
                 }
         }
@@ -425,20 +429,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
             const int row = t / p.ntiles * 256 + (int) rank * 128 + lg * 32 + lane;
             const int col0 = nt * NW + half * L::kCols;
             const bool live = row < p.rows, wlive = col0 < p.n;
-            const float* xs = p.xs + (int64_t) (live ? row : 0) * p.groups;
+            const float* xs = p.xs + (live ? row : 0) * p.xsr;
             const float* ws = p.ws + (int64_t) (wlive ? col0 / 128 : 0) * p.groups;
             float acc[L::kCols];
 #pragma unroll
             for (int j = 0; j < L::kCols; ++j) acc[j] = 0.f;
             // scales two steps ahead: a step is shorter than a load from L2
-            auto scales = [&](int kb) { return live && wlive && kb < p.groups ? make_float2(__ldcg(xs + kb), __ldg(ws + kb)) : make_float2(0.f, 0.f); };
+            auto scales = [&](int kb) { return live && wlive && kb < p.groups ? make_float2(__ldcg(xs + kb * p.xsg), __ldg(ws + kb)) : make_float2(0.f, 0.f); };
             float2 s0 = scales(0), s1 = scales(1);
             for (int kb = 0; kb < p.groups; ++kb, ++it) {
                 const int b = it % L::kBufs;
                 const float f = s0.x * s0.y;
                 s0 = s1;
                 s1 = scales(kb + 2);
-                ok = mbar_poll_lanes(&H.tfull[b], (it / L::kBufs) & 1u, status);
+                ok = mbar_poll_lanes(&H.done[it % L::kStages], (it / L::kStages) & 1u, status);
                 if (!ok) break;
                 tc_fence_after();
                 // the next 32 columns are on their way while these are scaled
@@ -459,42 +463,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
                     for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[c & 1][j]), f, acc[c * 32 + j]);
                 }
             }
-            if (!ok || !live) continue;
-            const int64_t at = (int64_t) row * p.ldy + col0;
+            if (!ok) break;
+            // Out through shared memory, 256 bytes of each row at a time, so that
+            // a warp stores whole rows' pieces: written straight from the
+            // registers (a row a lane) a tile took 8000 clocks.
+            const int es = p.y_dtype == 2 ? 4 : 2;
+            uint8_t* buf = stage_out + warp * L::kOut;
+            const int wrow = t / p.ntiles * 256 + (int) rank * 128 + lg * 32;
+            if (p.bias != nullptr) {
 #pragma unroll
-            for (int c = 0; c < L::kCols / 8; ++c) {
-                float v[8];
+                for (int j = 0; j < L::kCols; ++j)
+                    if (col0 + j < p.n) acc[j] += load_f32(p.bias, p.bias_dtype, col0 + j);
+            }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = acc[c * 8 + j];
-                const int col = col0 + c * 8;
-                if (col >= p.n) break;
-                if (p.bias != nullptr)
+            for (int h = 0; h < 2; ++h) {
+                // 16-bit types: all kCols at once in pass 0; fp32: 64 in each pass
+                const int cols = es == 4 ? 64 : L::kCols;
+                if (h * cols >= L::kCols) break;
+                __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (col + j < p.n) v[j] += load_f32(p.bias, p.bias_dtype, col + j);
-                if (p.yvec && col + 8 <= p.n) {
-                    if (p.y_dtype == 2) {
-                        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + at + c * 8);
-                        o[0] = make_float4(v[0], v[1], v[2], v[3]);
-                        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+                for (int c = 0; c < 16; ++c) {
+                    uint4 w;
+                    if (es == 4) {
+                        if (h * 64 + c * 4 + 3 >= L::kCols) break;
+                        w = make_uint4(__float_as_uint(acc[h * 64 + c * 4]), __float_as_uint(acc[h * 64 + c * 4 + 1]),
+                                       __float_as_uint(acc[h * 64 + c * 4 + 2]), __float_as_uint(acc[h * 64 + c * 4 + 3]));
                     } else {
-                        uint32_t w[4];
+                        if (c * 8 + 7 >= L::kCols || h > 0) break;
+                        uint32_t q[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
+                            const float lo = acc[c * 8 + 2 * j], hi = acc[c * 8 + 2 * j + 1];
                             if (p.y_dtype == 0) {
-                                const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                                const __half2 v = __floats2half2_rn(lo, hi);
+                                q[j] = *reinterpret_cast<const uint32_t*>(&v);
                             } else {
-                                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-                                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                                const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+                                q[j] = *reinterpret_cast<const uint32_t*>(&v);
                             }
                         }
-                        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.y) + at + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                        w = make_uint4(q[0], q[1], q[2], q[3]);
+                    }
+                    *reinterpret_cast<uint4*>(buf + fg_out(lane, c)) = w;
+                }
+                __syncwarp();
+                const int c0 = col0 + h * cols, left = min(cols, p.n - c0);       // columns of this pass
+                if (left <= 0) continue;
+                const int rows = min(32, p.rows - wrow);
+                uint8_t* y = static_cast<uint8_t*>(p.y) + ((int64_t) wrow * p.ldy + c0) * es;
+                if (p.yvec && (left * es) % 16 == 0) {
+                    const int per = left * es / 16;                               // 16-byte pieces of a row: 1 .. 16
+                    if (per == 16) {
+                        for (int i = lane; i < rows * 16; i += 32)
+                            *reinterpret_cast<uint4*>(y + (int64_t) (i >> 4) * p.ldy * es + (i & 15) * 16) =
+                                *reinterpret_cast<const uint4*>(buf + fg_out(i >> 4, i & 15));
+                    } else {
+                        for (int i = lane; i < rows * per; i += 32)
+                            *reinterpret_cast<uint4*>(y + (int64_t) (i / per) * p.ldy * es + (i % per) * 16) =
+                                *reinterpret_cast<const uint4*>(buf + fg_out(i / per, i % per));
                     }
                 } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (col + j < p.n) store_out(p.y, p.y_dtype, at + c * 8 + j, v[j]);
+                    for (int r = 0; r < rows; ++r)
+                        for (int j = lane; j < left; j += 32) {
+                            if (es == 4) reinterpret_cast<uint32_t*>(y + (int64_t) r * p.ldy * 4)[j] = *reinterpret_cast<const uint32_t*>(buf + fg_out(r, j >> 2) + (j & 3) * 4);
+                            else reinterpret_cast<uint16_t*>(y + (int64_t) r * p.ldy * 2)[j] = *reinterpret_cast<const uint16_t*>(buf + fg_out(r, j >> 3) + (j & 7) * 2);
+                        }
                 }
             }
         }
@@ -634,7 +667,7 @@ int64_t fp8_ldq(int64_t k) { return (k + 15) / 16 * 16; }
 }  // namespace
 
 int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
-                        float* scale, int block_rows, bool pow2, cudaStream_t s);
+                        float* scale, int64_t sr, int64_t sg, int block_rows, bool pow2, cudaStream_t s);
 
 }  // namespace exl3
 
@@ -658,7 +691,7 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
     const int es = x_dtype == 2 ? 4 : x_dtype == 3 ? 1 : 2;
     int rc;
     FsParams p{};
-    p.x = x; p.ldx = ldx; p.xs = x_scale; p.ws = w_scale; p.bias = bias; p.y = y; p.ldy = ldy;
+    p.x = x; p.ldx = ldx; p.xs = x_scale; p.xsr = groups; p.xsg = 1; p.ws = w_scale; p.bias = bias; p.y = y; p.ldy = ldy;
     p.x_dtype = x_dtype; p.y_dtype = y_dtype; p.bias_dtype = bias_dtype; p.pow2 = pow2 != 0;
     p.rows = (int) rows; p.n = (int) n; p.k = (int) k; p.groups = groups;
     p.xvec = k % 4 == 0 && ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * es) == 0;
@@ -669,6 +702,7 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
     const void* xq = x;
     int64_t ldq = ldx;
     const float* xs = x_scale;
+    int64_t xsr = groups, xsg = 1;           // here one group's scales lie together: a warp's rows read them in one piece
     int early = 0;
     if (x_dtype != EXL3_DTYPE_E4M3 || !aligned16(x) || ldx % 16 != 0) {
         const int64_t need = exl3_fp8_linear_scratch_bytes(rows, k, n, x_dtype);
@@ -680,15 +714,17 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
             EXL3_CUDA(cudaMemcpy2DAsync(scratch, (size_t) ldq, x, (size_t) ldx, (size_t) k, (size_t) rows, cudaMemcpyDeviceToDevice, s));
         } else {
             float* sc = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + align_up(rows * ldq, 256));
-            if ((rc = fp8_quantize_launch(x, x_dtype, rows, k, ldx, scratch, ldq, sc, 1, pow2 != 0, s)) != EXL3_OK) return rc;
+            if ((rc = fp8_quantize_launch(x, x_dtype, rows, k, ldx, scratch, ldq, sc, 1, rows, 1, pow2 != 0, s)) != EXL3_OK) return rc;
             xs = sc;
+            xsr = 1;
+            xsg = rows;
             early = 1;
         }
     }
     if (rows <= kFsMaxRows) {
         const int nt = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
         if ((rc = fp8_map(&p.xmap, xq, rows, k, ldq, nt, "exl3_fp8_linear")) != EXL3_OK) return rc;
-        p.xs = xs;
+        p.xs = xs; p.xsr = xsr; p.xsg = xsg;
         p.early = early;
         return nt == 32 ? fs_launch<32, true>(p, s) : nt == 64 ? fs_launch<64, true>(p, s) : fs_launch<128, true>(p, s);
     }
@@ -704,7 +740,7 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
     FgParams g{};
     if ((rc = fp8_map(&g.xmap, xq, rows, k, ldq, 128, "exl3_fp8_linear")) != EXL3_OK) return rc;
     if ((rc = fp8_map(&g.wmap, w, n, k, ldw, nw / 2, "exl3_fp8_linear")) != EXL3_OK) return rc;
-    g.xs = xs; g.ws = w_scale; g.bias = bias; g.y = y; g.ldy = ldy;
+    g.xs = xs; g.xsr = xsr; g.xsg = xsg; g.ws = w_scale; g.bias = bias; g.y = y; g.ldy = ldy;
     g.y_dtype = y_dtype; g.bias_dtype = bias_dtype; g.early = early;
     g.yvec = aligned16(y) && ldy % (y_dtype == 2 ? 4 : 8) == 0;
     g.rows = (int) rows; g.n = (int) n; g.groups = groups;

@@ -72,7 +72,7 @@ constexpr int kQuantIlp = 4;        // 16-byte loads in flight for each lane
 // consecutive items, all loads first.
 template <int DT>
 __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(
-    const void* x, int64_t ldx, int64_t rows, int cols, uint8_t* q, int64_t ldq, float* scale, bool pow2, bool fast) {
+    const void* x, int64_t ldx, int64_t rows, int cols, uint8_t* q, int64_t ldq, float* scale, int64_t sr, int64_t sg, bool pow2, bool fast) {
     using V = QuantVec<DT>;
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(
         for (int o = 1; o < V::LANES; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float s = fp8_scale(m, pow2), inv = __frcp_rn(s);
         v[i].store(q, row[i] * ldq + col[i], cols - col[i], fast, s, inv, pow2);
-        if ((lane & (V::LANES - 1)) == 0 && col[i] < cols) scale[row[i] * groups + col[i] / kFp8Block] = s;
+        if ((lane & (V::LANES - 1)) == 0 && col[i] < cols) scale[row[i] * sr + col[i] / kFp8Block * sg] = s;
     }
 }
 
@@ -142,9 +142,10 @@ __global__ void __launch_bounds__(256) fp8_quant_blocks_kernel(
     if (tid == 0) scale[(int64_t) blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 
-// Arguments are checked by the callers.  rows >= 1, cols in 1..INT32_MAX - 4096.
+// Arguments are checked by the callers.  rows >= 1, cols in 1..2^30.  Rows'
+// scales lie at scale[row * sr + group * sg].
 int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
-                        float* scale, int block_rows, bool pow2, cudaStream_t s) {
+                        float* scale, int64_t sr, int64_t sg, int block_rows, bool pow2, cudaStream_t s) {
     const int es = dtype == 2 ? 4 : 2, vec = 16 / es;
     const bool fast = cols % vec == 0 && ldx % vec == 0 && ldq % vec == 0 && aligned16(x) &&
                       (reinterpret_cast<uintptr_t>(q) % (uintptr_t) vec) == 0;
@@ -155,7 +156,7 @@ int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, in
         const int64_t grid = (rows * per_row + kQuantWarps * kQuantIlp - 1) / (kQuantWarps * kQuantIlp);
         EXL3_REQUIRE(grid <= INT32_MAX, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: too many elements for one launch");
         auto kern = dtype == 0 ? fp8_quant_rows_kernel<0> : dtype == 1 ? fp8_quant_rows_kernel<1> : fp8_quant_rows_kernel<2>;
-        kern<<<(unsigned) grid, kQuantWarps * 32, 0, s>>>(x, ldx, rows, (int) cols, qb, ldq, scale, pow2, fast);
+        kern<<<(unsigned) grid, kQuantWarps * 32, 0, s>>>(x, ldx, rows, (int) cols, qb, ldq, scale, sr, sg, pow2, fast);
     } else {
         const int64_t rb = (rows + kFp8Block - 1) / kFp8Block;
         EXL3_REQUIRE(rb <= 65535, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: more than 65535 blocks of 128 rows");
@@ -180,6 +181,6 @@ extern "C" int exl3_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64
     EXL3_REQUIRE(x && q && scale, EXL3_ERR_ARG, "exl3_fp8_quantize: null pointer");
     EXL3_REQUIRE(reinterpret_cast<uintptr_t>(x) % (x_dtype == 2 ? 4 : 2) == 0 && reinterpret_cast<uintptr_t>(scale) % 4 == 0,
                  EXL3_ERR_ARG, "exl3_fp8_quantize: x and scale must be aligned to their elements");
-    return fp8_quantize_launch(x, x_dtype, rows, cols, ldx, q, ldq, scale, block_rows, pow2 != 0,
+    return fp8_quantize_launch(x, x_dtype, rows, cols, ldx, q, ldq, scale, (cols + 127) / 128, 1, block_rows, pow2 != 0,
                                static_cast<cudaStream_t>(stream));
 }
