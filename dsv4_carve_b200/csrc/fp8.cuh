@@ -31,10 +31,9 @@ __device__ __forceinline__ float fp8_scale(uint32_t amax_bits, bool pow2) {
 
 // x / s to within the e4m3 rounding that follows, i.e. RN_e4m3 of the result
 // is RN_e4m3 of the real quotient.  x * (1 / s) is off by at most two units in
-// its last place (two roundings of 2^-24), which moves the e4m3 rounding only next to a midpoint of
-// two e4m3 values (low 20 bits 0x80000 for normal ones, low 19 bits 0 below
-// 2^-6); only there the quotient is taken by division and a remainder that
-// the division lost breaks the false tie.
+// its last place (two roundings of 2^-24), which moves the e4m3 rounding only
+// next to a midpoint of two e4m3 values; only there the quotient is taken by
+// division, and a remainder that the division lost breaks the false tie.
 static __device__ __noinline__ float fp8_quotient_slow(float x, float s) {
     const float q = __fdiv_rn(x, s);
     const uint32_t b = __float_as_uint(q);
@@ -45,14 +44,17 @@ static __device__ __noinline__ float fp8_quotient_slow(float x, float s) {
     return __uint_as_float(away ? b + 1u : b - 1u);
 }
 
+// Whether q lies within two units of a midpoint of two e4m3 values: 0x80000 in
+// the low 20 bits of a normal one.  Values below 2^-6, where e4m3 steps stay
+// 2^-9 wide, are moved up by 2^-6 into the binade with that step first.
+__device__ __forceinline__ bool fp8_near_midpoint(float q) {
+    const float a = fabsf(q), m = a < 0x1p-6f ? a + 0x1p-6f : a;
+    return ((__float_as_uint(m) + 0x80002u) & 0xFFFFFu) <= 4u;
+}
+
 __device__ __forceinline__ float fp8_quotient(float x, float s, float inv, bool pow2) {
-    const float q = x * inv;
-    if (pow2) return q;                            // exact
-    const uint32_t b = __float_as_uint(q);
-    const bool mid = ((b + 0x80002u) & 0xFFFFFu) <= 4u;
-    const bool small = (b & 0x7FFFFFFFu) < 0x3C800000u && ((b + 2u) & 0x7FFFFu) <= 4u && (b << 1) != 0u;
-    if (mid || small) return fp8_quotient_slow(x, s);
-    return q;
+    const float q = x * inv;                       // exact for a power of two
+    return !pow2 && fp8_near_midpoint(q) ? fp8_quotient_slow(x, s) : q;
 }
 
 // Two fp32 -> two e4m3 bytes (nearest, ties to even, finite values saturate),
@@ -282,6 +284,18 @@ __device__ __forceinline__ float ld_dsmem(uint32_t addr, uint32_t rank) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
     return v;
 }
+
+// Tile of this CTA's shared memory -> global, asynchronously; what lies outside
+// the tensor is not written.
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                 :: "l"(tmap), "r"(c0), "r"(c1), "r"(smem_u32(src)) : "memory");
+}
+
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// This thread's stores have read their source / are complete.
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Brings one tile into L2 ahead of the load that will use it.
 __device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int c0, int c1) {

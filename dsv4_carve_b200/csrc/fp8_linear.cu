@@ -298,6 +298,7 @@ constexpr int kFgTmemCols = 512;
 struct FgParams {
     CUtensorMap xmap;            // e4m3 x [rows][k], box [128 k, 128 rows]
     CUtensorMap wmap;            // W [n][k], box [128 k, NW / 2]
+    CUtensorMap ymap;            // y [rows][n], box [128 bytes, 32 rows] (yvec)
     const float* xs;             // xs[row * xsr + group * xsg]
     const float* ws;             // [ceil(n / 128)][groups]
     const void* bias;
@@ -317,9 +318,9 @@ struct FgLayout {
     static constexpr int kSmem = 1024 + kStages * kStage + kFgEpiWarps * kOut + 512;
 };
 
-// Byte offset of 16-byte piece c of row r in a warp's output buffer: pieces are
-// permuted in each row so that neither rows nor pieces meet in a bank.
-__device__ __forceinline__ int fg_out(int r, int c) { return r * 256 + ((c ^ (r & 7)) << 4); }
+// Byte offset of 16-byte piece c (< 16) of row r in a warp's output buffer: two
+// tiles of 32 rows x 128 bytes, each with the 128-byte swizzle.
+__device__ __forceinline__ int fg_out(int r, int c) { return (c >> 3) * 4096 + r * 128 + (((c ^ r) & 7) << 4); }
 
 template <int NW>
 struct FgHead {
@@ -464,9 +465,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
                 }
             }
             if (!ok) break;
-            // Out through shared memory, 256 bytes of each row at a time, so that
-            // a warp stores whole rows' pieces: written straight from the
-            // registers (a row a lane) a tile took 8000 clocks.
+            // Out through shared memory, 256 bytes of each row at a time, by TMA
+            // stores that run on while the next tile is accumulated: written
+            // straight from the registers (a row a lane) a tile took 8000 clocks,
+            // by the warps from shared memory 5500.
             const int es = p.y_dtype == 2 ? 4 : 2;
             uint8_t* buf = stage_out + warp * L::kOut;
             const int wrow = t / p.ntiles * 256 + (int) rank * 128 + lg * 32;
@@ -480,6 +482,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
                 // 16-bit types: all kCols at once in pass 0; fp32: 64 in each pass
                 const int cols = es == 4 ? 64 : L::kCols;
                 if (h * cols >= L::kCols) break;
+                if (lane == 0) bulk_wait_read();                                  // the buffer's last stores
                 __syncwarp();
 #pragma unroll
                 for (int c = 0; c < 16; ++c) {
@@ -506,31 +509,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
                     }
                     *reinterpret_cast<uint4*>(buf + fg_out(lane, c)) = w;
                 }
+                fence_proxy_async_smem();
                 __syncwarp();
                 const int c0 = col0 + h * cols, left = min(cols, p.n - c0);       // columns of this pass
-                if (left <= 0) continue;
                 const int rows = min(32, p.rows - wrow);
-                uint8_t* y = static_cast<uint8_t*>(p.y) + ((int64_t) wrow * p.ldy + c0) * es;
-                if (p.yvec && (left * es) % 16 == 0) {
-                    const int per = left * es / 16;                               // 16-byte pieces of a row: 1 .. 16
-                    if (per == 16) {
-                        for (int i = lane; i < rows * 16; i += 32)
-                            *reinterpret_cast<uint4*>(y + (int64_t) (i >> 4) * p.ldy * es + (i & 15) * 16) =
-                                *reinterpret_cast<const uint4*>(buf + fg_out(i >> 4, i & 15));
-                    } else {
-                        for (int i = lane; i < rows * per; i += 32)
-                            *reinterpret_cast<uint4*>(y + (int64_t) (i / per) * p.ldy * es + (i % per) * 16) =
-                                *reinterpret_cast<const uint4*>(buf + fg_out(i / per, i % per));
+                if (left <= 0 || rows <= 0) continue;
+                if (p.yvec) {
+                    const int wide = 128 / es;                                    // columns of a box
+                    if (lane == 0) {
+                        for (int c = 0; c < left; c += wide) tma_store_2d(&p.ymap, buf + c / wide * 4096, c0 + c, wrow);
+                        bulk_commit();
                     }
                 } else {
+                    uint8_t* y = static_cast<uint8_t*>(p.y) + ((int64_t) wrow * p.ldy + c0) * es;
                     for (int r = 0; r < rows; ++r)
                         for (int j = lane; j < left; j += 32) {
                             if (es == 4) reinterpret_cast<uint32_t*>(y + (int64_t) r * p.ldy * 4)[j] = *reinterpret_cast<const uint32_t*>(buf + fg_out(r, j >> 2) + (j & 3) * 4);
                             else reinterpret_cast<uint16_t*>(y + (int64_t) r * p.ldy * 2)[j] = *reinterpret_cast<const uint16_t*>(buf + fg_out(r, j >> 3) + (j & 7) * 2);
                         }
+                    __syncwarp();
                 }
             }
         }
+        if (lane == 0) bulk_wait();                        // stores are complete when the CTA retires
     }
     tc_fence_before();
     __syncthreads();
@@ -572,6 +573,22 @@ int fp8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int6
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     EXL3_REQUIRE(r == CUDA_SUCCESS, EXL3_ERR_CUDA, "%s: tensor map failed (%d)", what, (int) r);
+    return EXL3_OK;
+}
+
+// y [rows][n] of pitch ldy elements; box 128 bytes x 32 rows, 128-byte swizzle.
+int fp8_out_map(CUtensorMap* map, void* y, int64_t rows, int64_t n, int64_t ldy, int dtype) {
+    auto encode = fp8_encoder();
+    EXL3_REQUIRE(encode != nullptr, EXL3_ERR_CUDA, "exl3_fp8_linear: cuTensorMapEncodeTiled is not available");
+    const int es = dtype == 2 ? 4 : 2;
+    const cuuint64_t dims[2] = {(cuuint64_t) n, (cuuint64_t) rows};
+    const cuuint64_t strides[1] = {(cuuint64_t) (ldy * es)};
+    const cuuint32_t box[2] = {(cuuint32_t) (128 / es), 32u};
+    const cuuint32_t estr[2] = {1u, 1u};
+    const CUresult r = encode(map, dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                              2, y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    EXL3_REQUIRE(r == CUDA_SUCCESS, EXL3_ERR_CUDA, "exl3_fp8_linear: output tensor map failed (%d)", (int) r);
     return EXL3_OK;
 }
 
@@ -742,7 +759,9 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
     if ((rc = fp8_map(&g.wmap, w, n, k, ldw, nw / 2, "exl3_fp8_linear")) != EXL3_OK) return rc;
     g.xs = xs; g.xsr = xsr; g.xsg = xsg; g.ws = w_scale; g.bias = bias; g.y = y; g.ldy = ldy;
     g.y_dtype = y_dtype; g.bias_dtype = bias_dtype; g.early = early;
-    g.yvec = aligned16(y) && ldy % (y_dtype == 2 ? 4 : 8) == 0;
+    const int ys = y_dtype == 2 ? 4 : 2;
+    g.yvec = aligned16(y) && ldy * ys % 16 == 0;
+    if (g.yvec && (rc = fp8_out_map(&g.ymap, y, rows, n, ldy, y_dtype)) != EXL3_OK) return rc;
     g.rows = (int) rows; g.n = (int) n; g.groups = groups;
     return nw == 128 ? fg_launch<128>(g, di.sms, s) : fg_launch<256>(g, di.sms, s);
 }

@@ -11,160 +11,189 @@
 namespace exl3 {
 
 // A lane holds VEC = 16 bytes / es elements of one row; 128 / VEC lanes hold a
-// group.  `fast`: rows start and end on VEC-element boundaries, so whole
-// vectors are inside or outside; otherwise elements are moved one by one.
-template <int DT>
+// group.  FAST: rows start and end on VEC-element boundaries, so whole vectors
+// are inside or outside; otherwise elements are moved one by one.
+template <int DT, bool FAST>
 struct QuantVec {
     static constexpr int VEC = DT == 2 ? 4 : 8;
     static constexpr int LANES = kFp8Block / VEC;          // 32 (fp32) or 16
-    uint4 raw;
-    __device__ __forceinline__ void load(const void* x, int64_t at, int left, bool fast) {
-        raw = make_uint4(0u, 0u, 0u, 0u);
-        if (left <= 0) return;
-        if (fast) {
-            raw = DT == 2 ? __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(x) + at))
-                          : __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + at));
-        } else if (DT == 2) {
-            raw = load_raw4_tail(x, DT, at, left);
-        } else {
-            const uint4 a = load_raw4_tail(x, DT, at, left), b = load_raw4_tail(x, DT, at + 4, left - 4);
-            raw = make_uint4(a.x, a.y, b.x, b.y);
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const void* x, int64_t at, int left) {
+        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+        if (left > 0) {
+            if (FAST) {
+                raw = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + at * (DT == 2 ? 4 : 2)));
+            } else if (DT == 2) {
+                raw = load_raw4_tail(x, DT, at, left);
+            } else {
+                const uint4 a = load_raw4_tail(x, DT, at, left), b = load_raw4_tail(x, DT, at + 4, left - 4);
+                raw = make_uint4(a.x, a.y, b.x, b.y);
+            }
         }
+        w[0] = raw.x; w[1] = raw.y; w[2] = raw.z; w[3] = raw.w;
     }
-    __device__ __forceinline__ void get(int half, float (&v)[4]) const {
-        unpack4(DT == 2 ? raw : half ? make_uint4(raw.z, raw.w, 0u, 0u) : raw, DT, v);
-    }
+    // Bits of the largest magnitude as fp32, NaN kept; 16-bit types two at a time.
     __device__ __forceinline__ uint32_t amax() const {
-        float v[4];
-        get(0, v);
-        uint32_t m = abs_bits4(v);
-        if (DT != 2) {
-            get(1, v);
-            m = max(m, abs_bits4(v));
-        }
-        return m;
-    }
-    __device__ __forceinline__ void store(uint8_t* q, int64_t at, int left, bool fast, float s, float inv, bool pow2) const {
-        if (left <= 0) return;
-        float v[4];
-        uint32_t w[2] = {0u, 0u};
+        if (DT == 2) return max(max(w[0] & 0x7FFFFFFFu, w[1] & 0x7FFFFFFFu), max(w[2] & 0x7FFFFFFFu, w[3] & 0x7FFFFFFFu));
+        uint32_t a[4];
 #pragma unroll
-        for (int h = 0; h < VEC / 4; ++h) {
-            get(h, v);
-            w[h] = fp8_quant4(v, s, inv, pow2);
+        for (int i = 0; i < 4; ++i) a[i] = w[i] & 0x7FFF7FFFu;
+        if (DT == 1) {
+            auto h = [&](int i) { return *reinterpret_cast<const __nv_bfloat162*>(&a[i]); };
+            const float2 f = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h(0), h(1)), __hmax2_nan(h(2), h(3))));
+            return max(abs_bits(f.x), abs_bits(f.y));
         }
-        if (fast) {
-            if (DT == 2) *reinterpret_cast<uint32_t*>(q + at) = w[0];
-            else *reinterpret_cast<uint2*>(q + at) = make_uint2(w[0], w[1]);
+        auto h = [&](int i) { return *reinterpret_cast<const __half2*>(&a[i]); };
+        const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(h(0), h(1)), __hmax2_nan(h(2), h(3))));
+        return max(abs_bits(f.x), abs_bits(f.y));
+    }
+    __device__ __forceinline__ void values(float (&v)[VEC]) const {
+        float t[4];
+        unpack4(make_uint4(w[0], w[1], w[2], w[3]), DT, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = t[i];
+        if constexpr (DT != 2) {
+            unpack4(make_uint4(w[2], w[3], 0u, 0u), DT, t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 + i] = t[i];
+        }
+    }
+    template <bool POW2>
+    __device__ __forceinline__ void store(uint8_t* q, int64_t at, int left, float s) const {
+        if (left <= 0) return;
+        const float inv = __frcp_rn(s);
+        float v[VEC];
+        values(v);
+        bool again = false;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float r = v[i] * inv;
+            if (!POW2) again |= fp8_near_midpoint(r);
+            v[i] = r;
+        }
+        if (!POW2 && again) {
+            values(v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = fp8_quotient_slow(v[i], s);
+        }
+        uint32_t o[VEC / 4];
+#pragma unroll
+        for (int i = 0; i < VEC / 4; ++i)
+            o[i] = e4m3x2(v[4 * i], v[4 * i + 1]) | (e4m3x2(v[4 * i + 2], v[4 * i + 3]) << 16);
+        if (FAST) {
+            if constexpr (DT == 2) *reinterpret_cast<uint32_t*>(q + at) = o[0];
+            else *reinterpret_cast<uint2*>(q + at) = make_uint2(o[0], o[1]);
         } else {
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
-                if (e < left) q[at + e] = (uint8_t) (w[e >> 2] >> (8 * (e & 3)));
+                if (e < left) q[at + e] = (uint8_t) (o[e >> 2] >> (8 * (e & 3)));
         }
     }
 };
 
 constexpr int kQuantWarps = 8;
-constexpr int kQuantIlp = 4;        // 16-byte loads in flight for each lane
 
-// One scale for each row and group of 128 columns.  An item is a row's 32-lane
-// span: one group (fp32) or two neighbours (16-bit); a warp takes kQuantIlp
-// consecutive items, all loads first.
-template <int DT>
-__global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(
-    const void* x, int64_t ldx, int64_t rows, int cols, uint8_t* q, int64_t ldq, float* scale, int64_t sr, int64_t sg, bool pow2, bool fast) {
-    using V = QuantVec<DT>;
+struct QuantArgs {
+    const void* x;
+    uint8_t* q;
+    float* scale;                // scale[row * sr + group * sg]; blocks: [row block][group]
+    int64_t ldx, ldq, sr, sg, rows;
+    int cols, groups, spans;     // spans: 32-lane pieces of a row
+};
+
+// One scale for each row and group of 128 columns.  A warp takes one span of a
+// row -- one group (fp32) or two neighbours (16-bit) -- in RP consecutive
+// rows, all loads first.
+template <int DT, bool POW2, bool FAST, int RP>
+__global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(const __grid_constant__ QuantArgs p) {
+    using V = QuantVec<DT, FAST>;
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const int groups = (cols + kFp8Block - 1) / kFp8Block;
-    constexpr int GP = 32 / V::LANES;                      // groups in an item
-    const int per_row = (groups + GP - 1) / GP;
-    const int64_t items = rows * per_row;
-    const int64_t first = ((int64_t) blockIdx.x * kQuantWarps + (threadIdx.x >> 5)) * kQuantIlp;
-    if (first >= items) return;
-    V v[kQuantIlp];
-    int64_t row[kQuantIlp];
-    int col[kQuantIlp];
-    row[0] = first / per_row;
-    int in_row = (int) (first - row[0] * per_row);
-    int64_t r = row[0];
+    const uint32_t item = blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
+    const int64_t row0 = (int64_t) (item / (uint32_t) p.spans) * RP;
+    const int col = (int) (item % (uint32_t) p.spans) * (32 * V::VEC) + lane * V::VEC, left = p.cols - col;
+    if (row0 >= p.rows) return;
+    const int n = p.rows - row0 < RP ? (int) (p.rows - row0) : RP;
+    V v[RP];
 #pragma unroll
-    for (int i = 0; i < kQuantIlp; ++i) {
-        row[i] = first + i < items ? r : -1;
-        col[i] = in_row * GP * kFp8Block + lane * V::VEC;
-        v[i].load(x, r * ldx + col[i], row[i] < 0 ? 0 : cols - col[i], fast);
-        if (++in_row == per_row) { in_row = 0; ++r; }
-    }
+    for (int i = 0; i < RP; ++i) v[i].load(p.x, (row0 + i) * p.ldx + col, i < n ? left : 0);
 #pragma unroll
-    for (int i = 0; i < kQuantIlp; ++i) {
-        if (row[i] < 0) return;
+    for (int i = 0; i < RP; ++i) {
         uint32_t m = v[i].amax();
 #pragma unroll
         for (int o = 1; o < V::LANES; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float s = fp8_scale(m, pow2), inv = __frcp_rn(s);
-        v[i].store(q, row[i] * ldq + col[i], cols - col[i], fast, s, inv, pow2);
-        if ((lane & (V::LANES - 1)) == 0 && col[i] < cols) scale[row[i] * sr + col[i] / kFp8Block * sg] = s;
+        if (i >= n) break;
+        const float s = fp8_scale(m, POW2);
+        v[i].template store<POW2>(p.q, (row0 + i) * p.ldq + col, left, s);
+        if ((lane & (V::LANES - 1)) == 0 && left > 0) p.scale[(row0 + i) * p.sr + col / kFp8Block * p.sg] = s;
     }
 }
 
-// One scale for each 128 x 128 block: a CTA of 256 threads holds the block in
-// registers (32 of them for 16-bit types, 64 for fp32).
-template <int DT>
-__global__ void __launch_bounds__(256) fp8_quant_blocks_kernel(
-    const void* x, int64_t ldx, int64_t rows, int cols, uint8_t* q, int64_t ldq, float* scale, bool pow2, bool fast) {
-    using V = QuantVec<DT>;
-    constexpr int RP = 256 / V::LANES;                     // rows in a pass
+// One scale for each 128 x 128 block, held in registers: 512 threads of four
+// 16-byte pieces (16-bit types) or eight (fp32).
+template <int DT, bool POW2, bool FAST>
+__global__ void __launch_bounds__(512) fp8_quant_blocks_kernel(const __grid_constant__ QuantArgs p) {
+    using V = QuantVec<DT, FAST>;
+    constexpr int RP = 512 / V::LANES;                     // rows in a pass
     constexpr int N = kFp8Block / RP;                      // passes
-    __shared__ uint32_t wmax[8];
+    __shared__ uint32_t wmax[16];
     const int tid = threadIdx.x;
     const int64_t row0 = (int64_t) blockIdx.y * kFp8Block + tid / V::LANES;
-    const int col = blockIdx.x * kFp8Block + (tid % V::LANES) * V::VEC;
+    const int col = blockIdx.x * kFp8Block + (tid % V::LANES) * V::VEC, left = p.cols - col;
     V v[N];
     uint32_t m = 0u;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int64_t r = row0 + i * RP;
-        v[i].load(x, r * ldx + col, r < rows ? cols - col : 0, fast);
-    }
+    for (int i = 0; i < N; ++i) v[i].load(p.x, (row0 + i * RP) * p.ldx + col, row0 + i * RP < p.rows ? left : 0);
 #pragma unroll
     for (int i = 0; i < N; ++i) m = max(m, v[i].amax());
     m = __reduce_max_sync(0xffffffffu, m);
     if ((tid & 31) == 0) wmax[tid >> 5] = m;
     __syncthreads();
+    m = __reduce_max_sync(0xffffffffu, wmax[tid & 15]);
+    const float s = fp8_scale(m, POW2);
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = max(m, wmax[w]);
-    const float s = fp8_scale(m, pow2), inv = __frcp_rn(s);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int64_t r = row0 + i * RP;
-        v[i].store(q, r * ldq + col, r < rows ? cols - col : 0, fast, s, inv, pow2);
+    for (int i = 0; i < N; ++i)
+        v[i].template store<POW2>(p.q, (row0 + i * RP) * p.ldq + col, row0 + i * RP < p.rows ? left : 0, s);
+    if (tid == 0) p.scale[(int64_t) blockIdx.y * gridDim.x + blockIdx.x] = s;
+}
+
+template <int DT, bool POW2, bool FAST>
+int quant_launch(QuantArgs& a, int block_rows, cudaStream_t s) {
+    if (block_rows == 1) {
+        a.spans = DT == 2 ? a.groups : (a.groups + 1) / 2;
+        // Four rows a warp keep 2 KB a warp in flight; with fewer than about
+        // two warps an SM that way, one row a warp spreads a small batch wider.
+        const int rp = a.rows * a.spans < 4 * 2 * 148 * kQuantWarps ? 1 : 4;
+        const int64_t items = (a.rows + rp - 1) / rp * a.spans, grid = (items + kQuantWarps - 1) / kQuantWarps;
+        EXL3_REQUIRE(items <= INT32_MAX, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: too many elements for one launch");
+        if (rp == 1) fp8_quant_rows_kernel<DT, POW2, FAST, 1><<<(unsigned) grid, kQuantWarps * 32, 0, s>>>(a);
+        else fp8_quant_rows_kernel<DT, POW2, FAST, 4><<<(unsigned) grid, kQuantWarps * 32, 0, s>>>(a);
+    } else {
+        const int64_t rb = (a.rows + kFp8Block - 1) / kFp8Block;
+        EXL3_REQUIRE(rb <= 65535, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: more than 65535 blocks of 128 rows");
+        fp8_quant_blocks_kernel<DT, POW2, FAST><<<dim3((unsigned) a.groups, (unsigned) rb), 512, 0, s>>>(a);
     }
-    if (tid == 0) scale[(int64_t) blockIdx.y * gridDim.x + blockIdx.x] = s;
+    EXL3_CUDA(cudaGetLastError());
+    return EXL3_OK;
+}
+
+template <int DT>
+int quant_dispatch(QuantArgs& a, int block_rows, bool pow2, bool fast, cudaStream_t s) {
+    if (fast) return pow2 ? quant_launch<DT, true, true>(a, block_rows, s) : quant_launch<DT, false, true>(a, block_rows, s);
+    return pow2 ? quant_launch<DT, true, false>(a, block_rows, s) : quant_launch<DT, false, false>(a, block_rows, s);
 }
 
 // Arguments are checked by the callers.  rows >= 1, cols in 1..2^30.  Rows'
 // scales lie at scale[row * sr + group * sg].
 int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
                         float* scale, int64_t sr, int64_t sg, int block_rows, bool pow2, cudaStream_t s) {
-    const int es = dtype == 2 ? 4 : 2, vec = 16 / es;
+    const int vec = dtype == 2 ? 4 : 8;
     const bool fast = cols % vec == 0 && ldx % vec == 0 && ldq % vec == 0 && aligned16(x) &&
                       (reinterpret_cast<uintptr_t>(q) % (uintptr_t) vec) == 0;
-    const int64_t groups = (cols + kFp8Block - 1) / kFp8Block;
-    uint8_t* qb = static_cast<uint8_t*>(q);
-    if (block_rows == 1) {
-        const int64_t per_row = dtype == 2 ? groups : (groups + 1) / 2;
-        const int64_t grid = (rows * per_row + kQuantWarps * kQuantIlp - 1) / (kQuantWarps * kQuantIlp);
-        EXL3_REQUIRE(grid <= INT32_MAX, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: too many elements for one launch");
-        auto kern = dtype == 0 ? fp8_quant_rows_kernel<0> : dtype == 1 ? fp8_quant_rows_kernel<1> : fp8_quant_rows_kernel<2>;
-        kern<<<(unsigned) grid, kQuantWarps * 32, 0, s>>>(x, ldx, rows, (int) cols, qb, ldq, scale, sr, sg, pow2, fast);
-    } else {
-        const int64_t rb = (rows + kFp8Block - 1) / kFp8Block;
-        EXL3_REQUIRE(rb <= 65535, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: more than 65535 blocks of 128 rows");
-        auto kern = dtype == 0 ? fp8_quant_blocks_kernel<0> : dtype == 1 ? fp8_quant_blocks_kernel<1> : fp8_quant_blocks_kernel<2>;
-        kern<<<dim3((unsigned) groups, (unsigned) rb), 256, 0, s>>>(x, ldx, rows, (int) cols, qb, ldq, scale, pow2, fast);
-    }
-    EXL3_CUDA(cudaGetLastError());
-    return EXL3_OK;
+    QuantArgs a{x, static_cast<uint8_t*>(q), scale, ldx, ldq, sr, sg, rows, (int) cols, (int) ((cols + kFp8Block - 1) / kFp8Block), 0};
+    if (dtype == 0) return quant_dispatch<0>(a, block_rows, pow2, fast, s);
+    if (dtype == 1) return quant_dispatch<1>(a, block_rows, pow2, fast, s);
+    return quant_dispatch<2>(a, block_rows, pow2, fast, s);
 }
 
 }  // namespace exl3
