@@ -64,18 +64,8 @@ struct QuantVec {
         const float inv = __frcp_rn(s);
         float v[VEC];
         values(v);
-        bool again = false;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float r = v[i] * inv;
-            if (!POW2) again |= fp8_near_midpoint(r);
-            v[i] = r;
-        }
-        if (!POW2 && again) {
-            values(v);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = fp8_quotient_slow(v[i], s);
-        }
+        for (int i = 0; i < VEC; ++i) v[i] = fp8_quotient(v[i], s, inv, POW2);
         uint32_t o[VEC / 4];
 #pragma unroll
         for (int i = 0; i < VEC / 4; ++i)
