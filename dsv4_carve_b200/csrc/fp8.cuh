@@ -61,17 +61,7 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
-__device__ __forceinline__ uint32_t fp8_quant4(const float (&v)[4], float s, float inv, bool pow2) {
-    const uint32_t a = e4m3x2(fp8_quotient(v[0], s, inv, pow2), fp8_quotient(v[1], s, inv, pow2));
-    const uint32_t b = e4m3x2(fp8_quotient(v[2], s, inv, pow2), fp8_quotient(v[3], s, inv, pow2));
-    return a | (b << 16);
-}
-
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-
-__device__ __forceinline__ uint32_t abs_bits4(const float (&v)[4]) {
-    return max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
-}
 
 // ---------------------------------------------------------------- loads
 __device__ __forceinline__ float load_f32(const void* x, int dtype, int64_t i) {
@@ -80,23 +70,9 @@ __device__ __forceinline__ float load_f32(const void* x, int dtype, int64_t i) {
     return reinterpret_cast<const float*>(x)[i];
 }
 
-// Four values starting at element i, as they lie in memory (8 bytes of a
-// 16-bit type in raw.x, raw.y): a load that can stay in flight.
-__device__ __forceinline__ uint4 load_raw4(const void* x, int dtype, int64_t i) {
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (dtype == 2) {
-        raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(x) + i);
-    } else if (dtype == kDtE4M3) {
-        raw.x = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(x) + i);
-    } else {
-        const uint2 h = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(x) + i);
-        raw.x = h.x; raw.y = h.y;
-    }
-    return raw;
-}
-
-// The same four values one by one, those at or past `left` as zero: rows whose
-// start or pitch is not a multiple of the vector, and the last columns.
+// Four values from element i on, as they lie in memory (a 16-bit type in the
+// first two words, e4m3 in the first), read one by one; those at or past `left`
+// are zero.
 __device__ __forceinline__ uint4 load_raw4_tail(const void* x, int dtype, int64_t i, int left) {
     uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -122,6 +98,104 @@ __device__ __forceinline__ void unpack4(const uint4& raw, int dtype, float (&v)[
         v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
     }
 }
+
+// A warp's share of quantising rows of x into a stage: four rows, eight lanes
+// and 16 elements a lane each -- one chain of latencies for four rows -- or a
+// lone row over all 32 lanes, where the shorter chain counts.
+struct XRows {
+    uint4 r[4];                  // a lane's elements as they lie in memory
+
+    __device__ __forceinline__ static int row(int cnt, int lane) { return cnt == 1 ? 0 : lane >> 3; }
+    __device__ __forceinline__ static int col(int cnt, int lane) { return cnt == 1 ? lane * 4 : (lane & 7) * 16; }
+
+    // This lane's elements from element `at` on, those at or past `left` as zero.
+    // vec: starts are aligned to 16 bytes (e4m3: four elements) and `left` is a
+    // multiple of the lane's elements.
+    __device__ __forceinline__ void load(int cnt, const void* x, int dtype, int64_t at, int left, bool vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (left <= 0) return;
+        const uint8_t* src = static_cast<const uint8_t*>(x) + at * (dtype == 2 ? 4 : dtype == kDtE4M3 ? 1 : 2);
+        if (!vec) {
+            const int n = cnt == 1 ? 1 : 4;
+            uint4 t[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = i < n ? load_raw4_tail(x, dtype, at + 4 * i, left - 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+            if (dtype == 2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = t[i];
+            } else if (dtype == kDtE4M3) {
+                r[0] = make_uint4(t[0].x, t[1].x, t[2].x, t[3].x);
+            } else {
+                r[0] = make_uint4(t[0].x, t[0].y, t[1].x, t[1].y);
+                r[1] = make_uint4(t[2].x, t[2].y, t[3].x, t[3].y);
+            }
+        } else if (cnt == 1) {
+            if (dtype == 2) r[0] = *reinterpret_cast<const uint4*>(src);
+            else if (dtype == kDtE4M3) r[0].x = *reinterpret_cast<const uint32_t*>(src);
+            else {
+                const uint2 h = *reinterpret_cast<const uint2*>(src);
+                r[0].x = h.x; r[0].y = h.y;
+            }
+        } else {
+            const uint4* v = reinterpret_cast<const uint4*>(src);
+            r[0] = v[0];
+            if (dtype != kDtE4M3) r[1] = v[1];
+            if (dtype == 2) { r[2] = v[2]; r[3] = v[3]; }
+        }
+    }
+
+    // The lane's elements in e4m3 (cnt == 1: the first word); `s`: their row's scale.
+    __device__ __forceinline__ uint4 quantize(int cnt, int dtype, bool pow2, float& s) const {
+        float v[16];
+        if (dtype == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[4 * i] = __uint_as_float(r[i].x); v[4 * i + 1] = __uint_as_float(r[i].y);
+                v[4 * i + 2] = __uint_as_float(r[i].z); v[4 * i + 3] = __uint_as_float(r[i].w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float t[4];
+                unpack4(r[i], dtype, t);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[8 * i + j] = t[j];
+                unpack4(make_uint4(r[i].z, r[i].w, 0u, 0u), dtype, t);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[8 * i + 4 + j] = t[j];
+            }
+        }
+        uint32_t m = 0u;
+        uint32_t q[4] = {0u, 0u, 0u, 0u};
+        if (cnt == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = max(m, abs_bits(v[i]));
+            m = __reduce_max_sync(0xffffffffu, m);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = max(m, abs_bits(v[i]));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+        s = fp8_scale(m, pow2);
+        const float inv = __frcp_rn(s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i > 0 && cnt == 1) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * i + j] = fp8_quotient(v[4 * i + j], s, inv, pow2);
+            q[i] = e4m3x2(v[4 * i], v[4 * i + 1]) | (e4m3x2(v[4 * i + 2], v[4 * i + 3]) << 16);
+        }
+        return make_uint4(q[0], q[1], q[2], q[3]);
+    }
+
+    // Into a K-major tile of 128-byte rows with the 128-byte swizzle, this lane's row being `row`.
+    __device__ __forceinline__ static void store(int cnt, uint8_t* tile, int row, int lane, const uint4& q) {
+        if (cnt == 1) *reinterpret_cast<uint32_t*>(tile + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) = q.x;
+        else *reinterpret_cast<uint4*>(tile + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) = q;
+    }
+};
 
 // ---------------------------------------------------------------- waits
 // mbar_wait (2 s, then the ring-timeout bit) for pipelines whose steps take a
@@ -177,12 +251,6 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t dtmem, uint64_t adesc, uint64
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
                  :: "r"(dtmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc) : "memory");
-}
-
-// Byte offset of byte k (< 128) of a row in a K-major tile with 128-byte rows
-// and the 128-byte swizzle.
-__device__ __forceinline__ uint32_t sw128_byte(int row, int k) {
-    return (uint32_t) (row * 128 + (((k >> 4) ^ (row & 7)) << 4) + (k & 15));
 }
 
 // The same over a pair of CTAs: each holds its half of A's rows (128 of 256)
@@ -243,6 +311,10 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_dst, uint32_t col
 
 __device__ __forceinline__ void tmem_free_pair(uint32_t taddr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(taddr), "r"(cols) : "memory");
+}
+
+__device__ __forceinline__ void tmap_prefetch(const void* tmap) {
+    asm volatile("prefetch.tensormap [%0];" :: "l"(tmap) : "memory");
 }
 
 // ---------------------------------------------------------------- clusters

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(&H.full[s], PRE ? 2 : 1 + rows);
+            mbar_init(&H.full[s], PRE ? 2 : 1 + (rows + 3) / 4);
             mbar_init(&H.empty[s], 1 + kFsEpiWarps);
         }
         for (int b = 0; b < L::kBufs; ++b) { mbar_init(&H.tfull[b], 1); mbar_init(&H.tempty[b], kFsEpiWarps); }
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = H.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, H.tmem, 0);
 
     float acc[NT];
 #pragma unroll
@@ -154,8 +154,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
         const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
         for (int s = 0; s < nsteps; ++s) {
             const int st = s % p.stages, b = s % L::kBufs;
-            if (!mbar_wait_lanes(&H.full[st], (s / p.stages) & 1u, status)) break;
-            if (!mbar_wait_lanes(&H.tempty[b], ((s / L::kBufs) + 1u) & 1u, status)) break;
+            if (!mbar_poll2_lanes(&H.full[st], (s / p.stages) & 1u, &H.tempty[b], ((s / L::kBufs) + 1u) & 1u, status)) break;
             tc_fence_after();
             const uint64_t wd = desc0 + (uint64_t) (st * (L::kStage >> 4)), xd = wd + (kFp8WTile >> 4);
             if (elect_lane()) {
@@ -185,37 +184,31 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
             if (lane == 0) mbar_arrive(&H.full[st]);
         }
     } else if (warp >= kFsEpiWarps) {
-        // x: one warp for each (step, row), four elements a lane.  Rows of the B
-        // operand behind the last one hold whatever the stage held: each is a
-        // column of D of its own, and those columns are never used.
+        // x: one warp for each step and four rows.  Rows of the B operand behind
+        // the last one hold whatever the stage held: each is a column of D of its
+        // own, and those columns are never used.
         pdl_wait();
-        const int xw = warp - kFsEpiWarps, items = nsteps * rows, k4 = lane * 4;
+        const int xw = warp - kFsEpiWarps, quads = (rows + 3) >> 2, items = nsteps * quads;
+        XRows next;
         auto fetch = [&](int i) {
-            const int col = (kbeg + i / rows) * 128 + k4;
-            const int64_t at = (int64_t) (row0 + i % rows) * p.ldx + col;
-            if (p.xvec) return col < p.k ? load_raw4(p.x, p.x_dtype, at) : make_uint4(0u, 0u, 0u, 0u);
-            return load_raw4_tail(p.x, p.x_dtype, at, p.k - col);
+            const int r = (i % quads) * 4, cnt = min(4, rows - r), lr = XRows::row(cnt, lane);
+            const int col = (kbeg + i / quads) * 128 + XRows::col(cnt, lane);
+            next.load(cnt, p.x, p.x_dtype, (int64_t) (row0 + r + lr) * p.ldx + col, lr < cnt ? p.k - col : 0, p.xvec);
         };
-        uint4 next = xw < items ? fetch(xw) : make_uint4(0u, 0u, 0u, 0u);
+        if (xw < items) fetch(xw);
         for (int i = xw; i < items; i += kFsXWarps) {
-            const uint4 raw = next;
-            if (i + kFsXWarps < items) next = fetch(i + kFsXWarps);
-            const int s = i / rows, r = i % rows, st = s % p.stages;
-            float sx;
-            uint32_t q;
-            if (p.x_dtype == kDtE4M3) {
-                q = raw.x;
-                sx = __ldg(p.xs + (row0 + r) * p.xsr + (kbeg + s) * p.xsg);
-            } else {
-                float v[4];
-                unpack4(raw, p.x_dtype, v);
-                sx = fp8_scale(__reduce_max_sync(0xffffffffu, abs_bits4(v)), p.pow2);
-                q = fp8_quant4(v, sx, __frcp_rn(sx), p.pow2);
-            }
-            const float f = sx * __ldg(p.ws + (int64_t) tile * p.groups + kbeg + s);
+            const XRows cur = next;
+            if (i + kFsXWarps < items) fetch(i + kFsXWarps);
+            const int s = i / quads, r = (i % quads) * 4, cnt = min(4, rows - r), lr = XRows::row(cnt, lane), st = s % p.stages;
+            const float ws = __ldg(p.ws + (int64_t) tile * p.groups + kbeg + s);
+            const bool head = lr < cnt && (cnt == 1 ? lane == 0 : (lane & 7) == 0);
+            float sx = 0.f;
+            uint4 q = cur.r[0];
+            if (p.x_dtype != kDtE4M3) q = cur.quantize(cnt, p.x_dtype, p.pow2, sx);
+            else if (head) sx = __ldcg(p.xs + (row0 + r + lr) * p.xsr + (kbeg + s) * p.xsg);
             if (!mbar_wait_lanes(&H.empty[st], ((s / p.stages) + 1u) & 1u, status)) break;
-            *reinterpret_cast<uint32_t*>(ring + st * L::kStage + kFp8WTile + sw128_byte(r, k4)) = q;
-            if (lane == 0) H.fac[st][r] = f;
+            if (lr < cnt) XRows::store(cnt, ring + st * L::kStage + kFp8WTile, r + lr, lane, q);
+            if (head) H.fac[st][r + lr] = sx * ws;
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&H.full[st]);
@@ -711,7 +704,7 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
     p.x = x; p.ldx = ldx; p.xs = x_scale; p.xsr = groups; p.xsg = 1; p.ws = w_scale; p.bias = bias; p.y = y; p.ldy = ldy;
     p.x_dtype = x_dtype; p.y_dtype = y_dtype; p.bias_dtype = bias_dtype; p.pow2 = pow2 != 0;
     p.rows = (int) rows; p.n = (int) n; p.k = (int) k; p.groups = groups;
-    p.xvec = k % 4 == 0 && ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * es) == 0;
+    p.xvec = k % 16 == 0 && ldx * es % 16 == 0 && aligned16(x);
     if (rows <= kFsMaxRows && (rc = fp8_map(&p.wmap, w, n, k, ldw, 128, "exl3_fp8_linear")) != EXL3_OK) return rc;
     if (rows <= kFsInlineRows) return fs_launch<16, false>(p, s);
 

@@ -40,8 +40,8 @@ constexpr int kFmMaxCtas = 160;
 constexpr int kFmThreads = 320;              // warps 0-3 epilogue, 4-7 x, 8 producer, 9 MMA
 constexpr int kFmProducerWarp = 8;
 constexpr int kFmMmaWarp = 9;
-constexpr int kFmMaxStages = 8;
-constexpr int kFmMaxBufs = 4;
+constexpr int kFmMaxSlotsW = 12;             // weight blocks in the ring
+constexpr int kFmMaxBufs = 4;                // steps whose sums and inputs are held
 // Control region (uint32 words): [2] status; counters of kernel 1's output
 // tiles (expert group, 128 columns of I) and of kernel 2's (128 columns of H).
 constexpr int kFmCntA = 16;
@@ -64,7 +64,7 @@ struct FmParams {
     RouteIn route;
     float limit;
     int x_dtype, out_dtype, pow2, xvec;
-    int m, topk, E, H, I, stages;
+    int m, topk, E, H, I, slots;
 };
 
 // Pairs are the valid (token, slot)s ordered by (expert, slot); a group is up
@@ -79,25 +79,34 @@ struct FmPlan {
     int G;
 };
 
+// Shared memory of a CTA: a ring of weight blocks (16 KB each, so that few bytes
+// wait while many are in flight; kernel 2: with the NT input rows of the block),
+// kernel 1's quantised x of kBufs steps, the head, kernel 2's output rows.
+// A step is one block of k: kernel 1 multiplies the gate and the up block, each
+// into TMEM columns of its own, kernel 2 the down block.
 template <int NT, int PH>
 struct FmLayout {
-    static constexpr int kMats = PH == 0 ? 2 : 1;                    // gate and up, or down
-    static constexpr int kW = kMats * (int) kFp8WTile;
-    static constexpr int kStage = kW + NT * 128;
+    static constexpr int kMats = PH == 0 ? 2 : 1;
     static constexpr int kBufs = NT <= 16 ? 4 : PH == 0 ? 2 : NT <= 32 ? 4 : 2;
     static constexpr int kTmemCols = NT * kMats * kBufs;             // 64 .. 256
+    static constexpr int kX = NT * 128;
+    static constexpr int kSlot = (int) kFp8WTile + (PH == 0 ? 0 : kX);
+    static constexpr int kXRing = PH == 0 ? kBufs * kX : 0;
 };
 
 template <int NT>
 struct FmHead {
     FmPlan plan;
-    uint64_t full[kFmMaxStages];
-    uint64_t empty[kFmMaxStages];
-    uint64_t tfull[kFmMaxBufs];
-    uint64_t tempty[kFmMaxBufs];
-    alignas(16) float fac[kFmMaxStages][NT];
-    float wsc[kFmMaxStages][2];
-    uint32_t wmax[4][NT];
+    uint64_t wfull[kFmMaxSlotsW];        // a weight block has arrived
+    uint64_t wdone[kFmMaxSlotsW];        // it has been multiplied
+    uint64_t xfull[kFmMaxBufs];          // a step's input rows (kernel 1) and factors are there
+    uint64_t tfull[kFmMaxBufs];          // a step's sums are in TMEM; its input rows have been read
+    uint64_t tempty[kFmMaxBufs];         // they have been read
+    // Factors of a step's columns.  Twice kBufs deep: x's warps write step s once
+    // step s - kBufs is in TMEM, i.e. the epilogue is done with s - 2 kBufs.
+    alignas(16) float fac[2 * kFmMaxBufs][NT];
+    float wsc[2 * kFmMaxBufs][2];
+    alignas(16) uint32_t wmax[4][NT];
     uint32_t tmem;
     uint32_t last;
 };
@@ -174,22 +183,27 @@ struct FmAt {
 template <int NT, int PH>
 __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_constant__ FmParams p) {
     using L = FmLayout<NT, PH>;
-    constexpr int kMats = L::kMats;
+    constexpr int kMats = L::kMats, kBufs = L::kBufs, kFacs = 2 * L::kBufs;
+    constexpr int kCh = NT < 32 ? 4 : 8;                              // columns handled together at a tile's end
     extern __shared__ uint8_t fm_raw[];
     uint8_t* ring = fm_raw + ((1024u - (smem_u32(fm_raw) & 1023u)) & 1023u);
-    FmHead<NT>& S = *reinterpret_cast<FmHead<NT>*>(ring + p.stages * L::kStage);
-    float* oacc = reinterpret_cast<float*>(ring + p.stages * L::kStage + sizeof(FmHead<NT>));    // PH 1: [m][128]
+    uint8_t* xring = ring + p.slots * L::kSlot;
+    FmHead<NT>& S = *reinterpret_cast<FmHead<NT>*>(xring + L::kXRing);
+    float* oacc = reinterpret_cast<float*>(xring + L::kXRing + sizeof(FmHead<NT>));    // PH 1: [m][128]
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const int C = (int) gridDim.x, cta = (int) blockIdx.x;
     const int NBI = p.I / 128, NBH = p.H / 128, KB = PH == 0 ? NBH : NBI;
+    const int W = p.slots;
     uint32_t* status = p.ctrl + 2;
 
     if (tid == 0) {
-        for (int s = 0; s < p.stages; ++s) {
-            mbar_init(&S.full[s], PH == 0 ? 1 + 4 : 1 + 1);
-            mbar_init(&S.empty[s], 1 + 4);
+        tmap_prefetch(PH == 0 ? &p.w13 : &p.w2);
+        for (int s = 0; s < W; ++s) { mbar_init(&S.wfull[s], 1); mbar_init(&S.wdone[s], 1); }
+        for (int b = 0; b < kBufs; ++b) {
+            mbar_init(&S.xfull[b], PH == 0 ? 4 : 1);
+            mbar_init(&S.tfull[b], 1);
+            mbar_init(&S.tempty[b], 4);
         }
-        for (int b = 0; b < L::kBufs; ++b) { mbar_init(&S.tfull[b], 1); mbar_init(&S.tempty[b], 4); }
         fence_barrier_init();
     }
     if (warp == kFmMmaWarp) tmem_alloc(&S.tmem, L::kTmemCols);
@@ -203,131 +217,133 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
     fm_plan(S.plan, p, NT, tid);
     tc_fence_after();
     const FmPlan& P = S.plan;
-    const uint32_t tmem = S.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, S.tmem, 0);
     const int G = P.G;
-    const int per_tile = PH == 0 ? KB : G * KB;                       // blocks of one output tile
+    const int per_tile = PH == 0 ? KB : G * KB;                       // steps of one output tile
     const int total = PH == 0 ? G * NBI * KB : NBH * per_tile;
     const int beg = fm_start(cta, C, total), end = fm_start(cta + 1, C, total), nsteps = end - beg;
-    const int sm = p.stages;
 
     if (warp == kFmProducerWarp) {
         if (lane == 0 && nsteps > 0) {
-            const CUtensorMap* wm = PH == 0 ? &p.w13 : &p.w2;
-            auto weights = [&](const FmAt<PH>& a, int st) {
+            const int nblk = nsteps * kMats;
+            auto weights = [&](const FmAt<PH>& a, int mat, int slot) {
                 const int e = P.pexp[P.gstart[a.g]];
-                mbar_arrive_expect_tx(&S.full[st], (uint32_t) (PH == 0 ? L::kW : L::kStage));
-                uint8_t* dst = ring + st * L::kStage;
-                if (PH == 0) {
-                    const int row = e * 2 * p.I + (a.tile % NBI) * 128;
-                    tma_load_2d(dst, wm, a.kb * 128, row, &S.full[st]);
-                    tma_load_2d(dst + kFp8WTile, wm, a.kb * 128, row + p.I, &S.full[st]);
-                } else {
-                    tma_load_2d(dst, wm, a.kb * 128, e * p.H + a.tile * 128, &S.full[st]);
-                }
+                mbar_arrive_expect_tx(&S.wfull[slot], (uint32_t) L::kSlot);
+                const int row = PH == 0 ? e * 2 * p.I + mat * p.I + (a.tile % NBI) * 128 : e * p.H + a.tile * 128;
+                tma_load_2d(ring + slot * L::kSlot, PH == 0 ? &p.w13 : &p.w2, a.kb * 128, row, &S.wfull[slot]);
             };
-            auto inputs = [&](const FmAt<PH>& a, int st) {
-                tma_load_2d(ring + st * L::kStage + L::kW, &p.amap, a.kb * 128, P.gstart[a.g], &S.full[st]);
+            auto inputs = [&](const FmAt<PH>& a, int slot) {
+                tma_load_2d(ring + slot * L::kSlot + kFp8WTile, &p.amap, a.kb * 128, P.gstart[a.g], &S.wfull[slot]);
             };
             FmAt<PH> a(beg, G, NBI, KB);
-            int issued = 0;
+            int t = 0;
             if (PH == 1) {
                 // the weights do not depend on kernel 1: a ring of them ahead of the wait
                 FmAt<PH> a0 = a;
-                for (; issued < min(sm, nsteps); ++issued) { weights(a, issued); a.next(); }
+                for (; t < min(W, nblk); ++t) { weights(a, 0, t); a.next(); }
                 pdl_wait();
                 fence_proxy_async_global();
-                for (int s = 0; s < issued; ++s) { inputs(a0, s); a0.next(); }
+                for (int s = 0; s < t; ++s) { inputs(a0, s); a0.next(); }
             }
-            for (int s = issued; s < nsteps; ++s, a.next()) {
-                const int st = s % sm;
-                if (!mbar_wait(&S.empty[st], ((s / sm) + 1u) & 1u, status)) break;
-                weights(a, st);
-                if (PH == 1) inputs(a, st);
+            int issued = t;
+            for (; t < nblk; ++t) {
+                const int slot = t % W;
+                if (t >= W && !mbar_wait(&S.wdone[slot], ((t / W) + 1u) & 1u, status)) break;
+                weights(a, PH == 0 ? t & 1 : 0, slot);
+                if (PH == 1) inputs(a, slot);
+                if (PH == 1 || (t & 1)) a.next();
                 ++issued;
             }
             // no copy may still be in flight when the CTA retires
-            for (int i = max(0, issued - sm); i < issued; ++i)
-                if (!mbar_wait(&S.full[i % sm], (i / sm) & 1u, status)) break;
+            for (int i = max(0, issued - W); i < issued; ++i)
+                if (!mbar_wait(&S.wfull[i % W], (i / W) & 1u, status)) break;
         } else if (PH == 1) {
             pdl_wait();
         }
     } else if (warp == kFmMmaWarp) {
-        const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
+        const uint64_t wdesc0 = sdesc_sw128(smem_u32(ring)), xdesc0 = sdesc_sw128(smem_u32(xring));
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
-        for (int s = 0; s < nsteps; ++s, a.next()) {
-            const int st = s % sm, b = s % L::kBufs;
+        int slot = 0;
+        uint32_t wpar = 0;
+        bool ok = true;
+        for (int s = 0; s < nsteps && ok; ++s, a.next()) {
+            const int b = s % kBufs;
             const int n = P.gstart[a.g + 1] - P.gstart[a.g];
             const uint32_t id = __shfl_sync(0xffffffffu, idesc_f16(128, (n + 15) & ~15), 0);
-            if (!mbar_wait_lanes(&S.full[st], (s / sm) & 1u, status)) break;
-            if (!mbar_wait_lanes(&S.tempty[b], ((s / L::kBufs) + 1u) & 1u, status)) break;
-            tc_fence_after();
-            const uint64_t wd = desc0 + (uint64_t) (st * (L::kStage >> 4)), xd = wd + (L::kW >> 4);
-            if (elect_lane()) {
+            ok = mbar_poll2_lanes(&S.xfull[b], (s / kBufs) & 1u, &S.tempty[b], ((s / kBufs) + 1u) & 1u, status);
 #pragma unroll
-                for (int mat = 0; mat < kMats; ++mat)
+            for (int mat = 0; mat < kMats; ++mat) {
+                ok = ok && mbar_poll_lanes(&S.wfull[slot], wpar, status);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t wd = wdesc0 + (uint64_t) (slot * (L::kSlot >> 4));
+                const uint64_t xd = PH == 0 ? xdesc0 + (uint64_t) (b * (L::kX >> 4)) : wd + (kFp8WTile >> 4);
+                if (elect_lane()) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        tc_mma_f8(tmem + (b * kMats + mat) * NT, wd + mat * (kFp8WTile >> 4) + 2 * q, xd + 2 * q, id, q);
-                tc_commit(&S.empty[st]);
-                tc_commit(&S.tfull[b]);
+                    for (int q = 0; q < 4; ++q) tc_mma_f8(tmem + (b * kMats + mat) * NT, wd + 2 * q, xd + 2 * q, id, q);
+                    tc_commit(&S.wdone[slot]);
+                    if (mat + 1 == kMats) tc_commit(&S.tfull[b]);
+                }
+                if (++slot == W) { slot = 0; wpar ^= 1u; }
             }
         }
     } else if (warp >= 4) {
         const int xw = warp - 4;
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
         if (PH == 0) {
-            // quantise the group's rows of x, one warp a row, 4 elements a lane
+            // Quantise the group's rows of x, four a warp; which four goes round
+            // with the steps, so that few rows keep all warps busy.
             if (cta == 0)
                 for (int i = tid - 128; i < NBH; i += 128) p.ctrl[kFmCntB + i] = 0u;   // kernel 2's counters
-            const int k4 = lane * 4;
-            auto fetch = [&](const FmAt<PH>& at, int r) {
-                const int tok = P.slot[P.gstart[at.g] + r] / p.topk;
-                const int64_t i = (int64_t) tok * p.H + at.kb * 128 + k4;
-                return p.xvec ? load_raw4(p.x, p.x_dtype, i) : load_raw4_tail(p.x, p.x_dtype, i, 4);
+            XRows next[2];                                    // the next rows of this warp, fetched ahead
+            FmAt<PH> f = a;
+            int fs = 0, fq = xw;
+            auto fetch = [&](XRows& to) {
+                while (fs < nsteps && fq * 4 >= P.gstart[f.g + 1] - P.gstart[f.g]) {
+                    ++fs;
+                    f.next();
+                    fq = (xw + fs) & 3;
+                }
+                if (fs >= nsteps) return;
+                const int p0 = P.gstart[f.g] + fq * 4, cnt = min(4, P.gstart[f.g + 1] - p0), lr = XRows::row(cnt, lane);
+                const int tok = P.slot[p0 + min(lr, cnt - 1)] / p.topk;
+                to.load(cnt, p.x, p.x_dtype, (int64_t) tok * p.H + f.kb * 128 + XRows::col(cnt, lane), lr < cnt ? 16 : 0, p.xvec);
+                fq += 4;
             };
-            uint4 next = make_uint4(0u, 0u, 0u, 0u);
-            if (nsteps > 0 && (xw & 3) < P.gstart[a.g + 1] - P.gstart[a.g]) next = fetch(a, xw & 3);
-            for (int s = 0; s < nsteps; ++s) {
-                const int st = s % sm, n = P.gstart[a.g + 1] - P.gstart[a.g];
-                FmAt<PH> b = a;
-                b.next();
-                // rows go round the warps, so that few rows keep all of them busy
-                const int r0 = (xw + s) & 3, r1 = (xw + s + 1) & 3;
-                uint4 raw = next;
-                if (s + 1 < nsteps && r1 < P.gstart[b.g + 1] - P.gstart[b.g]) next = fetch(b, r1);
-                bool ok = true;
-                if (r0 < n) {
-                    for (int r = r0; r < n; r += 4) {
-                        float v[4];
-                        unpack4(raw, p.x_dtype, v);
-                        if (r + 4 < n) raw = fetch(a, r + 4);
-                        const float sx = fp8_scale(__reduce_max_sync(0xffffffffu, abs_bits4(v)), p.pow2);
-                        const uint32_t q = fp8_quant4(v, sx, __frcp_rn(sx), p.pow2);
-                        if (r == r0) ok = mbar_wait_lanes(&S.empty[st], ((s / sm) + 1u) & 1u, status);
-                        if (!ok) break;
-                        *reinterpret_cast<uint32_t*>(ring + st * L::kStage + L::kW + sw128_byte(r, k4)) = q;
-                        if (lane == 0) S.fac[st][r] = sx;
-                    }
-                } else {
-                    ok = mbar_wait_lanes(&S.empty[st], ((s / sm) + 1u) & 1u, status);
+            fetch(next[0]);
+            fetch(next[1]);
+            for (int s = 0; s < nsteps; ++s, a.next()) {
+                const int b = s % kBufs, n = P.gstart[a.g + 1] - P.gstart[a.g], q0 = (xw + s) & 3;
+                uint8_t* tile = xring + b * L::kX;
+                float* fac = S.fac[s % kFacs];
+                float ws = 0.f;
+                if (q0 == 0 && lane < 2)
+                    ws = __ldg(p.w13s + ((int64_t) P.pexp[P.gstart[a.g]] * 2 * NBI + lane * NBI + a.tile % NBI) * NBH + a.kb);
+                bool free = false;
+                for (int q = q0; q * 4 < n; q += 4) {
+                    const XRows cur = next[0];
+                    next[0] = next[1];
+                    fetch(next[1]);
+                    const int cnt = min(4, n - q * 4), lr = XRows::row(cnt, lane);
+                    float sx;
+                    const uint4 v = cur.quantize(cnt, p.x_dtype, p.pow2, sx);
+                    if (!free && !(free = mbar_wait_lanes(&S.tfull[b], ((s / kBufs) + 1u) & 1u, status))) break;
+                    if (lr < cnt) XRows::store(cnt, tile, q * 4 + lr, lane, v);
+                    if (lr < cnt && (cnt == 1 ? lane == 0 : (lane & 7) == 0)) fac[q * 4 + lr] = sx;
                 }
-                if (!ok) break;
-                if (r0 == 0 && lane < 2) {
-                    const int e = P.pexp[P.gstart[a.g]];
-                    S.wsc[st][lane] = __ldg(p.w13s + ((int64_t) e * 2 * NBI + lane * NBI + a.tile % NBI) * NBH + a.kb);
-                }
+                if (!free && !mbar_wait_lanes(&S.tfull[b], ((s / kBufs) + 1u) & 1u, status)) break;
+                if (q0 == 0 && lane < 2) S.wsc[s % kFacs][lane] = ws;
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&S.full[st]);
-                a = b;
+                if (lane == 0) mbar_arrive(&S.xfull[b]);
             }
         } else {
-            // scales of the down input, the weight block and the route, one warp a block
+            // scales of the down input, the weight block and the route, one warp a step
             pdl_wait();
             for (int i = cta * 128 + tid - 128; i < G * NBI; i += C * 128) p.ctrl[kFmCntA + i] = 0u;   // kernel 1's
             for (int q = 0; q < xw && q < nsteps; ++q) a.next();
             for (int s = xw; s < nsteps; s += 4) {
-                const int st = s % sm, p0 = P.gstart[a.g], n = P.gstart[a.g + 1] - p0, e = P.pexp[p0];
+                const int b = s % kBufs, p0 = P.gstart[a.g], n = P.gstart[a.g + 1] - p0, e = P.pexp[p0];
                 const float ws = __ldg(p.w2s + ((int64_t) e * NBH + a.tile) * NBI + a.kb);
                 float f[(NT + 31) / 32];
 #pragma unroll
@@ -335,12 +351,12 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                     const int j = h * 32 + lane;
                     f[h] = j < n ? __ldcg(p.as + (int64_t) (p0 + j) * NBI + a.kb) * ws * route_weight(p.route, P.slot[p0 + j]) : 0.f;
                 }
-                if (!mbar_wait_lanes(&S.empty[st], ((s / sm) + 1u) & 1u, status)) break;
+                if (!mbar_wait_lanes(&S.tfull[b], ((s / kBufs) + 1u) & 1u, status)) break;
 #pragma unroll
                 for (int h = 0; h < (NT + 31) / 32; ++h)
-                    if (h * 32 + lane < NT) S.fac[st][h * 32 + lane] = f[h];
+                    if (h * 32 + lane < NT) S.fac[s % kFacs][h * 32 + lane] = f[h];
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&S.full[st]);
+                if (lane == 0) mbar_arrive(&S.xfull[b]);
                 for (int q = 0; q < 4; ++q) a.next();
             }
         }
@@ -353,14 +369,14 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[mat][j] = 0.f;
         };
-        // Counts this CTA's blocks of an output tile; true in the CTA that completes it.
-        auto completes = [&](int counter, int blocks) {
+        // Counts this CTA's steps of an output tile; true in the CTA that completes it.
+        auto completes = [&](int counter, int steps) {
             epi_sync();
-            if (tid == 0) S.last = atom_add_acq_rel_gpu(&p.ctrl[counter], (uint32_t) blocks) + blocks == (uint32_t) per_tile;
+            if (tid == 0) S.last = atom_add_acq_rel_gpu(&p.ctrl[counter], (uint32_t) steps) + steps == (uint32_t) per_tile;
             epi_sync();
             return S.last != 0u;
         };
-        // a tile's part: slot 1 where the tile began before this CTA's range did not
+        // a tile's part: slot 1 where the CTA's range began before the tile did
         const int rows_pt = PH == 0 ? kMats * NT : p.m;               // rows of 128 in a part
         auto part_of = [&](int c, int first) { return p.part + ((int64_t) c * 2 + (fm_start(c, C, total) >= first ? 0 : 1)) * rows_pt * 128; };
         if (PH == 1) {
@@ -372,55 +388,62 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
         }
         clear();
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
-        int seg = 0;                                                  // blocks of the current tile so far
+        int seg = 0;                                                  // steps of the current tile so far
         for (int s = 0; s < nsteps; ++s) {
-            const int st = s % sm, b = s % L::kBufs;
+            const int b = s % kBufs;
             const int p0 = P.gstart[a.g], n = P.gstart[a.g + 1] - p0;
-            if (!mbar_wait_lanes(&S.tfull[b], (s / L::kBufs) & 1u, status)) break;
+            if (!mbar_wait_lanes(&S.tfull[b], (s / kBufs) & 1u, status)) break;
             tc_fence_after();
 #pragma unroll
             for (int mat = 0; mat < kMats; ++mat) {
-                const float ws = PH == 0 ? S.wsc[st][mat] : 1.f;
+                const float ws = PH == 0 ? S.wsc[s % kFacs][mat] : 1.f;
+                const float4* f4 = reinterpret_cast<const float4*>(S.fac[s % kFacs]);
 #pragma unroll
                 for (int c = 0; c < NT / 16; ++c) {
                     if (c * 16 >= n) break;
                     float v[16];
                     tc_ld16(tmem + ((uint32_t) (warp * 32) << 16) + (uint32_t) ((b * kMats + mat) * NT + c * 16), v);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float f = PH == 0 ? S.fac[st][c * 16 + j] * ws : S.fac[st][c * 16 + j];
-                        acc[mat][c * 16 + j] = fmaf(v[j], f, acc[mat][c * 16 + j]);
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 f = f4[c * 4 + q];
+                        float* o = &acc[mat][c * 16 + q * 4];
+                        o[0] = fmaf(v[q * 4 + 0], f.x * ws, o[0]);
+                        o[1] = fmaf(v[q * 4 + 1], f.y * ws, o[1]);
+                        o[2] = fmaf(v[q * 4 + 2], f.z * ws, o[2]);
+                        o[3] = fmaf(v[q * 4 + 3], f.w * ws, o[3]);
                     }
                 }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&S.tempty[b]);
-                mbar_arrive(&S.empty[st]);
-            }
+            if (lane == 0) mbar_arrive(&S.tempty[b]);
             ++seg;
             const bool tile_end = (PH == 0 ? a.kb + 1 == KB : (a.kb + 1 == KB && a.g + 1 == G)) || s + 1 == nsteps;
             if (PH == 1 && (a.kb + 1 == KB || s + 1 == nsteps)) {
                 // the group's columns go to their tokens
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    if (j < n) oacc[(P.slot[p0 + j] / p.topk) * 128 + tid] += acc[0][j];
+                for (int j = 0; j < NT; ++j) {
+                    if (j >= n) break;
+                    oacc[(P.slot[p0 + j] / p.topk) * 128 + tid] += acc[0][j];
+                }
                 clear();
             }
             if (tile_end) {
-                const int first = a.tile * per_tile;                  // the tile's first block
-                bool whole = seg == per_tile, finish = whole;
-                if (!whole) {
+                const int first = a.tile * per_tile;                  // the tile's first step
+                bool finish = seg == per_tile;
+                if (!finish) {
                     float* dst = part_of(cta, first);
                     if (PH == 0) {
 #pragma unroll
-                        for (int mat = 0; mat < kMats; ++mat)
+                        for (int c = 0; c < NT / kCh; ++c) {
+                            if (c * kCh >= n) break;
 #pragma unroll
-                            for (int j = 0; j < NT; ++j)
-                                if (j < n) dst[(mat * NT + j) * 128 + tid] = acc[mat][j];
+                            for (int j = c * kCh; j < (c + 1) * kCh; ++j)
+#pragma unroll
+                                for (int mat = 0; mat < kMats; ++mat) __stcg(dst + (mat * NT + j) * 128 + tid, acc[mat][j]);
+                        }
                     } else {
-                        for (int t = 0; t < p.m; ++t) dst[t * 128 + tid] = oacc[t * 128 + tid];
+                        for (int t = 0; t < p.m; ++t) __stcg(dst + t * 128 + tid, oacc[t * 128 + tid]);
                     }
                     finish = completes((PH == 0 ? kFmCntA : kFmCntB) + a.tile, seg);
                     if (finish) {
@@ -432,39 +455,64 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                             const float* src = part_of(c, first);
                             if (PH == 0) {
 #pragma unroll
-                                for (int mat = 0; mat < kMats; ++mat)
+                                for (int h = 0; h < NT / kCh; ++h) {
+                                    if (h * kCh >= n) break;
+                                    float v[kMats][kCh];              // all of them on their way together
 #pragma unroll
-                                    for (int j = 0; j < NT; ++j)
-                                        if (j < n) acc[mat][j] += __ldcg(src + (mat * NT + j) * 128 + tid);
+                                    for (int j = 0; j < kCh; ++j)
+#pragma unroll
+                                        for (int mat = 0; mat < kMats; ++mat) v[mat][j] = __ldcg(src + (mat * NT + h * kCh + j) * 128 + tid);
+#pragma unroll
+                                    for (int j = 0; j < kCh; ++j)
+#pragma unroll
+                                        for (int mat = 0; mat < kMats; ++mat) acc[mat][h * kCh + j] += v[mat][j];
+                                }
                             } else {
-                                for (int t = 0; t < p.m; ++t) oacc[t * 128 + tid] += __ldcg(src + t * 128 + tid);
+                                for (int t = 0; t < p.m; t += 4) {
+                                    float v[4];
+#pragma unroll
+                                    for (int q = 0; q < 4; ++q) v[q] = t + q < p.m ? __ldcg(src + (t + q) * 128 + tid) : 0.f;
+#pragma unroll
+                                    for (int q = 0; q < 4; ++q)
+                                        if (t + q < p.m) oacc[(t + q) * 128 + tid] += v[q];
+                                }
                             }
                         }
                     }
                 }
                 if (finish && PH == 0) {
-                    // SwiGLU, then one scale for each token's 128 columns; NaN passes through
+                    // SwiGLU, then one scale for each token's 128 columns; NaN passes
+                    // through.  kCh columns at a time: columns behind the group's last
+                    // are computed with them and never stored.
                     const int ib = a.tile % NBI;
                     const float lim = p.limit;
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        if (j >= n) break;
-                        float g = acc[0][j], u = acc[kMats - 1][j];
-                        g = g > lim ? lim : g;
-                        u = u > lim ? lim : u < -lim ? -lim : u;
-                        acc[0][j] = g / (1.f + expf(-g)) * u;
-                        const uint32_t mx = __reduce_max_sync(0xffffffffu, abs_bits(acc[0][j]));
-                        if (lane == 0) S.wmax[warp][j] = mx;
+                    for (int c = 0; c < NT / kCh; ++c) {
+                        if (c * kCh >= n) break;
+#pragma unroll
+                        for (int j = c * kCh; j < (c + 1) * kCh; ++j) {
+                            float g = acc[0][j], u = acc[kMats - 1][j];
+                            g = g > lim ? lim : g;
+                            u = u > lim ? lim : u < -lim ? -lim : u;
+                            acc[0][j] = g / (1.f + expf(-g)) * u;
+                            const uint32_t mx = __reduce_max_sync(0xffffffffu, abs_bits(acc[0][j]));
+                            if (lane == 0) S.wmax[warp][j] = mx;
+                        }
                     }
                     epi_sync();
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        if (j >= n) break;
-                        const uint32_t mx = max(max(S.wmax[0][j], S.wmax[1][j]), max(S.wmax[2][j], S.wmax[3][j]));
-                        const float sa = fp8_scale(mx, p.pow2);
-                        p.aq[(int64_t) (p0 + j) * p.I + ib * 128 + tid] =
-                            (uint8_t) e4m3x2(fp8_quotient(acc[0][j], sa, __frcp_rn(sa), p.pow2), 0.f);
-                        if (tid == 0) p.as[(int64_t) (p0 + j) * NBI + ib] = sa;
+                    for (int c = 0; c < NT / kCh; ++c) {
+                        if (c * kCh >= n) break;
+#pragma unroll
+                        for (int j = c * kCh; j < (c + 1) * kCh; ++j) {
+                            const uint32_t mx = max(max(S.wmax[0][j], S.wmax[1][j]), max(S.wmax[2][j], S.wmax[3][j]));
+                            const float sa = fp8_scale(mx, p.pow2);
+                            const uint32_t q = e4m3x2(fp8_quotient(acc[0][j], sa, __frcp_rn(sa), p.pow2), 0.f);
+                            if (j < n) {
+                                p.aq[(int64_t) (p0 + j) * p.I + ib * 128 + tid] = (uint8_t) q;
+                                if (tid == 0) p.as[(int64_t) (p0 + j) * NBI + ib] = sa;
+                            }
+                        }
                     }
                     epi_sync();                                       // wmax is free for the next tile
                 }
@@ -513,11 +561,11 @@ int fm_launch(FmParams p, int sms, cudaStream_t stream) {
     // Up to 32 rows the two kernels share an SM while kernel 2 waits (shared
     // memory 120 + 104 KB); above that their registers leave room for one.
     constexpr int kBudget = (NT > 32 ? 200 : PH == 0 ? 120 : 104) * 1024;
-    const int extra = 1024 + (int) sizeof(FmHead<NT>) + (PH == 1 ? p.m * 512 : 0);
-    int stages = (kBudget - extra) / L::kStage;
-    if (stages > kFmMaxStages) stages = kFmMaxStages;
-    p.stages = stages;
-    const int smem = extra + stages * L::kStage;
+    const int extra = 1024 + (int) sizeof(FmHead<NT>) + L::kXRing + (PH == 1 ? p.m * 512 : 0);
+    int slots = (kBudget - extra) / L::kSlot;
+    if (slots > kFmMaxSlotsW) slots = kFmMaxSlotsW;
+    p.slots = slots;
+    const int smem = extra + slots * L::kSlot;
     static std::once_flag once[64];
     int dev = 0;
     EXL3_CUDA(cudaGetDevice(&dev));
@@ -603,7 +651,7 @@ extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, void* out, int ou
     p.route = RouteIn{route->ids, route->weights, route->expert_map, route->n_global, route->ids_dtype, route->weights_dtype};
     p.limit = swiglu_limit;
     p.x_dtype = x_dtype; p.out_dtype = out_dtype; p.pow2 = pow2 != 0;
-    p.xvec = reinterpret_cast<uintptr_t>(x) % (x_dtype == 2 ? 16 : 8) == 0;
+    p.xvec = aligned16(x);
     p.m = (int) m; p.topk = (int) topk; p.E = (int) n_experts; p.H = (int) hidden; p.I = (int) inter;
     auto s = static_cast<cudaStream_t>(stream);
     if (g.nt == 16) return fm_run<16>(p, di.sms, s);
