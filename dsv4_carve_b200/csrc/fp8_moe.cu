@@ -30,6 +30,8 @@
 namespace exl3 {
 
 int fp8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, const char* what);
+int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
+                        float* scale, int64_t sr, int64_t sg, int block_rows, bool pow2, cudaStream_t s);
 
 constexpr int kFmMaxRows = 64;
 constexpr int kFmMaxSlots = 256;             // m * topk
@@ -37,9 +39,17 @@ constexpr int kFmMaxTopk = 16;
 constexpr int kFmMaxInter = 8192;
 constexpr int kFmMaxHidden = 16384;
 constexpr int kFmMaxCtas = 160;
-constexpr int kFmThreads = 320;              // warps 0-3 epilogue, 4-7 x, 8 producer, 9 MMA
-constexpr int kFmProducerWarp = 8;
-constexpr int kFmMmaWarp = 9;
+// Warps 0-3 epilogue, 4 producer, 5 MMA, 6-7 x.  Two warps on each of an SM's
+// four register files: CTAs of both kernels fit side by side (kernel 2 waits
+// there, its ring filled), which three would not.
+constexpr int kFmThreads = 256;
+constexpr int kFmProducerWarp = 4;
+constexpr int kFmMmaWarp = 5;
+constexpr int kFmXWarp = 6;
+constexpr int kFmXWarps = 2;
+// Rows up to which kernel 1 quantises the rows of x that it multiplies itself;
+// above, a launch of the quantiser does it once for all CTAs.
+constexpr int kFmInlineRows = 16;
 constexpr int kFmMaxSlotsW = 12;             // weight blocks in the ring
 constexpr int kFmMaxBufs = 4;                // steps whose sums and inputs are held
 // Control region (uint32 words): [2] status; counters of kernel 1's output
@@ -53,10 +63,12 @@ struct FmParams {
     CUtensorMap w13;             // [E * 2 I][H], box 128 x 128
     CUtensorMap w2;              // [E * H][I], box 128 x 128
     CUtensorMap amap;            // down input [slots][I], box 128 x NT
+    CUtensorMap xmap;            // more than kFmInlineRows rows: x in e4m3 [m][H], box 128 x NT
     const void* x;
     void* out;
     const float* w13s;           // [E][2 I / 128][H / 128]
     const float* w2s;            // [E][H / 128][I / 128]
+    const float* xs;             // its scales [H / 128][m]
     uint8_t* aq;                 // [slots][I] e4m3
     float* as;                   // [slots][I / 128]
     float* part;                 // partial sums of the CTAs' first and last tiles
@@ -80,18 +92,21 @@ struct FmPlan {
 };
 
 // Shared memory of a CTA: a ring of weight blocks (16 KB each, so that few bytes
-// wait while many are in flight; kernel 2: with the NT input rows of the block),
-// kernel 1's quantised x of kBufs steps, the head, kernel 2's output rows.
-// A step is one block of k: kernel 1 multiplies the gate and the up block, each
-// into TMEM columns of its own, kernel 2 the down block.
+// wait while many are in flight; with the NT input rows of the block where TMA
+// brings them), kernel 1's own quantised rows of x of kBufs steps, the head,
+// kernel 2's output rows.  A step is one block of k: kernel 1 multiplies the gate
+// and the up block, each into TMEM columns of its own, kernel 2 the down block.
+// D's columns are the group's pairs, or all tokens where kernel 1's x comes
+// quantised (NT > 16): columns of other tokens are never used.
 template <int NT, int PH>
 struct FmLayout {
+    static constexpr bool kInline = PH == 0 && NT <= kFmInlineRows;
     static constexpr int kMats = PH == 0 ? 2 : 1;
     static constexpr int kBufs = NT <= 16 ? 4 : PH == 0 ? 2 : NT <= 32 ? 4 : 2;
     static constexpr int kTmemCols = NT * kMats * kBufs;             // 64 .. 256
     static constexpr int kX = NT * 128;
-    static constexpr int kSlot = (int) kFp8WTile + (PH == 0 ? 0 : kX);
-    static constexpr int kXRing = PH == 0 ? kBufs * kX : 0;
+    static constexpr int kSlot = (int) kFp8WTile + (kInline ? 0 : kX);
+    static constexpr int kXRing = kInline ? kBufs * kX : 0;
 };
 
 template <int NT>
@@ -107,6 +122,7 @@ struct FmHead {
     alignas(16) float fac[2 * kFmMaxBufs][NT];
     float wsc[2 * kFmMaxBufs][2];
     alignas(16) uint32_t wmax[4][NT];
+    short tokpair[NT];                   // a token's first pair in the group
     uint32_t tmem;
     uint32_t last;
 };
@@ -116,15 +132,14 @@ __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" :::
 // Every thread of the CTA calls this; ends with a barrier.
 __device__ void fm_plan(FmPlan& P, const FmParams& p, int nt, int tid) {
     const int n = p.m * p.topk;
+    static_assert(kFmThreads == kFmMaxSlots, "every slot has its own thread");
     int id = INT32_MAX;
-    if (tid < kFmMaxSlots) {
-        if (tid < n) {
-            const int e = route_local_id(p.route, tid, p.E);
-            if (e >= 0) id = e;
-        }
-        P.id[tid] = id;
-        P.first[tid] = 0;
+    if (tid < n) {
+        const int e = route_local_id(p.route, tid, p.E);
+        if (e >= 0) id = e;
     }
+    P.id[tid] = id;
+    P.first[tid] = 0;
     const int pairs = __syncthreads_count(id != INT32_MAX);
     if (id != INT32_MAX) {
         int before = 0, rank = 0;
@@ -143,11 +158,11 @@ __device__ void fm_plan(FmPlan& P, const FmParams& p, int nt, int tid) {
         P.first[before] = rank % nt == 0;
     }
     __syncthreads();
-    const bool f = tid < kFmMaxSlots && P.first[tid] != 0;
+    const bool f = P.first[tid] != 0;
     const uint32_t mask = __ballot_sync(0xffffffffu, f);
-    if (tid < kFmMaxSlots && (tid & 31) == 0) P.wsum[tid >> 5] = __popc(mask);
+    if ((tid & 31) == 0) P.wsum[tid >> 5] = __popc(mask);
     __syncthreads();
-    if (tid < kFmMaxSlots) {
+    {
         int g = __popc(mask & ((1u << (tid & 31)) - 1u)), total = 0;
         for (int w = 0; w < 8; ++w) {
             g += w < (tid >> 5) ? P.wsum[w] : 0;
@@ -159,9 +174,11 @@ __device__ void fm_plan(FmPlan& P, const FmParams& p, int nt, int tid) {
     __syncthreads();
 }
 
-// Equal ranges: CTA c of C has blocks [start(c), start(c + 1)) of `total`.
-__device__ __forceinline__ int fm_start(int c, int C, int total) { return (int) ((int64_t) c * total / C); }
-__device__ __forceinline__ int fm_owner(int t, int C, int total) { return (int) (((int64_t) (t + 1) * C - 1) / total); }
+// Equal ranges: CTA c of C has steps [start(c), start(c + 1)) of `total`, at most
+// 256 groups x 64 x 128 blocks, so the products stay below 2^32.
+static_assert((int64_t) kFmMaxSlots * (kFmMaxInter / 128) * (kFmMaxHidden / 128) * kFmMaxCtas < (int64_t) 1 << 32, "");
+__device__ __forceinline__ int fm_start(int c, int C, int total) { return (int) ((uint32_t) c * (uint32_t) total / (uint32_t) C); }
+__device__ __forceinline__ int fm_owner(int t, int C, int total) { return (int) (((uint32_t) (t + 1) * (uint32_t) C - 1u) / (uint32_t) total); }
 
 // The block a CTA is at, and the step to the next one.
 template <int PH>
@@ -184,6 +201,7 @@ template <int NT, int PH>
 __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_constant__ FmParams p) {
     using L = FmLayout<NT, PH>;
     constexpr int kMats = L::kMats, kBufs = L::kBufs, kFacs = 2 * L::kBufs;
+    constexpr bool kInline = L::kInline, kTokens = PH == 0 && !kInline;   // kTokens: D's columns are all tokens
     constexpr int kCh = NT < 32 ? 4 : 8;                              // columns handled together at a tile's end
     extern __shared__ uint8_t fm_raw[];
     uint8_t* ring = fm_raw + ((1024u - (smem_u32(fm_raw) & 1023u)) & 1023u);
@@ -200,7 +218,7 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
         tmap_prefetch(PH == 0 ? &p.w13 : &p.w2);
         for (int s = 0; s < W; ++s) { mbar_init(&S.wfull[s], 1); mbar_init(&S.wdone[s], 1); }
         for (int b = 0; b < kBufs; ++b) {
-            mbar_init(&S.xfull[b], PH == 0 ? 4 : 1);
+            mbar_init(&S.xfull[b], kInline ? kFmXWarps : 1);
             mbar_init(&S.tfull[b], 1);
             mbar_init(&S.tempty[b], 4);
         }
@@ -208,9 +226,11 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
     }
     if (warp == kFmMmaWarp) tmem_alloc(&S.tmem, L::kTmemCols);
     if (PH == 0) {
-        // Kernel 1 lets kernel 2 start only behind its own wait, so what came
-        // before the layer (the routes among it) is complete for kernel 2 too.
-        pdl_wait();
+        // Kernel 2 may start once what came before the layer (the routes among
+        // it) is complete: behind this kernel's own wait, or at once where the
+        // quantiser, an ordinary launch, ran in between.  Then only x is waited
+        // for, by those who read it.
+        if (kInline) pdl_wait();
         pdl_launch_dependents();
     }
     tc_fence_before();
@@ -233,31 +253,34 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                 tma_load_2d(ring + slot * L::kSlot, PH == 0 ? &p.w13 : &p.w2, a.kb * 128, row, &S.wfull[slot]);
             };
             auto inputs = [&](const FmAt<PH>& a, int slot) {
-                tma_load_2d(ring + slot * L::kSlot + kFp8WTile, &p.amap, a.kb * 128, P.gstart[a.g], &S.wfull[slot]);
+                if (PH == 0) tma_load_2d(ring + slot * L::kSlot + kFp8WTile, &p.xmap, a.kb * 128, 0, &S.wfull[slot]);
+                else tma_load_2d(ring + slot * L::kSlot + kFp8WTile, &p.amap, a.kb * 128, P.gstart[a.g], &S.wfull[slot]);
             };
             FmAt<PH> a(beg, G, NBI, KB);
+            auto mat_of = [](int t) { return PH == 0 ? t & 1 : 0; };
+            auto next = [&](FmAt<PH>& at, int t) { if (PH == 1 || (t & 1)) at.next(); };
             int t = 0;
-            if (PH == 1) {
-                // the weights do not depend on kernel 1: a ring of them ahead of the wait
+            if (!kInline) {
+                // a ring of weights ahead of the wait: no kernel that may still run writes them
                 FmAt<PH> a0 = a;
-                for (; t < min(W, nblk); ++t) { weights(a, 0, t); a.next(); }
+                for (; t < min(W, nblk); ++t) { weights(a, mat_of(t), t); next(a, t); }
                 pdl_wait();
                 fence_proxy_async_global();
-                for (int s = 0; s < t; ++s) { inputs(a0, s); a0.next(); }
+                for (int i = 0; i < t; ++i) { inputs(a0, i); next(a0, i); }
             }
             int issued = t;
             for (; t < nblk; ++t) {
                 const int slot = t % W;
                 if (t >= W && !mbar_wait(&S.wdone[slot], ((t / W) + 1u) & 1u, status)) break;
-                weights(a, PH == 0 ? t & 1 : 0, slot);
-                if (PH == 1) inputs(a, slot);
-                if (PH == 1 || (t & 1)) a.next();
+                weights(a, mat_of(t), slot);
+                if (!kInline) inputs(a, slot);
+                next(a, t);
                 ++issued;
             }
             // no copy may still be in flight when the CTA retires
             for (int i = max(0, issued - W); i < issued; ++i)
                 if (!mbar_wait(&S.wfull[i % W], (i / W) & 1u, status)) break;
-        } else if (PH == 1) {
+        } else if (!kInline) {
             pdl_wait();
         }
     } else if (warp == kFmMmaWarp) {
@@ -268,7 +291,7 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
         bool ok = true;
         for (int s = 0; s < nsteps && ok; ++s, a.next()) {
             const int b = s % kBufs;
-            const int n = P.gstart[a.g + 1] - P.gstart[a.g];
+            const int n = kTokens ? p.m : P.gstart[a.g + 1] - P.gstart[a.g];
             const uint32_t id = __shfl_sync(0xffffffffu, idesc_f16(128, (n + 15) & ~15), 0);
             ok = mbar_poll2_lanes(&S.xfull[b], (s / kBufs) & 1u, &S.tempty[b], ((s / kBufs) + 1u) & 1u, status);
 #pragma unroll
@@ -277,7 +300,7 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t wd = wdesc0 + (uint64_t) (slot * (L::kSlot >> 4));
-                const uint64_t xd = PH == 0 ? xdesc0 + (uint64_t) (b * (L::kX >> 4)) : wd + (kFp8WTile >> 4);
+                const uint64_t xd = kInline ? xdesc0 + (uint64_t) (b * (L::kX >> 4)) : wd + (kFp8WTile >> 4);
                 if (elect_lane()) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) tc_mma_f8(tmem + (b * kMats + mat) * NT, wd + 2 * q, xd + 2 * q, id, q);
@@ -287,14 +310,14 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                 if (++slot == W) { slot = 0; wpar ^= 1u; }
             }
         }
-    } else if (warp >= 4) {
-        const int xw = warp - 4;
+    } else if (warp >= kFmXWarp) {
+        const int xw = warp - kFmXWarp, xt = tid - kFmXWarp * 32;
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
-        if (PH == 0) {
+        if (PH == 0 && cta == 0)
+            for (int i = xt; i < NBH; i += 32 * kFmXWarps) p.ctrl[kFmCntB + i] = 0u;   // kernel 2's counters
+        if (kInline) {
             // Quantise the group's rows of x, four a warp; which four goes round
-            // with the steps, so that few rows keep all warps busy.
-            if (cta == 0)
-                for (int i = tid - 128; i < NBH; i += 128) p.ctrl[kFmCntB + i] = 0u;   // kernel 2's counters
+            // with the steps, so that few rows keep both warps busy.
             XRows next[2];                                    // the next rows of this warp, fetched ahead
             FmAt<PH> f = a;
             int fs = 0, fq = xw;
@@ -302,25 +325,25 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                 while (fs < nsteps && fq * 4 >= P.gstart[f.g + 1] - P.gstart[f.g]) {
                     ++fs;
                     f.next();
-                    fq = (xw + fs) & 3;
+                    fq = (xw + fs) % kFmXWarps;
                 }
                 if (fs >= nsteps) return;
                 const int p0 = P.gstart[f.g] + fq * 4, cnt = min(4, P.gstart[f.g + 1] - p0), lr = XRows::row(cnt, lane);
                 const int tok = P.slot[p0 + min(lr, cnt - 1)] / p.topk;
                 to.load(cnt, p.x, p.x_dtype, (int64_t) tok * p.H + f.kb * 128 + XRows::col(cnt, lane), lr < cnt ? 16 : 0, p.xvec);
-                fq += 4;
+                fq += kFmXWarps;
             };
             fetch(next[0]);
             fetch(next[1]);
             for (int s = 0; s < nsteps; ++s, a.next()) {
-                const int b = s % kBufs, n = P.gstart[a.g + 1] - P.gstart[a.g], q0 = (xw + s) & 3;
+                const int b = s % kBufs, n = P.gstart[a.g + 1] - P.gstart[a.g], q0 = (xw + s) % kFmXWarps;
                 uint8_t* tile = xring + b * L::kX;
                 float* fac = S.fac[s % kFacs];
                 float ws = 0.f;
                 if (q0 == 0 && lane < 2)
                     ws = __ldg(p.w13s + ((int64_t) P.pexp[P.gstart[a.g]] * 2 * NBI + lane * NBI + a.tile % NBI) * NBH + a.kb);
                 bool free = false;
-                for (int q = q0; q * 4 < n; q += 4) {
+                for (int q = q0; q * 4 < n; q += kFmXWarps) {
                     const XRows cur = next[0];
                     next[0] = next[1];
                     fetch(next[1]);
@@ -338,26 +361,34 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(&S.xfull[b]);
             }
         } else {
-            // scales of the down input, the weight block and the route, one warp a step
+            // The factors of a step's columns, one warp a step: x's scales and the two
+            // blocks' (kernel 1), or the down input's, the block's and the route's.
             pdl_wait();
-            for (int i = cta * 128 + tid - 128; i < G * NBI; i += C * 128) p.ctrl[kFmCntA + i] = 0u;   // kernel 1's
+            if (PH == 1) {
+                for (int i = cta * 32 * kFmXWarps + xt; i < G * NBI; i += C * 32 * kFmXWarps) p.ctrl[kFmCntA + i] = 0u;   // kernel 1's
+            }
             for (int q = 0; q < xw && q < nsteps; ++q) a.next();
-            for (int s = xw; s < nsteps; s += 4) {
-                const int b = s % kBufs, p0 = P.gstart[a.g], n = P.gstart[a.g + 1] - p0, e = P.pexp[p0];
-                const float ws = __ldg(p.w2s + ((int64_t) e * NBH + a.tile) * NBI + a.kb);
+            for (int s = xw; s < nsteps; s += kFmXWarps) {
+                const int b = s % kBufs, p0 = P.gstart[a.g], n = PH == 0 ? p.m : P.gstart[a.g + 1] - p0, e = P.pexp[p0];
+                float ws = 0.f;
+                if (PH == 1) ws = __ldg(p.w2s + ((int64_t) e * NBH + a.tile) * NBI + a.kb);
+                else if (lane < 2) ws = __ldg(p.w13s + ((int64_t) e * 2 * NBI + lane * NBI + a.tile % NBI) * NBH + a.kb);
                 float f[(NT + 31) / 32];
 #pragma unroll
                 for (int h = 0; h < (NT + 31) / 32; ++h) {
                     const int j = h * 32 + lane;
-                    f[h] = j < n ? __ldcg(p.as + (int64_t) (p0 + j) * NBI + a.kb) * ws * route_weight(p.route, P.slot[p0 + j]) : 0.f;
+                    f[h] = 0.f;
+                    if (j < n) f[h] = PH == 0 ? __ldcg(p.xs + (int64_t) a.kb * p.m + j)
+                                              : __ldcg(p.as + (int64_t) (p0 + j) * NBI + a.kb) * ws * route_weight(p.route, P.slot[p0 + j]);
                 }
                 if (!mbar_wait_lanes(&S.tfull[b], ((s / kBufs) + 1u) & 1u, status)) break;
 #pragma unroll
                 for (int h = 0; h < (NT + 31) / 32; ++h)
                     if (h * 32 + lane < NT) S.fac[s % kFacs][h * 32 + lane] = f[h];
+                if (PH == 0 && lane < 2) S.wsc[s % kFacs][lane] = ws;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S.xfull[b]);
-                for (int q = 0; q < 4; ++q) a.next();
+                for (int q = 0; q < kFmXWarps; ++q) a.next();
             }
         }
     } else {
@@ -391,7 +422,7 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
         int seg = 0;                                                  // steps of the current tile so far
         for (int s = 0; s < nsteps; ++s) {
             const int b = s % kBufs;
-            const int p0 = P.gstart[a.g], n = P.gstart[a.g + 1] - p0;
+            const int p0 = P.gstart[a.g], pairs = P.gstart[a.g + 1] - p0, n = kTokens ? p.m : pairs;   // n: D's columns
             if (!mbar_wait_lanes(&S.tfull[b], (s / kBufs) & 1u, status)) break;
             tc_fence_after();
 #pragma unroll
@@ -431,12 +462,19 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
             if (tile_end) {
                 const int first = a.tile * per_tile;                  // the tile's first step
                 bool finish = seg == per_tile;
+                // the columns that the group has, a bit each
+                uint64_t have = n < 64 ? (1ull << n) - 1ull : ~0ull;
+                if (kTokens) {
+                    have = 0;
+                    for (int j = 0; j < pairs; ++j) have |= 1ull << (P.slot[p0 + j] / p.topk);
+                }
+                auto chunk = [&](int c) { return (have >> (c * kCh) & ((1ull << kCh) - 1ull)) != 0; };
                 if (!finish) {
                     float* dst = part_of(cta, first);
                     if (PH == 0) {
 #pragma unroll
                         for (int c = 0; c < NT / kCh; ++c) {
-                            if (c * kCh >= n) break;
+                            if (!chunk(c)) continue;
 #pragma unroll
                             for (int j = c * kCh; j < (c + 1) * kCh; ++j)
 #pragma unroll
@@ -456,7 +494,7 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                             if (PH == 0) {
 #pragma unroll
                                 for (int h = 0; h < NT / kCh; ++h) {
-                                    if (h * kCh >= n) break;
+                                    if (!chunk(h)) continue;
                                     float v[kMats][kCh];              // all of them on their way together
 #pragma unroll
                                     for (int j = 0; j < kCh; ++j)
@@ -486,9 +524,14 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                     // are computed with them and never stored.
                     const int ib = a.tile % NBI;
                     const float lim = p.limit;
+                    if (kTokens)
+                        for (int j = tid; j < pairs; j += 128) {
+                            const int t = P.slot[p0 + j] / p.topk;
+                            if (j == 0 || P.slot[p0 + j - 1] / p.topk != t) S.tokpair[t] = (short) (p0 + j);
+                        }
 #pragma unroll
                     for (int c = 0; c < NT / kCh; ++c) {
-                        if (c * kCh >= n) break;
+                        if (!chunk(c)) continue;
 #pragma unroll
                         for (int j = c * kCh; j < (c + 1) * kCh; ++j) {
                             float g = acc[0][j], u = acc[kMats - 1][j];
@@ -502,15 +545,19 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                     epi_sync();
 #pragma unroll
                     for (int c = 0; c < NT / kCh; ++c) {
-                        if (c * kCh >= n) break;
+                        if (!chunk(c)) continue;
 #pragma unroll
                         for (int j = c * kCh; j < (c + 1) * kCh; ++j) {
                             const uint32_t mx = max(max(S.wmax[0][j], S.wmax[1][j]), max(S.wmax[2][j], S.wmax[3][j]));
                             const float sa = fp8_scale(mx, p.pow2);
                             const uint32_t q = e4m3x2(fp8_quotient(acc[0][j], sa, __frcp_rn(sa), p.pow2), 0.f);
-                            if (j < n) {
-                                p.aq[(int64_t) (p0 + j) * p.I + ib * 128 + tid] = (uint8_t) q;
-                                if (tid == 0) p.as[(int64_t) (p0 + j) * NBI + ib] = sa;
+                            if (have >> j & 1ull) {
+                                // an expert listed twice for a token has two pairs next to each other
+                                int pr = kTokens ? S.tokpair[j] : p0 + j;
+                                do {
+                                    p.aq[(int64_t) pr * p.I + ib * 128 + tid] = (uint8_t) q;
+                                    if (tid == 0) p.as[(int64_t) pr * NBI + ib] = sa;
+                                } while (kTokens && ++pr < p0 + pairs && P.slot[pr] / p.topk == j);
                             }
                         }
                     }
@@ -539,17 +586,19 @@ namespace {
 
 struct FmGeom {
     int nt;
-    int64_t off_aq, off_as, off_part, bytes;
+    int64_t off_aq, off_as, off_xq, off_xs, off_part, bytes;
 };
 
 FmGeom fm_geom(int64_t m, int64_t topk, int64_t H, int64_t I) {
     FmGeom g{};
-    (void) H;
+    const bool xq = m > kFmInlineRows;
     g.nt = m <= 16 ? 16 : m <= 32 ? 32 : 64;
     const int64_t slots = m * topk;
     g.off_aq = EXL3_FP8_MOE_CTRL_BYTES;
     g.off_as = g.off_aq + align_up(slots * I, 256);
-    g.off_part = g.off_as + align_up(slots * (I / 128) * 4, 256);
+    g.off_xq = g.off_as + align_up(slots * (I / 128) * 4, 256);
+    g.off_xs = g.off_xq + (xq ? align_up(m * H, 256) : 0);
+    g.off_part = g.off_xs + (xq ? align_up(m * (H / 128) * 4, 256) : 0);
     const int64_t part_rows = 2 * g.nt > m ? 2 * g.nt : m;
     g.bytes = g.off_part + (int64_t) kFmMaxCtas * 2 * part_rows * 128 * 4;
     return g;
@@ -558,10 +607,10 @@ FmGeom fm_geom(int64_t m, int64_t topk, int64_t H, int64_t I) {
 template <int NT, int PH>
 int fm_launch(FmParams p, int sms, cudaStream_t stream) {
     using L = FmLayout<NT, PH>;
-    // Up to 32 rows the two kernels share an SM while kernel 2 waits (shared
-    // memory 120 + 104 KB); above that their registers leave room for one.
-    constexpr int kBudget = (NT > 32 ? 200 : PH == 0 ? 120 : 104) * 1024;
+    // The two kernels share an SM while kernel 2 waits: 120 + 104 KB of its memory.
+    constexpr int kBudget = (PH == 0 ? 120 : 104) * 1024;
     const int extra = 1024 + (int) sizeof(FmHead<NT>) + L::kXRing + (PH == 1 ? p.m * 512 : 0);
+    static_assert(sizeof(FmHead<64>) + 64 * 512 + 1024 + 2 * FmLayout<64, 1>::kSlot <= 104 * 1024, "room for two blocks");
     int slots = (kBudget - extra) / L::kSlot;
     if (slots > kFmMaxSlotsW) slots = kFmMaxSlotsW;
     p.slots = slots;
@@ -645,6 +694,7 @@ extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, void* out, int ou
     if ((rc = fp8_map(&p.amap, sb + g.off_aq, m * topk, inter, inter, g.nt, "exl3_fp8_moe_decode")) != EXL3_OK) return rc;
     p.x = x; p.out = out; p.w13s = gate_up_scale; p.w2s = down_scale;
     p.aq = sb + g.off_aq;
+    p.xs = reinterpret_cast<const float*>(sb + g.off_xs);
     p.as = reinterpret_cast<float*>(sb + g.off_as);
     p.part = reinterpret_cast<float*>(sb + g.off_part);
     p.ctrl = reinterpret_cast<uint32_t*>(sb);
@@ -654,6 +704,12 @@ extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, void* out, int ou
     p.xvec = aligned16(x);
     p.m = (int) m; p.topk = (int) topk; p.E = (int) n_experts; p.H = (int) hidden; p.I = (int) inter;
     auto s = static_cast<cudaStream_t>(stream);
+    if (m > kFmInlineRows) {
+        if ((rc = fp8_map(&p.xmap, sb + g.off_xq, m, hidden, hidden, g.nt, "exl3_fp8_moe_decode")) != EXL3_OK) return rc;
+        if ((rc = fp8_quantize_launch(x, x_dtype, m, hidden, hidden, sb + g.off_xq, hidden, reinterpret_cast<float*>(sb + g.off_xs),
+                                      1, m, 1, pow2 != 0, s)) != EXL3_OK)
+            return rc;
+    }
     if (g.nt == 16) return fm_run<16>(p, di.sms, s);
     if (g.nt == 32) return fm_run<32>(p, di.sms, s);
     return fm_run<64>(p, di.sms, s);
