@@ -66,7 +66,7 @@ _SIGS = {
     "exl3_fp8_status": (_I, [_I, _P, _P]),
     "exl3_fp8_moe_scratch_bytes": (_I64, [_I64, _I64, _I64, _I64]),
     "exl3_fp8_moe_max_rows": (_I64, []),
-    "exl3_fp8_moe_decode": (_I, [_P, _I, _P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _I64, C.c_float, _I, _P,
+    "exl3_fp8_moe_decode": (_I, [_P, _I, _P, _P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _I64, C.c_float, _I, _P,
                                  _I64, _P]),
     "exl3_decode_roof_out_floats": (_I64, []),
     "exl3_decode_roof": (_I, [_I, _I, _I, _P, _I64, _P, _I64, _P, _P]),

@@ -1,13 +1,17 @@
 // fp8_moe.cu -- routed-expert MoE layer for a few tokens over e4m3 experts with
 // one fp32 scale for each 128 x 128 block of a weight, in two kernels.
-//   G = x . Wgate_e^T, U = x . Wup_e^T      (x quantised by row and 128 columns)
+//   G = x . Wgate_e^T, U = x . Wup_e^T      (x in e4m3, scales by row and 128 columns)
 //   a = silu(min(G, L)) * clamp(U, -L, L)   (fp32; quantised the same way)
 //   out[t] = sum over the valid slots of weight * (a . Wdown_e^T)   (fp32, one cast)
+// An x in 16 or 32 bits goes through the quantiser's kernel first.  (Quantising
+// it inside kernel 1, for every output tile anew, cost one warp about 2000
+// clocks a row and block: four tokens took 232 us.)
+//
 // Bound: the routed experts' weights, 3 * H * I bytes each, read once.  So both
 // kernels do nothing but stream weight blocks: a 128 x 128 block is one TMA box
-// and the M operand of four tcgen05.mma (K = 32 e4m3 each), the tokens of the
-// expert are N, and each block's sums are read back from TMEM, scaled by the
-// two scales and added to fp32 registers while the next block is multiplied.
+// and the M operand of four tcgen05.mma (K = 32 e4m3 each), the tokens are N, and
+// each block's sums are read back from TMEM, scaled by the two scales and added
+// to fp32 registers while the next block is multiplied.
 //
 // Work is cut evenly, not by experts: the layer's blocks in one fixed order
 // (kernel 1: expert, 128 columns of I, block of H; kernel 2: 128 columns of H,
@@ -39,17 +43,13 @@ constexpr int kFmMaxTopk = 16;
 constexpr int kFmMaxInter = 8192;
 constexpr int kFmMaxHidden = 16384;
 constexpr int kFmMaxCtas = 160;
-// Warps 0-3 epilogue, 4 producer, 5 MMA, 6-7 x.  Two warps on each of an SM's
-// four register files: CTAs of both kernels fit side by side (kernel 2 waits
-// there, its ring filled), which three would not.
+// Warps 0-3 epilogue, 4 producer, 5 MMA, 6 factors, 7 finisher.  Two warps on each of
+// an SM's four register files: CTAs of both kernels fit side by side (kernel 2
+// waits there, its ring filled), which three would not.
 constexpr int kFmThreads = 256;
 constexpr int kFmProducerWarp = 4;
 constexpr int kFmMmaWarp = 5;
-constexpr int kFmXWarp = 6;
-constexpr int kFmXWarps = 2;
-// Rows up to which kernel 1 quantises the rows of x that it multiplies itself;
-// above, a launch of the quantiser does it once for all CTAs.
-constexpr int kFmInlineRows = 16;
+constexpr int kFmFacWarp = 6;
 constexpr int kFmMaxSlotsW = 12;             // weight blocks in the ring
 constexpr int kFmMaxBufs = 4;                // steps whose sums and inputs are held
 // Control region (uint32 words): [2] status; counters of kernel 1's output
@@ -63,19 +63,20 @@ struct FmParams {
     CUtensorMap w13;             // [E * 2 I][H], box 128 x 128
     CUtensorMap w2;              // [E * H][I], box 128 x 128
     CUtensorMap amap;            // down input [slots][I], box 128 x NT
-    CUtensorMap xmap;            // more than kFmInlineRows rows: x in e4m3 [m][H], box 128 x NT
-    const void* x;
+    CUtensorMap xmap;            // x in e4m3 [m][H], box 128 x NT
     void* out;
     const float* w13s;           // [E][2 I / 128][H / 128]
     const float* w2s;            // [E][H / 128][I / 128]
-    const float* xs;             // its scales [H / 128][m]
+    const float* xs;             // its scales: xs[token * xsr + block * xsg]
+    int64_t xsr, xsg;
     uint8_t* aq;                 // [slots][I] e4m3
     float* as;                   // [slots][I / 128]
     float* part;                 // partial sums of the CTAs' first and last tiles
     uint32_t* ctrl;
     RouteIn route;
     float limit;
-    int x_dtype, out_dtype, pow2, xvec;
+    int out_dtype, pow2;
+    int early;                   // all before the quantiser's launch is complete when kernel 1 starts
     int m, topk, E, H, I, slots;
 };
 
@@ -84,6 +85,7 @@ struct FmParams {
 struct FmPlan {
     alignas(16) int id[kFmMaxSlots];
     short slot[kFmMaxSlots];          // pair -> slot
+    short tok[kFmMaxSlots];           // pair -> token
     short pexp[kFmMaxSlots];          // pair -> expert
     short gstart[kFmMaxSlots + 2];    // group -> first pair; [G] = pairs
     uint8_t first[kFmMaxSlots];       // pair begins a group
@@ -91,22 +93,18 @@ struct FmPlan {
     int G;
 };
 
-// Shared memory of a CTA: a ring of weight blocks (16 KB each, so that few bytes
-// wait while many are in flight; with the NT input rows of the block where TMA
-// brings them), kernel 1's own quantised rows of x of kBufs steps, the head,
-// kernel 2's output rows.  A step is one block of k: kernel 1 multiplies the gate
-// and the up block, each into TMEM columns of its own, kernel 2 the down block.
-// D's columns are the group's pairs, or all tokens where kernel 1's x comes
-// quantised (NT > 16): columns of other tokens are never used.
+// Shared memory of a CTA: a ring of weight blocks with the NT input rows of the
+// block (16 + 2 .. 8 KB, so that few bytes wait while many are in flight), the
+// head, kernel 2's output rows.  A step is one block of k: kernel 1 multiplies
+// the gate and the up block, each into TMEM columns of its own, kernel 2 the down
+// block.  D's columns are all tokens in kernel 1 -- those that are not the
+// expert's are never used -- and the group's pairs in kernel 2.
 template <int NT, int PH>
 struct FmLayout {
-    static constexpr bool kInline = PH == 0 && NT <= kFmInlineRows;
     static constexpr int kMats = PH == 0 ? 2 : 1;
     static constexpr int kBufs = NT <= 16 ? 4 : PH == 0 ? 2 : NT <= 32 ? 4 : 2;
     static constexpr int kTmemCols = NT * kMats * kBufs;             // 64 .. 256
-    static constexpr int kX = NT * 128;
-    static constexpr int kSlot = (int) kFp8WTile + (kInline ? 0 : kX);
-    static constexpr int kXRing = kInline ? kBufs * kX : 0;
+    static constexpr int kSlot = (int) kFp8WTile + NT * 128;
 };
 
 template <int NT>
@@ -114,10 +112,10 @@ struct FmHead {
     FmPlan plan;
     uint64_t wfull[kFmMaxSlotsW];        // a weight block has arrived
     uint64_t wdone[kFmMaxSlotsW];        // it has been multiplied
-    uint64_t xfull[kFmMaxBufs];          // a step's input rows (kernel 1) and factors are there
-    uint64_t tfull[kFmMaxBufs];          // a step's sums are in TMEM; its input rows have been read
+    uint64_t ffull[kFmMaxBufs];          // a step's factors are there
+    uint64_t tfull[kFmMaxBufs];          // a step's sums are in TMEM
     uint64_t tempty[kFmMaxBufs];         // they have been read
-    // Factors of a step's columns.  Twice kBufs deep: x's warps write step s once
+    // Factors of a step's columns.  Twice kBufs deep: step s's are written once
     // step s - kBufs is in TMEM, i.e. the epilogue is done with s - 2 kBufs.
     alignas(16) float fac[2 * kFmMaxBufs][NT];
     float wsc[2 * kFmMaxBufs][2];
@@ -128,6 +126,9 @@ struct FmHead {
 };
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The epilogue hands a part that it has stored to the finisher and goes on.
+__device__ __forceinline__ void part_ready() { asm volatile("bar.arrive 2, 160;" ::: "memory"); }
+__device__ __forceinline__ void part_wait() { asm volatile("bar.sync 2, 160;" ::: "memory"); }
 
 // Every thread of the CTA calls this; ends with a barrier.
 __device__ void fm_plan(FmPlan& P, const FmParams& p, int nt, int tid) {
@@ -154,6 +155,7 @@ __device__ void fm_plan(FmPlan& P, const FmParams& p, int nt, int tid) {
             }
         }
         P.slot[before] = (short) tid;
+        P.tok[before] = (short) (tid / p.topk);
         P.pexp[before] = (short) id;
         P.first[before] = rank % nt == 0;
     }
@@ -197,17 +199,60 @@ struct FmAt {
     }
 };
 
+// A step's factors on their way: column h * 32 + lane, and a block's scale.
+template <int NT>
+struct FmFac {
+    float f[(NT + 31) / 32];
+    float ws;
+};
+
+// A CTA's part of a tile that it shares: slot 1 where its range began before the tile did.
+__device__ __forceinline__ float* fm_part(float* part, int rows_pt, int c, int first, int C, int total) {
+    return part + ((int64_t) c * 2 + (fm_start(c, C, total) >= first ? 0 : 1)) * rows_pt * 128;
+}
+
+// Sums of rows of the parts of CTAs c0 .. c1, in their order; four values a lane,
+// the loads of four CTAs in flight.
+template <int NR>
+__device__ __forceinline__ void fm_sum(float4 (&out)[NR], const int (&row)[NR], int n, float* part, int rows_pt, int c0, int c1,
+                                       int first, int C, int total, int lane) {
+#pragma unroll
+    for (int h = 0; h < NR; ++h) out[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = c0; c <= c1; c += 4) {
+        float4 v[4][NR];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const bool on = c + q <= c1 && fm_start(c + q, C, total) != fm_start(c + q + 1, C, total);
+            const float4* src = reinterpret_cast<const float4*>(fm_part(part, rows_pt, min(c + q, c1), first, C, total));
+#pragma unroll
+            for (int h = 0; h < NR; ++h)
+                v[q][h] = on && h < n ? __ldcg(src + row[h] * 32 + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+                out[h].x += v[q][h].x; out[h].y += v[q][h].y; out[h].z += v[q][h].z; out[h].w += v[q][h].w;
+            }
+    }
+}
+
+// silu(min(g, L)) * clamp(u, -L, L); NaN passes through
+__device__ __forceinline__ float fm_swiglu(float g, float u, float lim) {
+    g = g > lim ? lim : g;
+    u = u > lim ? lim : u < -lim ? -lim : u;
+    return g / (1.f + expf(-g)) * u;
+}
+
 template <int NT, int PH>
-__global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_constant__ FmParams p) {
+__global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(const __grid_constant__ FmParams p) {
     using L = FmLayout<NT, PH>;
     constexpr int kMats = L::kMats, kBufs = L::kBufs, kFacs = 2 * L::kBufs;
-    constexpr bool kInline = L::kInline, kTokens = PH == 0 && !kInline;   // kTokens: D's columns are all tokens
     constexpr int kCh = NT < 32 ? 4 : 8;                              // columns handled together at a tile's end
     extern __shared__ uint8_t fm_raw[];
     uint8_t* ring = fm_raw + ((1024u - (smem_u32(fm_raw) & 1023u)) & 1023u);
-    uint8_t* xring = ring + p.slots * L::kSlot;
-    FmHead<NT>& S = *reinterpret_cast<FmHead<NT>*>(xring + L::kXRing);
-    float* oacc = reinterpret_cast<float*>(xring + L::kXRing + sizeof(FmHead<NT>));    // PH 1: [m][128]
+    FmHead<NT>& S = *reinterpret_cast<FmHead<NT>*>(ring + p.slots * L::kSlot);
+    float* oacc = reinterpret_cast<float*>(ring + p.slots * L::kSlot + sizeof(FmHead<NT>));    // PH 1: [m][128]
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const int C = (int) gridDim.x, cta = (int) blockIdx.x;
     const int NBI = p.I / 128, NBH = p.H / 128, KB = PH == 0 ? NBH : NBI;
@@ -218,7 +263,7 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
         tmap_prefetch(PH == 0 ? &p.w13 : &p.w2);
         for (int s = 0; s < W; ++s) { mbar_init(&S.wfull[s], 1); mbar_init(&S.wdone[s], 1); }
         for (int b = 0; b < kBufs; ++b) {
-            mbar_init(&S.xfull[b], kInline ? kFmXWarps : 1);
+            mbar_init(&S.ffull[b], 1);
             mbar_init(&S.tfull[b], 1);
             mbar_init(&S.tempty[b], 4);
         }
@@ -227,10 +272,10 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
     if (warp == kFmMmaWarp) tmem_alloc(&S.tmem, L::kTmemCols);
     if (PH == 0) {
         // Kernel 2 may start once what came before the layer (the routes among
-        // it) is complete: behind this kernel's own wait, or at once where the
-        // quantiser, an ordinary launch, ran in between.  Then only x is waited
-        // for, by those who read it.
-        if (kInline) pdl_wait();
+        // it) is complete: at once where the quantiser, an ordinary launch, ran in
+        // between -- only x is waited for then, by those who read it -- otherwise
+        // behind this kernel's own wait.
+        if (!p.early) pdl_wait();
         pdl_launch_dependents();
     }
     tc_fence_before();
@@ -242,6 +287,59 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
     const int per_tile = PH == 0 ? KB : G * KB;                       // steps of one output tile
     const int total = PH == 0 ? G * NBI * KB : NBH * per_tile;
     const int beg = fm_start(cta, C, total), end = fm_start(cta + 1, C, total), nsteps = end - beg;
+    // Parts: what a CTA has of a tile that it shares; slot 1 where its range began before the tile did.
+    const int rows_pt = PH == 0 ? kMats * NT : p.m;                   // rows of 128 in a part
+    auto token = [&](int pair) { return (int) P.tok[pair]; };
+
+    // A shared tile whose count this CTA completed: the parts are added in CTA
+    // order and the tile is finished, by warp w of n.
+    auto finish_shared = [&](int tile, int w, int nw) {
+        const int first = tile * per_tile;
+        const int c0 = fm_owner(first, C, total), c1 = fm_owner(first + per_tile - 1, C, total);
+        float4 o[2 * kMats];
+        int row[2 * kMats];
+        if (PH == 0) {
+            const int g = tile / NBI, ib = tile % NBI, p0 = P.gstart[g], pe = P.gstart[g + 1];
+            for (int pr = p0 + 2 * w; pr < pe; pr += 2 * nw) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int col = token(min(pr + h, pe - 1));
+                    row[h * kMats] = col;
+                    row[h * kMats + kMats - 1] = (kMats - 1) * NT + col;
+                }
+                fm_sum<2 * kMats>(o, row, pr + 1 < pe ? 2 * kMats : kMats, p.part, rows_pt, c0, c1, first, C, total, lane);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (pr + h >= pe) break;
+                    const float4 g4 = o[h * kMats], u4 = o[h * kMats + kMats - 1];
+                    float v[4] = {fm_swiglu(g4.x, u4.x, p.limit), fm_swiglu(g4.y, u4.y, p.limit),
+                                  fm_swiglu(g4.z, u4.z, p.limit), fm_swiglu(g4.w, u4.w, p.limit)};
+                    const uint32_t mx = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+                    const float sa = fp8_scale(__reduce_max_sync(0xffffffffu, mx), p.pow2), inv = __frcp_rn(sa);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = fp8_quotient(v[j], sa, inv, p.pow2);
+                    *reinterpret_cast<uint32_t*>(p.aq + (int64_t) (pr + h) * p.I + ib * 128 + lane * 4) =
+                        e4m3x2(v[0], v[1]) | (e4m3x2(v[2], v[3]) << 16);
+                    if (lane == 0) p.as[(int64_t) (pr + h) * NBI + ib] = sa;
+                }
+            }
+        } else {
+            for (int t = 2 * w; t < p.m; t += 2 * nw) {
+                row[0] = t;
+                row[1] = t + 1;
+                fm_sum<2 * kMats>(o, row, min(2, p.m - t), p.part, rows_pt, c0, c1, first, C, total, lane);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (t + h >= p.m) break;
+                    const int64_t at = (int64_t) (t + h) * p.H + tile * 128 + lane * 4;
+                    store_out(p.out, p.out_dtype, at, o[h].x);
+                    store_out(p.out, p.out_dtype, at + 1, o[h].y);
+                    store_out(p.out, p.out_dtype, at + 2, o[h].z);
+                    store_out(p.out, p.out_dtype, at + 3, o[h].w);
+                }
+            }
+        }
+    };
 
     if (warp == kFmProducerWarp) {
         if (lane == 0 && nsteps > 0) {
@@ -259,48 +357,45 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
             FmAt<PH> a(beg, G, NBI, KB);
             auto mat_of = [](int t) { return PH == 0 ? t & 1 : 0; };
             auto next = [&](FmAt<PH>& at, int t) { if (PH == 1 || (t & 1)) at.next(); };
+            // a ring of weights ahead of the wait: no kernel that may still run writes them
+            FmAt<PH> a0 = a;
             int t = 0;
-            if (!kInline) {
-                // a ring of weights ahead of the wait: no kernel that may still run writes them
-                FmAt<PH> a0 = a;
-                for (; t < min(W, nblk); ++t) { weights(a, mat_of(t), t); next(a, t); }
-                pdl_wait();
-                fence_proxy_async_global();
-                for (int i = 0; i < t; ++i) { inputs(a0, i); next(a0, i); }
-            }
+            for (; t < min(W, nblk); ++t) { weights(a, mat_of(t), t); next(a, t); }
+            pdl_wait();
+            fence_proxy_async_global();
+            for (int i = 0; i < t; ++i) { inputs(a0, i); next(a0, i); }
             int issued = t;
             for (; t < nblk; ++t) {
                 const int slot = t % W;
                 if (t >= W && !mbar_wait(&S.wdone[slot], ((t / W) + 1u) & 1u, status)) break;
                 weights(a, mat_of(t), slot);
-                if (!kInline) inputs(a, slot);
+                inputs(a, slot);
                 next(a, t);
                 ++issued;
             }
             // no copy may still be in flight when the CTA retires
             for (int i = max(0, issued - W); i < issued; ++i)
                 if (!mbar_wait(&S.wfull[i % W], (i / W) & 1u, status)) break;
-        } else if (!kInline) {
+        } else {
             pdl_wait();
         }
     } else if (warp == kFmMmaWarp) {
-        const uint64_t wdesc0 = sdesc_sw128(smem_u32(ring)), xdesc0 = sdesc_sw128(smem_u32(xring));
+        const uint64_t wdesc0 = sdesc_sw128(smem_u32(ring));
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
         int slot = 0;
         uint32_t wpar = 0;
         bool ok = true;
         for (int s = 0; s < nsteps && ok; ++s, a.next()) {
             const int b = s % kBufs;
-            const int n = kTokens ? p.m : P.gstart[a.g + 1] - P.gstart[a.g];
+            const int n = PH == 0 ? p.m : P.gstart[a.g + 1] - P.gstart[a.g];
             const uint32_t id = __shfl_sync(0xffffffffu, idesc_f16(128, (n + 15) & ~15), 0);
-            ok = mbar_poll2_lanes(&S.xfull[b], (s / kBufs) & 1u, &S.tempty[b], ((s / kBufs) + 1u) & 1u, status);
+            ok = mbar_poll2_lanes(&S.ffull[b], (s / kBufs) & 1u, &S.tempty[b], ((s / kBufs) + 1u) & 1u, status);
 #pragma unroll
             for (int mat = 0; mat < kMats; ++mat) {
                 ok = ok && mbar_poll_lanes(&S.wfull[slot], wpar, status);
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t wd = wdesc0 + (uint64_t) (slot * (L::kSlot >> 4));
-                const uint64_t xd = kInline ? xdesc0 + (uint64_t) (b * (L::kX >> 4)) : wd + (kFp8WTile >> 4);
+                const uint64_t wd = wdesc0 + (uint64_t) (slot * (L::kSlot >> 4)), xd = wd + (kFp8WTile >> 4);
                 if (elect_lane()) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) tc_mma_f8(tmem + (b * kMats + mat) * NT, wd + 2 * q, xd + 2 * q, id, q);
@@ -310,85 +405,65 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                 if (++slot == W) { slot = 0; wpar ^= 1u; }
             }
         }
-    } else if (warp >= kFmXWarp) {
-        const int xw = warp - kFmXWarp, xt = tid - kFmXWarp * 32;
+    } else if (warp == kFmFacWarp) {
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
         if (PH == 0 && cta == 0)
-            for (int i = xt; i < NBH; i += 32 * kFmXWarps) p.ctrl[kFmCntB + i] = 0u;   // kernel 2's counters
-        if (kInline) {
-            // Quantise the group's rows of x, four a warp; which four goes round
-            // with the steps, so that few rows keep both warps busy.
-            XRows next[2];                                    // the next rows of this warp, fetched ahead
-            FmAt<PH> f = a;
-            int fs = 0, fq = xw;
-            auto fetch = [&](XRows& to) {
-                while (fs < nsteps && fq * 4 >= P.gstart[f.g + 1] - P.gstart[f.g]) {
-                    ++fs;
-                    f.next();
-                    fq = (xw + fs) % kFmXWarps;
-                }
-                if (fs >= nsteps) return;
-                const int p0 = P.gstart[f.g] + fq * 4, cnt = min(4, P.gstart[f.g + 1] - p0), lr = XRows::row(cnt, lane);
-                const int tok = P.slot[p0 + min(lr, cnt - 1)] / p.topk;
-                to.load(cnt, p.x, p.x_dtype, (int64_t) tok * p.H + f.kb * 128 + XRows::col(cnt, lane), lr < cnt ? 16 : 0, p.xvec);
-                fq += kFmXWarps;
-            };
-            fetch(next[0]);
-            fetch(next[1]);
-            for (int s = 0; s < nsteps; ++s, a.next()) {
-                const int b = s % kBufs, n = P.gstart[a.g + 1] - P.gstart[a.g], q0 = (xw + s) % kFmXWarps;
-                uint8_t* tile = xring + b * L::kX;
-                float* fac = S.fac[s % kFacs];
-                float ws = 0.f;
-                if (q0 == 0 && lane < 2)
-                    ws = __ldg(p.w13s + ((int64_t) P.pexp[P.gstart[a.g]] * 2 * NBI + lane * NBI + a.tile % NBI) * NBH + a.kb);
-                bool free = false;
-                for (int q = q0; q * 4 < n; q += kFmXWarps) {
-                    const XRows cur = next[0];
-                    next[0] = next[1];
-                    fetch(next[1]);
-                    const int cnt = min(4, n - q * 4), lr = XRows::row(cnt, lane);
-                    float sx;
-                    const uint4 v = cur.quantize(cnt, p.x_dtype, p.pow2, sx);
-                    if (!free && !(free = mbar_wait_lanes(&S.tfull[b], ((s / kBufs) + 1u) & 1u, status))) break;
-                    if (lr < cnt) XRows::store(cnt, tile, q * 4 + lr, lane, v);
-                    if (lr < cnt && (cnt == 1 ? lane == 0 : (lane & 7) == 0)) fac[q * 4 + lr] = sx;
-                }
-                if (!free && !mbar_wait_lanes(&S.tfull[b], ((s / kBufs) + 1u) & 1u, status)) break;
-                if (q0 == 0 && lane < 2) S.wsc[s % kFacs][lane] = ws;
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&S.xfull[b]);
-            }
-        } else {
-            // The factors of a step's columns, one warp a step: x's scales and the two
-            // blocks' (kernel 1), or the down input's, the block's and the route's.
-            pdl_wait();
-            if (PH == 1) {
-                for (int i = cta * 32 * kFmXWarps + xt; i < G * NBI; i += C * 32 * kFmXWarps) p.ctrl[kFmCntA + i] = 0u;   // kernel 1's
-            }
-            for (int q = 0; q < xw && q < nsteps; ++q) a.next();
-            for (int s = xw; s < nsteps; s += kFmXWarps) {
-                const int b = s % kBufs, p0 = P.gstart[a.g], n = PH == 0 ? p.m : P.gstart[a.g + 1] - p0, e = P.pexp[p0];
-                float ws = 0.f;
-                if (PH == 1) ws = __ldg(p.w2s + ((int64_t) e * NBH + a.tile) * NBI + a.kb);
-                else if (lane < 2) ws = __ldg(p.w13s + ((int64_t) e * 2 * NBI + lane * NBI + a.tile % NBI) * NBH + a.kb);
-                float f[(NT + 31) / 32];
+            for (int i = lane; i < NBH; i += 32) p.ctrl[kFmCntB + i] = 0u;   // kernel 2's counters
+        // The factors of a step's columns: x's scales and the two blocks' (kernel 1),
+        // or the down input's, the block's and the route's.  Loaded two steps ahead.
+        pdl_wait();
+        if (PH == 1)
+            for (int i = cta * 32 + lane; i < G * NBI; i += C * 32) p.ctrl[kFmCntA + i] = 0u;   // kernel 1's
+        FmAt<PH> at = a;
+        auto load = [&](int s) {
+            FmFac<NT> v;
+            v.ws = 0.f;
 #pragma unroll
-                for (int h = 0; h < (NT + 31) / 32; ++h) {
-                    const int j = h * 32 + lane;
-                    f[h] = 0.f;
-                    if (j < n) f[h] = PH == 0 ? __ldcg(p.xs + (int64_t) a.kb * p.m + j)
-                                              : __ldcg(p.as + (int64_t) (p0 + j) * NBI + a.kb) * ws * route_weight(p.route, P.slot[p0 + j]);
-                }
-                if (!mbar_wait_lanes(&S.tfull[b], ((s / kBufs) + 1u) & 1u, status)) break;
+            for (int h = 0; h < (NT + 31) / 32; ++h) v.f[h] = 0.f;
+            if (s >= nsteps) return v;
+            const int p0 = P.gstart[at.g], n = PH == 0 ? p.m : P.gstart[at.g + 1] - p0, e = P.pexp[p0];
+            if (PH == 1) v.ws = __ldg(p.w2s + ((int64_t) e * NBH + at.tile) * NBI + at.kb);
+            else if (lane < 2) v.ws = __ldg(p.w13s + ((int64_t) e * 2 * NBI + lane * NBI + at.tile % NBI) * NBH + at.kb);
 #pragma unroll
-                for (int h = 0; h < (NT + 31) / 32; ++h)
-                    if (h * 32 + lane < NT) S.fac[s % kFacs][h * 32 + lane] = f[h];
-                if (PH == 0 && lane < 2) S.wsc[s % kFacs][lane] = ws;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&S.xfull[b]);
-                for (int q = 0; q < kFmXWarps; ++q) a.next();
+            for (int h = 0; h < (NT + 31) / 32; ++h) {
+                const int j = h * 32 + lane;
+                if (j < n) v.f[h] = PH == 0 ? __ldcg(p.xs + j * p.xsr + at.kb * p.xsg) : __ldcg(p.as + (int64_t) (p0 + j) * NBI + at.kb);
+            }
+            at.next();
+            return v;
+        };
+        FmFac<NT> v0 = load(0), v1 = load(1);
+        for (int s = 0; s < nsteps; ++s, a.next()) {
+            const int b = s % kBufs, p0 = P.gstart[a.g], n = P.gstart[a.g + 1] - p0;
+            const FmFac<NT> v = v0;
+            v0 = v1;
+            v1 = load(s + 2);
+            if (!mbar_wait_lanes(&S.tfull[b], ((s / kBufs) + 1u) & 1u, status)) break;
+#pragma unroll
+            for (int h = 0; h < (NT + 31) / 32; ++h) {
+                const int j = h * 32 + lane;
+                float f = v.f[h];
+                if (PH == 1) f = j < n ? f * v.ws * route_weight(p.route, P.slot[p0 + j]) : 0.f;
+                if (j < NT) S.fac[s % kFacs][j] = f;
+            }
+            if (PH == 0 && lane < 2) S.wsc[s % kFacs][lane] = v.ws;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.ffull[b]);
+        }
+    } else if (warp > kFmFacWarp) {
+        // -------------------------------------------------------------- finisher
+        // The first tile of the CTA's range, where the CTA shares it and goes on
+        // behind it: a chain of trips to L2, during which the epilogue takes the
+        // next steps (6 us for one token when the epilogue did it itself, with the
+        // CTA's weights waiting).
+        if (PH == 1) pdl_wait();
+        if (nsteps > 0) {
+            const int first = beg / per_tile * per_tile, steps = min(end, first + per_tile) - beg;
+            if (steps != per_tile && beg + steps < end) {
+                part_wait();
+                uint32_t done = 0u;
+                if (lane == 0) done = atom_add_acq_rel_gpu(&p.ctrl[(PH == 0 ? kFmCntA : kFmCntB) + first / per_tile], (uint32_t) steps) + (uint32_t) steps;
+                if (__shfl_sync(0xffffffffu, done, 0) == (uint32_t) per_tile) finish_shared(first / per_tile, 0, 1);
             }
         }
     } else {
@@ -400,16 +475,6 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[mat][j] = 0.f;
         };
-        // Counts this CTA's steps of an output tile; true in the CTA that completes it.
-        auto completes = [&](int counter, int steps) {
-            epi_sync();
-            if (tid == 0) S.last = atom_add_acq_rel_gpu(&p.ctrl[counter], (uint32_t) steps) + steps == (uint32_t) per_tile;
-            epi_sync();
-            return S.last != 0u;
-        };
-        // a tile's part: slot 1 where the CTA's range began before the tile did
-        const int rows_pt = PH == 0 ? kMats * NT : p.m;               // rows of 128 in a part
-        auto part_of = [&](int c, int first) { return p.part + ((int64_t) c * 2 + (fm_start(c, C, total) >= first ? 0 : 1)) * rows_pt * 128; };
         if (PH == 1) {
             pdl_wait();
             if (total == 0)
@@ -420,9 +485,10 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
         clear();
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
         int seg = 0;                                                  // steps of the current tile so far
+        bool handed = false;
         for (int s = 0; s < nsteps; ++s) {
             const int b = s % kBufs;
-            const int p0 = P.gstart[a.g], pairs = P.gstart[a.g + 1] - p0, n = kTokens ? p.m : pairs;   // n: D's columns
+            const int p0 = P.gstart[a.g], pairs = P.gstart[a.g + 1] - p0, n = PH == 0 ? p.m : pairs;   // n: D's columns
             if (!mbar_wait_lanes(&S.tfull[b], (s / kBufs) & 1u, status)) break;
             tc_fence_after();
 #pragma unroll
@@ -455,22 +521,19 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     if (j >= n) break;
-                    oacc[(P.slot[p0 + j] / p.topk) * 128 + tid] += acc[0][j];
+                    oacc[token(p0 + j) * 128 + tid] += acc[0][j];
                 }
                 clear();
             }
             if (tile_end) {
-                const int first = a.tile * per_tile;                  // the tile's first step
-                bool finish = seg == per_tile;
-                // the columns that the group has, a bit each
-                uint64_t have = n < 64 ? (1ull << n) - 1ull : ~0ull;
-                if (kTokens) {
-                    have = 0;
-                    for (int j = 0; j < pairs; ++j) have |= 1ull << (P.slot[p0 + j] / p.topk);
-                }
+                const bool whole = seg == per_tile;
+                // kernel 1: the columns whose tokens the group has, a bit each
+                uint64_t have = 0;
+                if (PH == 0)
+                    for (int j = 0; j < pairs; ++j) have |= 1ull << token(p0 + j);
                 auto chunk = [&](int c) { return (have >> (c * kCh) & ((1ull << kCh) - 1ull)) != 0; };
-                if (!finish) {
-                    float* dst = part_of(cta, first);
+                if (!whole) {
+                    float* dst = fm_part(p.part, rows_pt, cta, a.tile * per_tile, C, total);
                     if (PH == 0) {
 #pragma unroll
                         for (int c = 0; c < NT / kCh; ++c) {
@@ -483,61 +546,32 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                     } else {
                         for (int t = 0; t < p.m; ++t) __stcg(dst + t * 128 + tid, oacc[t * 128 + tid]);
                     }
-                    finish = completes((PH == 0 ? kFmCntA : kFmCntB) + a.tile, seg);
-                    if (finish) {
-                        const int c0 = fm_owner(first, C, total), c1 = fm_owner(first + per_tile - 1, C, total);
-                        if (PH == 0) clear();
-                        else for (int t = 0; t < p.m; ++t) oacc[t * 128 + tid] = 0.f;
-                        for (int c = c0; c <= c1; ++c) {
-                            if (fm_start(c, C, total) == fm_start(c + 1, C, total)) continue;
-                            const float* src = part_of(c, first);
-                            if (PH == 0) {
-#pragma unroll
-                                for (int h = 0; h < NT / kCh; ++h) {
-                                    if (!chunk(h)) continue;
-                                    float v[kMats][kCh];              // all of them on their way together
-#pragma unroll
-                                    for (int j = 0; j < kCh; ++j)
-#pragma unroll
-                                        for (int mat = 0; mat < kMats; ++mat) v[mat][j] = __ldcg(src + (mat * NT + h * kCh + j) * 128 + tid);
-#pragma unroll
-                                    for (int j = 0; j < kCh; ++j)
-#pragma unroll
-                                        for (int mat = 0; mat < kMats; ++mat) acc[mat][h * kCh + j] += v[mat][j];
-                                }
-                            } else {
-                                for (int t = 0; t < p.m; t += 4) {
-                                    float v[4];
-#pragma unroll
-                                    for (int q = 0; q < 4; ++q) v[q] = t + q < p.m ? __ldcg(src + (t + q) * 128 + tid) : 0.f;
-#pragma unroll
-                                    for (int q = 0; q < 4; ++q)
-                                        if (t + q < p.m) oacc[(t + q) * 128 + tid] += v[q];
-                                }
-                            }
-                        }
+                    if (s + 1 < nsteps) {
+                        part_ready();
+                        handed = true;
+                    } else {
+                        epi_sync();
+                        if (tid == 0)
+                            S.last = atom_add_acq_rel_gpu(&p.ctrl[(PH == 0 ? kFmCntA : kFmCntB) + a.tile], (uint32_t) seg) + (uint32_t) seg == (uint32_t) per_tile;
+                        epi_sync();
+                        if (S.last) finish_shared(a.tile, warp, 4);
                     }
                 }
-                if (finish && PH == 0) {
+                if (whole && PH == 0) {
                     // SwiGLU, then one scale for each token's 128 columns; NaN passes
                     // through.  kCh columns at a time: columns behind the group's last
                     // are computed with them and never stored.
                     const int ib = a.tile % NBI;
-                    const float lim = p.limit;
-                    if (kTokens)
-                        for (int j = tid; j < pairs; j += 128) {
-                            const int t = P.slot[p0 + j] / p.topk;
-                            if (j == 0 || P.slot[p0 + j - 1] / p.topk != t) S.tokpair[t] = (short) (p0 + j);
+                    for (int j = tid; j < pairs; j += 128) {
+                            const int t = token(p0 + j);
+                            if (j == 0 || token(p0 + j - 1) != t) S.tokpair[t] = (short) (p0 + j);
                         }
 #pragma unroll
                     for (int c = 0; c < NT / kCh; ++c) {
                         if (!chunk(c)) continue;
 #pragma unroll
                         for (int j = c * kCh; j < (c + 1) * kCh; ++j) {
-                            float g = acc[0][j], u = acc[kMats - 1][j];
-                            g = g > lim ? lim : g;
-                            u = u > lim ? lim : u < -lim ? -lim : u;
-                            acc[0][j] = g / (1.f + expf(-g)) * u;
+                            acc[0][j] = fm_swiglu(acc[0][j], acc[kMats - 1][j], p.limit);
                             const uint32_t mx = __reduce_max_sync(0xffffffffu, abs_bits(acc[0][j]));
                             if (lane == 0) S.wmax[warp][j] = mx;
                         }
@@ -553,17 +587,17 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                             const uint32_t q = e4m3x2(fp8_quotient(acc[0][j], sa, __frcp_rn(sa), p.pow2), 0.f);
                             if (have >> j & 1ull) {
                                 // an expert listed twice for a token has two pairs next to each other
-                                int pr = kTokens ? S.tokpair[j] : p0 + j;
+                                int pr = S.tokpair[j];
                                 do {
                                     p.aq[(int64_t) pr * p.I + ib * 128 + tid] = (uint8_t) q;
                                     if (tid == 0) p.as[(int64_t) pr * NBI + ib] = sa;
-                                } while (kTokens && ++pr < p0 + pairs && P.slot[pr] / p.topk == j);
+                                } while (++pr < p0 + pairs && token(pr) == j);
                             }
                         }
                     }
                     epi_sync();                                       // wmax is free for the next tile
                 }
-                if (finish && PH == 1)
+                if (whole && PH == 1)
                     for (int t = 0; t < p.m; ++t)
                         store_out(p.out, p.out_dtype, (int64_t) t * p.H + a.tile * 128 + tid, oacc[t * 128 + tid]);
                 if (PH == 0) clear();
@@ -571,6 +605,11 @@ __global__ void __launch_bounds__(kFmThreads, 1) fp8_moe_kernel(const __grid_con
                 seg = 0;
             }
             a.next();
+        }
+        // after a wait that gave up: the finisher's barrier is met all the same
+        if (nsteps > 0 && !handed) {
+            const int steps = min(end, (beg / per_tile + 1) * per_tile) - beg;
+            if (steps != per_tile && beg + steps < end) part_ready();
         }
     }
     tc_fence_before();
@@ -591,14 +630,13 @@ struct FmGeom {
 
 FmGeom fm_geom(int64_t m, int64_t topk, int64_t H, int64_t I) {
     FmGeom g{};
-    const bool xq = m > kFmInlineRows;
     g.nt = m <= 16 ? 16 : m <= 32 ? 32 : 64;
     const int64_t slots = m * topk;
     g.off_aq = EXL3_FP8_MOE_CTRL_BYTES;
     g.off_as = g.off_aq + align_up(slots * I, 256);
     g.off_xq = g.off_as + align_up(slots * (I / 128) * 4, 256);
-    g.off_xs = g.off_xq + (xq ? align_up(m * H, 256) : 0);
-    g.off_part = g.off_xs + (xq ? align_up(m * (H / 128) * 4, 256) : 0);
+    g.off_xs = g.off_xq + align_up(m * H, 256);
+    g.off_part = g.off_xs + align_up(m * (H / 128) * 4, 256);
     const int64_t part_rows = 2 * g.nt > m ? 2 * g.nt : m;
     g.bytes = g.off_part + (int64_t) kFmMaxCtas * 2 * part_rows * 128 * 4;
     return g;
@@ -609,7 +647,7 @@ int fm_launch(FmParams p, int sms, cudaStream_t stream) {
     using L = FmLayout<NT, PH>;
     // The two kernels share an SM while kernel 2 waits: 120 + 104 KB of its memory.
     constexpr int kBudget = (PH == 0 ? 120 : 104) * 1024;
-    const int extra = 1024 + (int) sizeof(FmHead<NT>) + L::kXRing + (PH == 1 ? p.m * 512 : 0);
+    const int extra = 1024 + (int) sizeof(FmHead<NT>) + (PH == 1 ? p.m * 512 : 0);
     static_assert(sizeof(FmHead<64>) + 64 * 512 + 1024 + 2 * FmLayout<64, 1>::kSlot <= 104 * 1024, "room for two blocks");
     int slots = (kBudget - extra) / L::kSlot;
     if (slots > kFmMaxSlotsW) slots = kFmMaxSlotsW;
@@ -621,6 +659,8 @@ int fm_launch(FmParams p, int sms, cudaStream_t stream) {
     cudaError_t attr = cudaSuccess;
     std::call_once(once[dev & 63], [&] {
         attr = cudaFuncSetAttribute(fp8_moe_kernel<NT, PH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
+        if (attr == cudaSuccess)   // all of it, or the SM's split made for one CTA keeps the other kernel's out
+            attr = cudaFuncSetAttribute(fp8_moe_kernel<NT, PH>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     });
     EXL3_CUDA(attr);
     cudaLaunchConfig_t cfg{};
@@ -656,7 +696,7 @@ extern "C" int64_t exl3_fp8_moe_scratch_bytes(int64_t m, int64_t topk, int64_t h
     return fm_geom(m, topk, hidden, inter).bytes;
 }
 
-extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, void* out, int out_dtype, int64_t m, int64_t hidden,
+extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, const float* x_scale, void* out, int out_dtype, int64_t m, int64_t hidden,
                                    int64_t inter, const void* gate_up, const float* gate_up_scale, const void* down,
                                    const float* down_scale, int64_t n_experts, const exl3_moe_route* route, int64_t topk,
                                    float swiglu_limit, int pow2, void* scratch, int64_t scratch_bytes, void* stream) {
@@ -672,9 +712,11 @@ extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, void* out, int ou
                  "exl3_fp8_moe_decode: intermediate must be a multiple of 128 up to %d", kFmMaxInter);
     EXL3_REQUIRE(n_experts >= 1 && n_experts <= 32767 && n_experts * 2 * inter <= INT32_MAX && n_experts * hidden <= INT32_MAX,
                  EXL3_ERR_ARG, "exl3_fp8_moe_decode: expert count out of range");
-    EXL3_REQUIRE(x_dtype >= 0 && x_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2 && route->weights_dtype >= 0 &&
+    EXL3_REQUIRE(x_dtype >= 0 && x_dtype <= 3 && out_dtype >= 0 && out_dtype <= 2 && route->weights_dtype >= 0 &&
                      route->weights_dtype <= 2 && (route->ids_dtype == 0 || route->ids_dtype == 1),
-                 EXL3_ERR_ARG, "exl3_fp8_moe_decode: dtypes must be fp16, bf16 or fp32, ids int32 or int64");
+                 EXL3_ERR_ARG, "exl3_fp8_moe_decode: dtypes must be fp16, bf16 or fp32 (x: e4m3 too), ids int32 or int64");
+    EXL3_REQUIRE((x_dtype == EXL3_DTYPE_E4M3) == (x_scale != nullptr) && (x_scale == nullptr || aligned16(x)), EXL3_ERR_ARG,
+                 "exl3_fp8_moe_decode: x_scale goes with an e4m3 x, 16-byte aligned, and only with one");
     EXL3_REQUIRE(route->expert_map == nullptr || route->n_global >= 1, EXL3_ERR_ARG, "exl3_fp8_moe_decode: empty expert map");
     EXL3_REQUIRE(swiglu_limit > 0.f, EXL3_ERR_ARG, "exl3_fp8_moe_decode: the SwiGLU limit must be positive");
     EXL3_REQUIRE(aligned16(gate_up) && aligned16(down) && aligned16(scratch), EXL3_ERR_ARG,
@@ -692,24 +734,26 @@ extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, void* out, int ou
     if ((rc = fp8_map(&p.w13, gate_up, n_experts * 2 * inter, hidden, hidden, 128, "exl3_fp8_moe_decode")) != EXL3_OK) return rc;
     if ((rc = fp8_map(&p.w2, down, n_experts * hidden, inter, inter, 128, "exl3_fp8_moe_decode")) != EXL3_OK) return rc;
     if ((rc = fp8_map(&p.amap, sb + g.off_aq, m * topk, inter, inter, g.nt, "exl3_fp8_moe_decode")) != EXL3_OK) return rc;
-    p.x = x; p.out = out; p.w13s = gate_up_scale; p.w2s = down_scale;
+    p.out = out; p.w13s = gate_up_scale; p.w2s = down_scale;
     p.aq = sb + g.off_aq;
-    p.xs = reinterpret_cast<const float*>(sb + g.off_xs);
     p.as = reinterpret_cast<float*>(sb + g.off_as);
     p.part = reinterpret_cast<float*>(sb + g.off_part);
     p.ctrl = reinterpret_cast<uint32_t*>(sb);
     p.route = RouteIn{route->ids, route->weights, route->expert_map, route->n_global, route->ids_dtype, route->weights_dtype};
     p.limit = swiglu_limit;
-    p.x_dtype = x_dtype; p.out_dtype = out_dtype; p.pow2 = pow2 != 0;
-    p.xvec = aligned16(x);
+    p.out_dtype = out_dtype; p.pow2 = pow2 != 0;
     p.m = (int) m; p.topk = (int) topk; p.E = (int) n_experts; p.H = (int) hidden; p.I = (int) inter;
     auto s = static_cast<cudaStream_t>(stream);
-    if (m > kFmInlineRows) {
-        if ((rc = fp8_map(&p.xmap, sb + g.off_xq, m, hidden, hidden, g.nt, "exl3_fp8_moe_decode")) != EXL3_OK) return rc;
-        if ((rc = fp8_quantize_launch(x, x_dtype, m, hidden, hidden, sb + g.off_xq, hidden, reinterpret_cast<float*>(sb + g.off_xs),
-                                      1, m, 1, pow2 != 0, s)) != EXL3_OK)
-            return rc;
+    const void* xq = x;
+    p.xs = x_scale; p.xsr = hidden / 128; p.xsg = 1;
+    if (x_dtype != EXL3_DTYPE_E4M3) {
+        float* xs = reinterpret_cast<float*>(sb + g.off_xs);
+        xq = sb + g.off_xq;
+        if ((rc = fp8_quantize_launch(x, x_dtype, m, hidden, hidden, sb + g.off_xq, hidden, xs, 1, m, 1, pow2 != 0, s)) != EXL3_OK) return rc;
+        p.xs = xs; p.xsr = 1; p.xsg = m;
+        p.early = 1;
     }
+    if ((rc = fp8_map(&p.xmap, xq, m, hidden, hidden, g.nt, "exl3_fp8_moe_decode")) != EXL3_OK) return rc;
     if (g.nt == 16) return fm_run<16>(p, di.sms, s);
     if (g.nt == 32) return fm_run<32>(p, di.sms, s);
     return fm_run<64>(p, di.sms, s);

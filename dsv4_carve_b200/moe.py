@@ -292,7 +292,7 @@ def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, s
         scratch = _fp8_moe_scratch(x.device, _ext.fp8_moe_scratch_bytes(min(T, step), topk, state.hidden, state.inter))
         for t in range(0, T, step):
             part = slice(t, min(T, t + step))
-            _ext._fp8_moe_decode(x[part], out[part], state.gate_up, state.gate_up_scale, state.down, state.down_scale,
+            _ext._fp8_moe_decode(x[part], None, out[part], state.gate_up, state.gate_up_scale, state.down, state.down_scale,
                                  state.n_experts, state.hidden, state.inter, ids2[part], route_w[part], limit, scratch,
                                  expert_map, state.pow2_scale, None)
     _CALLS["b200"] += 1

@@ -712,9 +712,12 @@ def _fp8_moe_weight_checks(gate_up, gate_up_scale, down, down_scale) -> tuple:
 def fp8_moe_decode(x: torch.Tensor, out: torch.Tensor, gate_up: torch.Tensor, gate_up_scale: torch.Tensor,
                    down: torch.Tensor, down_scale: torch.Tensor, expert_ids: torch.Tensor,
                    routing_weights: torch.Tensor, swiglu_limit: float, scratch: torch.Tensor, *,
-                   expert_map: torch.Tensor | None = None, pow2_scale: bool = False,
-                   check_status: bool | None = None) -> torch.Tensor:
+                   x_scale: torch.Tensor | None = None, expert_map: torch.Tensor | None = None,
+                   pow2_scale: bool = False, check_status: bool | None = None) -> torch.Tensor:
     """Routed-expert layer for a few rows over e4m3 experts; writes and returns `out`.
+
+    x fp16 / bf16 / fp32 [m, hidden] (quantised by row and 128 columns inside the
+    call), or float8_e4m3fn with its ``x_scale`` fp32 [m, hidden / 128].
 
     gate_up [E, 2 * intermediate, hidden] (gate rows first) and down [E,
     hidden, intermediate] with one fp32 scale for each 128 x 128 block.  The
@@ -722,19 +725,28 @@ def fp8_moe_decode(x: torch.Tensor, out: torch.Tensor, gate_up: torch.Tensor, ga
     ids, fp32 / bf16 / fp16 weights, an optional expert_map); `scratch` as
     there, of fp8_moe_scratch_bytes() bytes, zeroed before its first use."""
     E, H, I = _fp8_moe_weight_checks(gate_up, gate_up_scale, down, down_scale)
-    return _fp8_moe_decode(x, out, gate_up, gate_up_scale, down, down_scale, E, H, I, expert_ids, routing_weights,
-                           swiglu_limit, scratch, expert_map, pow2_scale, check_status)
+    return _fp8_moe_decode(x, x_scale, out, gate_up, gate_up_scale, down, down_scale, E, H, I, expert_ids,
+                           routing_weights, swiglu_limit, scratch, expert_map, pow2_scale, check_status)
 
 
-def _fp8_moe_decode(x, out, gate_up, gate_up_scale, down, down_scale, E, H, I, expert_ids, routing_weights,
+def _fp8_moe_decode(x, x_scale, out, gate_up, gate_up_scale, down, down_scale, E, H, I, expert_ids, routing_weights,
                     swiglu_limit, scratch, expert_map, pow2_scale, check_status) -> torch.Tensor:
     """fp8_moe_decode behind the checks of the weights, which Fp8MoeState makes once."""
     import ctypes
 
     device = gate_up.device
-    _check(x.device == device and x.dtype in _DT and x.dim() == 2 and x.size(1) == H and x.is_contiguous(),
-           "fp8_moe_decode: x must be contiguous fp16, bf16 or fp32 [m, hidden] on the weights' device")
+    x_code = _DT_X8.get(x.dtype)
+    _check(x.device == device and x_code is not None and x.dim() == 2 and x.size(1) == H and x.is_contiguous(),
+           "fp8_moe_decode: x must be contiguous fp16, bf16, fp32 or float8_e4m3fn [m, hidden] on the weights' device")
     m = x.size(0)
+    xs_ptr = None
+    if x_code == _lib.DT_E4M3:
+        _check(x_scale is not None and x_scale.device == device and x_scale.dtype == torch.float32
+               and x_scale.shape == (m, H // _FP8_GROUP) and x_scale.is_contiguous() and x.data_ptr() % 16 == 0,
+               "fp8_moe_decode: an e4m3 x needs 16-byte alignment and x_scale contiguous fp32 [m, hidden / 128]")
+        xs_ptr = x_scale.data_ptr()
+    else:
+        _check(x_scale is None, "fp8_moe_decode: x_scale goes with an e4m3 x only")
     _check(out.device == device and out.dtype in _DT and out.shape == x.shape and out.is_contiguous(),
            "fp8_moe_decode: out must be contiguous fp16, bf16 or fp32 of x's shape on its device")
     _check(expert_ids.device == device and expert_ids.dtype in _IDS_DT and expert_ids.is_contiguous()
@@ -761,7 +773,7 @@ def _fp8_moe_decode(x, out, gate_up, gate_up_scale, down, down_scale, E, H, I, e
     route = _lib.MoeRoute(expert_ids.data_ptr(), _IDS_DT[expert_ids.dtype], routing_weights.data_ptr(),
                           _DT[routing_weights.dtype], map_ptr, n_global)
     with _on_device(device):
-        _lib.check(lib.exl3_fp8_moe_decode(x.data_ptr(), _DT[x.dtype], out.data_ptr(), _DT[out.dtype], m, H, I,
+        _lib.check(lib.exl3_fp8_moe_decode(x.data_ptr(), x_code, xs_ptr, out.data_ptr(), _DT[out.dtype], m, H, I,
                                            gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(),
                                            down_scale.data_ptr(), E, ctypes.addressof(route), topk, limit,
                                            int(bool(pow2_scale)), scratch.data_ptr(), scratch.numel(),

@@ -352,7 +352,9 @@ int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const float* x_scal
  * during graph capture. */
 int exl3_fp8_status(int clear, uint32_t* status, void* stream);
 
-/* Routed-expert MoE layer for a few tokens over e4m3 experts, two kernels.
+/* Routed-expert MoE layer for a few tokens over e4m3 experts, two kernels
+ * (behind the quantiser's, unless x is e4m3 with x_scale fp32
+ * [m, hidden / 128]; x_scale is NULL otherwise).
  * For every valid (row, slot), expert e = ids[row, slot]:
  *   g = x . Wgate_e^T, u = x . Wup_e^T      (as exl3_fp8_linear, x quantised by row)
  *   a = silu(min(g, L)) * clamp(u, -L, L)   (fp32), quantised by 128 columns
@@ -364,7 +366,7 @@ int exl3_fp8_status(int clear, uint32_t* status, void* stream);
  * down [n_experts, hidden, inter] with down_scale [n_experts, hidden / 128,
  * inter / 128]; all contiguous, weights 16-byte aligned.  m in
  * 1..exl3_fp8_moe_max_rows(), topk in 1..16, m * topk <= 256, hidden (<= 16384)
- * and inter (<= 8192) multiples of 128.  x, out fp16 / bf16 / fp32
+ * and inter (<= 8192) multiples of 128.  x, out fp16 / bf16 / fp32 (x: or e4m3)
  * [m, hidden]; swiglu_limit > 0 (infinity: no clamp); pow2 as above for x and
  * a.  `scratch`: >= exl3_fp8_moe_scratch_bytes(m, topk, hidden, inter) bytes
  * whose first EXL3_FP8_MOE_CTRL_BYTES are zero before first use (calls reset
@@ -375,7 +377,8 @@ int exl3_fp8_status(int clear, uint32_t* status, void* stream);
 #define EXL3_FP8_MOE_CTRL_BYTES 131072
 int64_t exl3_fp8_moe_scratch_bytes(int64_t m, int64_t topk, int64_t hidden, int64_t inter);
 int64_t exl3_fp8_moe_max_rows(void);
-int exl3_fp8_moe_decode(const void* x, int x_dtype, void* out, int out_dtype, int64_t m, int64_t hidden, int64_t inter,
+int exl3_fp8_moe_decode(const void* x, int x_dtype, const float* x_scale, void* out, int out_dtype, int64_t m,
+                        int64_t hidden, int64_t inter,
                         const void* gate_up, const float* gate_up_scale, const void* down, const float* down_scale,
                         int64_t n_experts, const exl3_moe_route* route, int64_t topk, float swiglu_limit, int pow2,
                         void* scratch, int64_t scratch_bytes, void* stream);

@@ -280,6 +280,19 @@ def test_moe_non_finite_tokens_stay_apart(cuda):
     assert torch.equal(y[keep], clean[keep]) and torch.isnan(y[2]).all()
 
 
+@pytest.mark.parametrize("T", [1, 5, 20])
+def test_moe_prequantised(cuda, T):
+    """An e4m3 x with its scales gives what quantising inside the call gives."""
+    layer = _layer(cuda, 8, 512, 256, 12)
+    ids, rw = _route(T, 8, 3, T, cuda)
+    x = R.activations(T, 512, T, torch.bfloat16, cuda)
+    scratch = torch.zeros(ext.fp8_moe_scratch_bytes(T, 3, 512, 256), dtype=torch.uint8, device=cuda)
+    q, s = ext.fp8_quantize(x)
+    a = ext.fp8_moe_decode(q, torch.empty_like(x), *layer, ids, rw, 10.0, scratch, x_scale=s)
+    b = ext.fp8_moe_decode(x, torch.empty_like(x), *layer, ids, rw, 10.0, scratch)
+    assert torch.equal(a, b)
+
+
 def test_moe_many_rows_in_pieces(cuda):
     layer = _layer(cuda, 4, 256, 128, 6)
     ids, rw = _route(150, 4, 2, 9, cuda)
@@ -411,6 +424,8 @@ def test_refusals(cuda):
         (lambda: ext.fp8_linear(x.cpu(), w, ws), "different devices"),
         (lambda: mo(x=xm[:, :128]), "contiguous"),
         (lambda: mo(x=xm.cpu()), "device"),
+        (lambda: mo(x=xm.to(R.F8)), "x_scale"),
+        (lambda: mo(x_scale=rw), "x_scale"),
         (lambda: mo(expert_ids=ids.short()), "expert_ids"),
         (lambda: mo(routing_weights=rw.double()), "routing_weights"),
         (lambda: mo(swiglu_limit=0.0), "limit"),
