@@ -113,7 +113,7 @@ class LinearFP8:
                 weight = padded.view(torch.float8_e4m3fn)[:, :k]
         self.weight = weight
         self.weight_scale = weight_scale.to(torch.float32).contiguous()
-        _ext._fp8_weight_checks(self.weight, self.weight_scale)
+        self._w = _ext._Fp8Weight(self.weight, self.weight_scale)
         self.out_features, self.in_features = (int(v) for v in weight.shape)
         self.bias = bias
         self.default_out_dtype = out_dtype or torch.half
@@ -127,8 +127,7 @@ class LinearFP8:
         return cls(q, scale, **kw)
 
     def forward(self, x: torch.Tensor, params: dict | None = None, out_dtype: torch.dtype | None = None):
-        return _ext._fp8_linear(x, self.weight, self.weight_scale, None, self.bias,
-                                out_dtype or self.default_out_dtype, self.pow2_scale)
+        return _ext._fp8_linear(x, self._w, None, self.bias, out_dtype or self.default_out_dtype, self.pow2_scale)
 
     def unload(self):
         pass

@@ -70,7 +70,7 @@ def _router_outputs(ids: torch.Tensor, weights: torch.Tensor, expert_map: torch.
     ids = ids.reshape(ids.shape[0], -1) if ids.dim() != 2 else ids
     if not ids.is_contiguous():
         ids = ids.contiguous()
-    w = weights.reshape(ids.shape)
+    w = weights if weights.shape == ids.shape else weights.reshape(ids.shape)
     if w.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         w = w.to(torch.float32)
     if not w.is_contiguous():
@@ -247,8 +247,8 @@ class Fp8MoeState:
         self.gate_up, self.down = gate_up, down
         self.gate_up_scale = gate_up_scale.to(torch.float32).contiguous()
         self.down_scale = down_scale.to(torch.float32).contiguous()
-        self.n_experts, self.hidden, self.inter = _ext._fp8_moe_weight_checks(
-            self.gate_up, self.gate_up_scale, self.down, self.down_scale)
+        self.experts = _ext._Fp8Experts(self.gate_up, self.gate_up_scale, self.down, self.down_scale)
+        self.n_experts, self.hidden, self.inter = self.experts.E, self.experts.H, self.experts.I
         self.pow2_scale = bool(pow2_scale)
 
 
@@ -263,7 +263,7 @@ def _fp8_moe_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
         scratch[:_ext._lib.FP8_MOE_CTRL_BYTES].zero_()
         return scratch
-    key = (device, _ext._stream(device))
+    key = (device.index, _ext._raw_stream(device.index))
     buf = _FP8_SCRATCH.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
@@ -274,27 +274,34 @@ def _fp8_moe_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
 def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, state: Fp8MoeState,
                   expert_map: torch.Tensor | None = None, limit: float = 10.0,
                   out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
-    """The routed experts of an e4m3 layer: two kernels up to the row ceiling
-    of fp8_moe_decode, the rows in pieces of that size above it.  Returns the
-    [T, hidden] output, or None when the call is declined."""
-    T, topk = int(x2d.shape[0]), int(ids.shape[-1])
-    if not x2d.is_cuda or x2d.dim() != 2 or T < 1 or int(x2d.shape[1]) != state.hidden or not 1 <= topk <= 16:
-        _decline(f"fp8 geometry x={tuple(x2d.shape)} topk={topk}")
+    """The routed experts of an e4m3 layer: fp8_moe_decode, the rows in pieces
+    above its row ceiling.  Returns the [T, hidden] output, or None when the
+    call is declined."""
+    if not x2d.is_cuda or x2d.dim() != 2 or x2d.size(0) < 1 or x2d.size(1) != state.hidden \
+            or not 1 <= ids.size(-1) <= 16:
+        _decline(f"fp8 geometry x={tuple(x2d.shape)} topk={int(ids.shape[-1])}")
         return None
+    T, topk = x2d.size(0), ids.size(-1)
     ids2, route_w = _router_outputs(ids, weights, expert_map)
-    x = x2d if x2d.dtype in (torch.float16, torch.bfloat16, torch.float32) else x2d.to(torch.float16)
-    x = x.contiguous()
+    x = x2d if x2d.dtype in _ext._DT else x2d.to(torch.float16)
+    if not x.is_contiguous():
+        x = x.contiguous()
     if out is None:
         out = torch.empty(x.shape, dtype=out_dtype or (x.dtype if x.dtype != torch.float32 else torch.float16),
                           device=x.device)
-    step = min(_ext.fp8_moe_max_rows(), 256 // topk)
-    with _ext._on_device(x.device):
-        scratch = _fp8_moe_scratch(x.device, _ext.fp8_moe_scratch_bytes(min(T, step), topk, state.hidden, state.inter))
+    step = min(64, 256 // topk)
+    w = state.experts
+    if torch.cuda.current_device() != x.device.index:      # captures are asked of the current device's stream
+        with _ext._on_device(x.device):
+            return apply_fp8_moe(x, ids2, route_w, state, expert_map, limit, out)
+    scratch = _fp8_moe_scratch(x.device, w.scratch_bytes(min(T, step), topk))
+    if T <= step:
+        _ext._fp8_moe_decode(x, None, out, w, ids2, route_w, limit, scratch, expert_map, state.pow2_scale, None)
+    else:
         for t in range(0, T, step):
             part = slice(t, min(T, t + step))
-            _ext._fp8_moe_decode(x[part], None, out[part], state.gate_up, state.gate_up_scale, state.down, state.down_scale,
-                                 state.n_experts, state.hidden, state.inter, ids2[part], route_w[part], limit, scratch,
-                                 expert_map, state.pow2_scale, None)
+            _ext._fp8_moe_decode(x[part], None, out[part], w, ids2[part], route_w[part], limit, scratch, expert_map,
+                                 state.pow2_scale, None)
     _CALLS["b200"] += 1
     return out
 

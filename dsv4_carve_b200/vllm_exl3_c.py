@@ -49,6 +49,11 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The raw handle without a Stream object around it: 0.1 us instead of 2.2 us, of a call's 10.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class _on_device:
     """Make `device` current for the C-ABI call when it is not already."""
 
@@ -563,13 +568,24 @@ def _rows_of(x: torch.Tensor) -> tuple:
     k = x.size(-1)
     if x.dim() != 2:
         x = x.reshape(-1, k)
-    rows, ld = x.size(0), x.stride(0)
-    if rows <= 1:
+    ld, step = x.stride()
+    if x.size(0) <= 1:
         ld = k
-    if (x.stride(1) != 1 and k > 1) or ld < k:
+    if (step != 1 and k > 1) or ld < k:
         x = x.contiguous()
         ld = k
     return x, ld
+
+
+def _c_call(index: int, fn, *args) -> None:
+    """fn(*args, stream) on device `index` and its current stream."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with _on_device(torch.device("cuda", index)):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def fp8_quantize(x: torch.Tensor, *, block_rows: int = 1, pow2_scale: bool = False) -> tuple:
@@ -579,20 +595,25 @@ def fp8_quantize(x: torch.Tensor, *, block_rows: int = 1, pow2_scale: bool = Fal
 
     scale = max(amax / 448, 2^-126); with ``pow2_scale`` the smallest power of
     two that is not below it.  q = e4m3 nearest to x / scale, ties to even."""
-    _check(x.is_cuda, "fp8_quantize: the B200 build runs on CUDA tensors only")
-    _check(x.dtype in _DT, "fp8_quantize: x must be fp16, bf16 or fp32")
-    _check(block_rows in (1, _FP8_GROUP), "fp8_quantize: block_rows must be 1 or 128")
-    _check(x.dim() >= 1 and x.size(-1) >= 1, "fp8_quantize: x must have at least one column")
-    _check(block_rows == 1 or x.dim() == 2, "fp8_quantize: blocks of 128 rows need a 2-D x")
+    code = _DT.get(x.dtype)
+    if not x.is_cuda or code is None or block_rows not in (1, _FP8_GROUP) or x.dim() < 1 or x.size(-1) < 1 \
+            or (block_rows != 1 and x.dim() != 2):
+        _check(x.is_cuda, "fp8_quantize: the B200 build runs on CUDA tensors only")
+        _check(code is not None, "fp8_quantize: x must be fp16, bf16 or fp32")
+        _check(block_rows in (1, _FP8_GROUP), "fp8_quantize: block_rows must be 1 or 128")
+        _check(x.dim() >= 1 and x.size(-1) >= 1, "fp8_quantize: x must have at least one column")
+        _check(False, "fp8_quantize: blocks of 128 rows need a 2-D x")
     x2, ld = _rows_of(x)
     rows, cols = x2.shape
-    q = torch.empty(x.shape, dtype=_F8, device=x.device)
     groups = -(-cols // _FP8_GROUP)
-    shape = (*x.shape[:-1], groups) if block_rows == 1 else (-(-rows // _FP8_GROUP), groups)
+    q = torch.empty(x.shape, dtype=_F8, device=x.device)
+    if block_rows == 1:
+        shape = (rows, groups) if x.dim() == 2 else (*x.shape[:-1], groups)
+    else:
+        shape = (-(-rows // _FP8_GROUP), groups)
     scale = torch.empty(shape, dtype=torch.float32, device=x.device)
-    with _on_device(x.device):
-        _lib.call("exl3_fp8_quantize", x2.data_ptr(), _DT[x.dtype], rows, cols, ld, q.data_ptr(), cols,
-                  scale.data_ptr(), int(block_rows), int(bool(pow2_scale)), _stream(x.device))
+    _c_call(x.device.index, _lib.load().exl3_fp8_quantize, x2.data_ptr(), code, rows, cols, ld, q.data_ptr(), cols,
+            scale.data_ptr(), block_rows, 1 if pow2_scale else 0)
     return q, scale
 
 
@@ -620,50 +641,67 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
     (``pow2_scale`` as in fp8_quantize), or x is float8_e4m3fn with its
     ``x_scale`` [..., ceil(k / 128)].  ``out_dtype`` defaults to x's type
     (bf16 for an e4m3 x)."""
-    _fp8_weight_checks(weight, weight_scale)
-    return _fp8_linear(x, weight, weight_scale, x_scale, bias, out_dtype, pow2_scale)
+    return _fp8_linear(x, _Fp8Weight(weight, weight_scale), x_scale, bias, out_dtype, pow2_scale)
 
 
-def _fp8_linear(x, weight, weight_scale, x_scale, bias, out_dtype, pow2_scale) -> torch.Tensor:
+class _Fp8Weight:
+    """An e4m3 weight as the C ABI takes it, checked once."""
+    __slots__ = ("weight", "scale", "n", "k", "groups", "device", "args")
+
+    def __init__(self, weight: torch.Tensor, weight_scale: torch.Tensor):
+        _fp8_weight_checks(weight, weight_scale)
+        self.weight, self.scale, self.device = weight, weight_scale, weight.device
+        self.n, self.k = (int(v) for v in weight.shape)
+        self.groups = -(-self.k // _FP8_GROUP)
+        ldw = weight.stride(0) if self.n > 1 else -(-self.k // 16) * 16
+        self.args = (weight.data_ptr(), ldw, weight_scale.data_ptr())
+
+
+def _fp8_linear(x, w: _Fp8Weight, x_scale, bias, out_dtype, pow2_scale) -> torch.Tensor:
     """fp8_linear behind the checks of the weight, which LinearFP8 makes once."""
-    n, k = weight.shape
-    device = weight.device
+    n, k, device = w.n, w.k, w.device
     x_code = _DT_X8.get(x.dtype)
-    _check(x_code is not None, "fp8_linear: x must be fp16, bf16, fp32 or float8_e4m3fn")
-    _check(x.device == device, "fp8_linear: x and weight on different devices")
-    _check(x.dim() >= 1 and x.size(-1) == k, "fp8_linear: x feature dimension does not match weight")
+    dim = x.dim()
+    if x_code is None or x.device != device or dim < 1 or x.size(-1) != k:
+        _check(x_code is not None, "fp8_linear: x must be fp16, bf16, fp32 or float8_e4m3fn")
+        _check(x.device == device, "fp8_linear: x and weight on different devices")
+        _check(False, "fp8_linear: x feature dimension does not match weight")
     x2, ld = _rows_of(x)
     rows = x2.size(0)
     xs_ptr = None
     if x_code == _lib.DT_E4M3:
         _check(x_scale is not None and x_scale.device == device and x_scale.dtype == torch.float32
-               and x_scale.shape == (*x.shape[:-1], -(-k // _FP8_GROUP)),
+               and x_scale.shape == (*x.shape[:-1], w.groups),
                "fp8_linear: an e4m3 x needs x_scale fp32 [..., ceil(in / 128)]")
         x_scale = x_scale.contiguous()
         xs_ptr = x_scale.data_ptr()
-    else:
-        _check(x_scale is None, "fp8_linear: x_scale goes with an e4m3 x only")
+    elif x_scale is not None:
+        _check(False, "fp8_linear: x_scale goes with an e4m3 x only")
     if out_dtype is None:
         out_dtype = torch.bfloat16 if x_code == _lib.DT_E4M3 else x.dtype
     y_code = _DT.get(out_dtype)
-    _check(y_code is not None, "fp8_linear: out_dtype must be fp16, bf16 or fp32")
+    if y_code is None:
+        _check(False, "fp8_linear: out_dtype must be fp16, bf16 or fp32")
     bias_ptr, bias_code = None, 0
     if bias is not None:
-        _check(bias.device == device and bias.dtype in _DT and bias.shape == (n,) and (bias.stride(0) == 1 or n == 1),
+        bias_code = _DT.get(bias.dtype)
+        _check(bias.device == device and bias_code is not None and bias.shape == (n,)
+               and (n == 1 or bias.stride(0) == 1),
                "fp8_linear: bias must be contiguous fp16, bf16 or fp32 [out_features]")
-        bias_ptr, bias_code = bias.data_ptr(), _DT[bias.dtype]
-    y = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=device)
+        bias_ptr = bias.data_ptr()
+    y = torch.empty((rows, n) if dim == 2 else (*x.shape[:-1], n), dtype=out_dtype, device=device)
     if rows == 0:
         return y
     lib = _lib.load()
-    need = lib.exl3_fp8_linear_scratch_bytes(rows, k, n, x_code)
-    scratch = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    with _on_device(device):
-        _lib.check(lib.exl3_fp8_linear(x2.data_ptr(), x_code, ld, xs_ptr, rows, k, n, weight.data_ptr(),
-                                       weight.stride(0) if n > 1 else -(-k // 16) * 16, weight_scale.data_ptr(),
-                                       bias_ptr, bias_code, y.data_ptr(), y_code, n, int(bool(pow2_scale)),
-                                       scratch.data_ptr() if scratch is not None else None, max(need, 0),
-                                       _stream(device)))
+    scratch, scratch_ptr, need = None, None, 0
+    if rows > 1:
+        need = lib.exl3_fp8_linear_scratch_bytes(rows, k, n, x_code)
+        if need > 0:
+            # from the allocator each time: a captured graph owns its own, and streams share none
+            scratch = torch.empty(need, dtype=torch.uint8, device=device)
+            scratch_ptr = scratch.data_ptr()
+    _c_call(device.index, lib.exl3_fp8_linear, x2.data_ptr(), x_code, ld, xs_ptr, rows, k, n, *w.args, bias_ptr,
+            bias_code, y.data_ptr(), y_code, n, 1 if pow2_scale else 0, scratch_ptr, need)
     return y
 
 
@@ -724,17 +762,35 @@ def fp8_moe_decode(x: torch.Tensor, out: torch.Tensor, gate_up: torch.Tensor, ga
     router's outputs go in as lna2_moe_decode_routed takes them (int32 or int64
     ids, fp32 / bf16 / fp16 weights, an optional expert_map); `scratch` as
     there, of fp8_moe_scratch_bytes() bytes, zeroed before its first use."""
-    E, H, I = _fp8_moe_weight_checks(gate_up, gate_up_scale, down, down_scale)
-    return _fp8_moe_decode(x, x_scale, out, gate_up, gate_up_scale, down, down_scale, E, H, I, expert_ids,
-                           routing_weights, swiglu_limit, scratch, expert_map, pow2_scale, check_status)
+    w = _Fp8Experts(gate_up, gate_up_scale, down, down_scale)
+    return _fp8_moe_decode(x, x_scale, out, w, expert_ids, routing_weights, swiglu_limit, scratch, expert_map,
+                           pow2_scale, check_status)
 
 
-def _fp8_moe_decode(x, x_scale, out, gate_up, gate_up_scale, down, down_scale, E, H, I, expert_ids, routing_weights,
-                    swiglu_limit, scratch, expert_map, pow2_scale, check_status) -> torch.Tensor:
+class _Fp8Experts:
+    """A layer's e4m3 experts as the C ABI takes them, checked once."""
+    __slots__ = ("tensors", "E", "H", "I", "device", "args", "need")
+
+    def __init__(self, gate_up, gate_up_scale, down, down_scale):
+        self.E, self.H, self.I = _fp8_moe_weight_checks(gate_up, gate_up_scale, down, down_scale)
+        self.tensors = (gate_up, gate_up_scale, down, down_scale)
+        self.device = gate_up.device
+        self.args = (*(t.data_ptr() for t in self.tensors), self.E)
+        self.need = {}
+
+    def scratch_bytes(self, m: int, topk: int) -> int:
+        need = self.need.get((m, topk))
+        if need is None:
+            need = self.need[(m, topk)] = fp8_moe_scratch_bytes(m, topk, self.H, self.I)
+        return need
+
+
+def _fp8_moe_decode(x, x_scale, out, w: _Fp8Experts, expert_ids, routing_weights, swiglu_limit, scratch, expert_map,
+                    pow2_scale, check_status) -> torch.Tensor:
     """fp8_moe_decode behind the checks of the weights, which Fp8MoeState makes once."""
     import ctypes
 
-    device = gate_up.device
+    device, H = w.device, w.H
     x_code = _DT_X8.get(x.dtype)
     _check(x.device == device and x_code is not None and x.dim() == 2 and x.size(1) == H and x.is_contiguous(),
            "fp8_moe_decode: x must be contiguous fp16, bf16, fp32 or float8_e4m3fn [m, hidden] on the weights' device")
@@ -745,23 +801,26 @@ def _fp8_moe_decode(x, x_scale, out, gate_up, gate_up_scale, down, down_scale, E
                and x_scale.shape == (m, H // _FP8_GROUP) and x_scale.is_contiguous() and x.data_ptr() % 16 == 0,
                "fp8_moe_decode: an e4m3 x needs 16-byte alignment and x_scale contiguous fp32 [m, hidden / 128]")
         xs_ptr = x_scale.data_ptr()
-    else:
-        _check(x_scale is None, "fp8_moe_decode: x_scale goes with an e4m3 x only")
-    _check(out.device == device and out.dtype in _DT and out.shape == x.shape and out.is_contiguous(),
+    elif x_scale is not None:
+        _check(False, "fp8_moe_decode: x_scale goes with an e4m3 x only")
+    out_code = _DT.get(out.dtype)
+    _check(out.device == device and out_code is not None and out.shape == x.shape and out.is_contiguous(),
            "fp8_moe_decode: out must be contiguous fp16, bf16 or fp32 of x's shape on its device")
-    _check(expert_ids.device == device and expert_ids.dtype in _IDS_DT and expert_ids.is_contiguous()
+    ids_code = _IDS_DT.get(expert_ids.dtype)
+    _check(expert_ids.device == device and ids_code is not None and expert_ids.is_contiguous()
            and expert_ids.dim() == 2 and expert_ids.size(0) == m,
            "fp8_moe_decode: expert_ids must be contiguous int32 or int64 [m, topk]")
     topk = expert_ids.size(1)
-    _check(routing_weights.device == device and routing_weights.dtype in _DT and routing_weights.is_contiguous()
+    w_code = _DT.get(routing_weights.dtype)
+    _check(routing_weights.device == device and w_code is not None and routing_weights.is_contiguous()
            and routing_weights.shape == expert_ids.shape,
            "fp8_moe_decode: routing_weights must be contiguous fp32, bf16 or fp16 [m, topk]")
-    lib = _lib.load()
-    need = lib.exl3_fp8_moe_scratch_bytes(m, topk, H, I)
-    _check(need > 0, "fp8_moe_decode: 1..64 rows, top-k 1..16, rows * top-k up to 256, hidden up to 16384 and "
-                     "intermediate up to 8192 are served")
+    need = w.scratch_bytes(m, topk)
     limit = float(swiglu_limit)
-    _check(limit > 0.0, "fp8_moe_decode: the SwiGLU limit must be positive")
+    if need <= 0 or not limit > 0.0:
+        _check(need > 0, "fp8_moe_decode: 1..64 rows, top-k 1..16, rows * top-k up to 256, hidden up to 16384 and "
+                         "intermediate up to 8192 are served")
+        _check(False, "fp8_moe_decode: the SwiGLU limit must be positive")
     _check(scratch.device == device and scratch.dtype == torch.uint8 and scratch.is_contiguous()
            and scratch.numel() >= need, "fp8_moe_decode: scratch too small")
     map_ptr, n_global = None, 0
@@ -770,14 +829,11 @@ def _fp8_moe_decode(x, x_scale, out, gate_up, gate_up_scale, down, down_scale, E
                and expert_map.is_contiguous() and expert_map.numel() >= 1,
                "EXL3 expert_map must be a contiguous CUDA int64 [n_global] on the hidden-state device")
         map_ptr, n_global = expert_map.data_ptr(), expert_map.numel()
-    route = _lib.MoeRoute(expert_ids.data_ptr(), _IDS_DT[expert_ids.dtype], routing_weights.data_ptr(),
-                          _DT[routing_weights.dtype], map_ptr, n_global)
-    with _on_device(device):
-        _lib.check(lib.exl3_fp8_moe_decode(x.data_ptr(), x_code, xs_ptr, out.data_ptr(), _DT[out.dtype], m, H, I,
-                                           gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(),
-                                           down_scale.data_ptr(), E, ctypes.addressof(route), topk, limit,
-                                           int(bool(pow2_scale)), scratch.data_ptr(), scratch.numel(),
-                                           _stream(device)))
-        if check_status_default() if check_status is None else check_status:
+    route = _lib.MoeRoute(expert_ids.data_ptr(), ids_code, routing_weights.data_ptr(), w_code, map_ptr, n_global)
+    _c_call(device.index, _lib.load().exl3_fp8_moe_decode, x.data_ptr(), x_code, xs_ptr, out.data_ptr(), out_code, m,
+            H, w.I, *w.args, ctypes.addressof(route), topk, limit, 1 if pow2_scale else 0, scratch.data_ptr(),
+            scratch.numel())
+    if check_status_default() if check_status is None else check_status:
+        with _on_device(device):
             _raise_on_status(scratch)
     return out
