@@ -24,6 +24,12 @@ dim 0 and suh).
 What is built is what the kernels bind to: a ``synth.MoeLayer`` with the nine
 device pointer tables and the per-expert K table of ``lna2_moe_decode``, and
 ``LinearEXL3`` for dense modules.  Nothing here touches the GPU kernels.
+
+Modules that the pack leaves in the checkpoint's e4m3 -- ``<prefix>.weight``
+float8_e4m3fn [out, in] with one scale for each 128 x 128 block in
+``<prefix>.scale``, ``.weight_scale_inv`` or ``.weight_scale`` (fp32, bf16, or
+float8_e8m0fnu for powers of two) -- load as ``LinearFP8`` and, for routed
+experts, as ``moe.Fp8MoeState``.
 """
 from __future__ import annotations
 
@@ -34,13 +40,15 @@ from typing import Any
 
 import torch
 
-from . import synth
-from .linear import LinearEXL3
+from . import moe, synth
+from .linear import LinearEXL3, LinearFP8
 
 MCG_MARKER = -877912083
 MUL1_MARKER = -2082680531
 EXL3_SUFFIXES = ("trellis", "suh", "svh", "mcg", "mul1")
 EXPERT_PROJ = {"gate": "w1", "up": "w3", "down": "w2"}
+FP8_SCALE_SUFFIXES = ("scale", "weight_scale_inv", "weight_scale")
+FP8_BLOCK = 128
 SUPPORTED_BITS = (2, 3, 4, 5, 6)
 _LAYER_RE = re.compile(r"(?:^|\.)layers\.(\d+)(?:\.|$)")
 
@@ -251,10 +259,81 @@ def load_moe_layer(ckpt: Checkpoint, layer: int, n_experts: int, rank: int = 0, 
     return L
 
 
-def load_linear(ckpt: Checkpoint, prefix: str, device="cuda", config: Exl3QuantConfig | None = None) -> LinearEXL3:
-    """A dense EXL3 module (attention / shared expert) as the LinearEXL3 the
-    plugin's dense branch calls; K is checked against non_routed_exl3 when the
-    config lists the module."""
+def has_fp8(ckpt: Checkpoint, prefix: str) -> bool:
+    """Whether the module is stored as an e4m3 weight with block scales."""
+    return (not ckpt.has(f"{prefix}.trellis") and ckpt.has(f"{prefix}.weight")
+            and any(ckpt.has(f"{prefix}.{s}") for s in FP8_SCALE_SUFFIXES))
+
+
+def load_fp8_weight(ckpt: Checkpoint, prefix: str, device="cpu") -> tuple:
+    """(weight e4m3 [out, in], scale fp32 [ceil(out / 128), ceil(in / 128)],
+    whether the scales are stored as powers of two)."""
+    weight = ckpt.get(f"{prefix}.weight", device)
+    name = next((f"{prefix}.{s}" for s in FP8_SCALE_SUFFIXES if ckpt.has(f"{prefix}.{s}")), None)
+    if name is None:
+        raise KeyError(f"{prefix}: no block scales ({', '.join(FP8_SCALE_SUFFIXES)})")
+    scale = ckpt.get(name, device)
+    if weight.dtype != torch.float8_e4m3fn or weight.dim() != 2:
+        raise ValueError(f"{prefix}.weight must be float8_e4m3fn [out, in], got {weight.dtype} {tuple(weight.shape)}")
+    want = tuple(-(-int(d) // FP8_BLOCK) for d in weight.shape)
+    pow2 = scale.dtype == torch.float8_e8m0fnu
+    if tuple(scale.shape) != want or not (pow2 or scale.dtype in (torch.float32, torch.bfloat16, torch.float16)):
+        raise ValueError(f"{name} must hold one floating scale for each 128 x 128 block, {want}, "
+                         f"got {scale.dtype} {tuple(scale.shape)}")
+    return weight.contiguous(), scale.to(torch.float32).contiguous(), pow2
+
+
+def shard_fp8_expert(proj: str, weight: torch.Tensor, scale: torch.Tensor, rank: int, world: int) -> tuple:
+    """This rank's part of an expert's e4m3 weight, whole 128-blocks of the
+    intermediate dim: rows of gate / up, columns of down."""
+    if world <= 1:
+        return weight, scale
+    dim = 0 if proj in ("gate", "up") else 1
+    size = int(weight.shape[dim])
+    if size % (world * FP8_BLOCK):
+        raise ValueError(f"e4m3 TP shard: {proj} dim {dim} size {size} is not a whole number of 128-blocks for tp={world}")
+    return _narrow(weight, dim, rank, world, proj), _narrow(scale, dim, rank, world, proj)
+
+
+def load_fp8_moe_layer(ckpt: Checkpoint, layer: int, n_experts: int, rank: int = 0, world: int = 1, device="cuda",
+                       prefix_fmt: str = "layers.{layer}.ffn.experts.{expert}") -> "moe.Fp8MoeState":
+    """All routed experts of one layer that are stored in e4m3, this rank's TP
+    shard, stacked on `device` as fp8_moe_decode and apply_moe take them."""
+    gu, gus, dn, dns, kinds = [], [], [], [], set()
+    for e in range(n_experts):
+        base = expert_prefix(layer, e, prefix_fmt)
+        w = {}
+        for proj, wname in EXPERT_PROJ.items():
+            weight, scale, pow2 = load_fp8_weight(ckpt, f"{base}.{wname}")
+            w[proj] = shard_fp8_expert(proj, weight, scale, rank, world)
+            kinds.add(pow2)
+        (g, gs), (u, us), (d, ds) = w["gate"], w["up"], w["down"]
+        if g.shape != u.shape or d.shape != (g.shape[1], g.shape[0]):
+            raise ValueError(f"{base}: gate/up/down shapes disagree")
+        if g.shape[0] % FP8_BLOCK or g.shape[1] % FP8_BLOCK:
+            raise ValueError(f"{base}: hidden {g.shape[1]} and intermediate shard {g.shape[0]} must be multiples of 128")
+        if gu and (torch.cat([g.view(torch.uint8)] * 2).shape != gu[0].shape):
+            raise ValueError(f"{base}: expert shape differs from the first expert's")
+        gu.append(torch.cat([g.view(torch.uint8), u.view(torch.uint8)]))
+        gus.append(torch.cat([gs, us]))
+        dn.append(d.view(torch.uint8))
+        dns.append(ds)
+    if len(kinds) != 1:
+        raise ValueError(f"layer {layer}: experts mix power-of-two and other scales")
+    f8 = torch.float8_e4m3fn
+    return moe.Fp8MoeState(torch.stack(gu).to(device).view(f8), torch.stack(gus).to(device),
+                           torch.stack(dn).to(device).view(f8), torch.stack(dns).to(device), pow2_scale=kinds.pop())
+
+
+def load_linear(ckpt: Checkpoint, prefix: str, device="cuda", config: Exl3QuantConfig | None = None):
+    """A dense module (attention / shared expert): the LinearEXL3 that the
+    plugin's dense branch calls, K checked against non_routed_exl3 when the
+    config lists the module; or LinearFP8 where the pack leaves the module in
+    e4m3 with block scales."""
+    if has_fp8(ckpt, prefix):
+        weight, scale, pow2 = load_fp8_weight(ckpt, prefix, device)
+        bias = ckpt.get(f"{prefix}.bias", device) if ckpt.has(f"{prefix}.bias") else None
+        return LinearFP8(weight, scale, bias=bias, pow2_scale=pow2, key=prefix)
     config = config or ckpt.config
     bits = None
     if config is not None and config.matches_non_routed(prefix):
