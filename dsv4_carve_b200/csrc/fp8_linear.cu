@@ -391,21 +391,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
         if (rank == 0) {
             const uint32_t id = idesc_f16(256, NW);
             const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
-            int it = 0;
-            bool ok = true;
-            for (int t = pair; t < p.tiles && ok; t += pairs)
-                for (int kb = 0; kb < p.groups; ++kb, ++it) {
-                    const int st = it % L::kStages, b = it % L::kBufs;
-                    ok = mbar_poll2_lanes(&H.full[st], (it / L::kStages) & 1u, &H.tempty[b], ((it / L::kBufs) + 1u) & 1u, status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t ad = desc0 + (uint64_t) (st * (L::kStage >> 4)), bd = ad + (L::kA >> 4);
-                    if (elect_lane()) {
+            const int total = ((p.tiles - pair + pairs - 1) / pairs) * p.groups;     // steps of this pair
+            for (int it = 0; it < total; ++it) {
+                const int st = it % L::kStages, b = it % L::kBufs;
+                if (!mbar_poll2_lanes(&H.full[st], (it / L::kStages) & 1u, &H.tempty[b], ((it / L::kBufs) + 1u) & 1u, status)) break;
+                tc_fence_after();
+                const uint64_t ad = desc0 + (uint64_t) (st * (L::kStage >> 4)), bd = ad + (L::kA >> 4);
+                if (elect_lane()) {
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) tc_mma_f8_pair(tmem + b * NW, ad + 2 * q, bd + 2 * q, id, q);
-                        tc_commit_pair(&H.done[st]);
-                    }
+                    for (int q = 0; q < 4; ++q) tc_mma_f8_pair(tmem + b * NW, ad + 2 * q, bd + 2 * q, id, q);
+                    tc_commit_pair(&H.done[st]);
                 }
+            }
         }
     } else if (warp > kFgMmaWarp) {
         regs_down();
@@ -466,9 +463,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
             uint8_t* buf = stage_out + warp * L::kOut;
             const int wrow = t / p.ntiles * 256 + (int) rank * 128 + lg * 32;
             if (p.bias != nullptr) {
+                // a column a lane, handed round
+                float bv[L::kCols / 32];
 #pragma unroll
-                for (int j = 0; j < L::kCols; ++j)
-                    if (col0 + j < p.n) acc[j] += load_f32(p.bias, p.bias_dtype, col0 + j);
+                for (int c = 0; c < L::kCols / 32; ++c)
+                    bv[c] = col0 + c * 32 + lane < p.n ? load_f32(p.bias, p.bias_dtype, col0 + c * 32 + lane) : 0.f;
+#pragma unroll
+                for (int j = 0; j < L::kCols; ++j) acc[j] += __shfl_sync(0xffffffffu, bv[j / 32], j % 32);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
