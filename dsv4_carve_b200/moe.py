@@ -291,7 +291,7 @@ def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, s
                           device=x.device)
     step = min(64, 256 // topk)
     w = state.experts
-    if torch.cuda.current_device() != x.device.index:      # captures are asked of the current device's stream
+    if _ext._current_device() != w.index:      # captures are asked of the current device's stream
         with _ext._on_device(x.device):
             return apply_fp8_moe(x, ids2, route_w, state, expert_map, limit, out)
     scratch = _fp8_moe_scratch(x.device, w.scratch_bytes(min(T, step), topk))

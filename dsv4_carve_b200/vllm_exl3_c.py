@@ -24,6 +24,7 @@ e4m3 with one fp32 scale for each 128 x 128 block.
 """
 from __future__ import annotations
 
+import ctypes
 import os
 
 import torch
@@ -49,9 +50,11 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-# The raw handle without a Stream object around it: 0.1 us instead of 2.2 us, of a call's 10.
+# The raw handle without a Stream object around it (0.1 us instead of 2.2 us, of a call's
+# 10), and the current device without the module's own initialisation check.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class _on_device:
@@ -577,17 +580,6 @@ def _rows_of(x: torch.Tensor) -> tuple:
     return x, ld
 
 
-def _c_call(index: int, fn, *args) -> None:
-    """fn(*args, stream) on device `index` and its current stream."""
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with _on_device(torch.device("cuda", index)):
-            rc = fn(*args, _raw_stream(index))
-    if rc:
-        _lib.check(rc)
-
-
 def fp8_quantize(x: torch.Tensor, *, block_rows: int = 1, pow2_scale: bool = False) -> tuple:
     """(q, scale): x in e4m3 with one fp32 scale for each row and 128 columns
     (``block_rows=1``: activations, x [..., cols]) or for each 128 x 128 block
@@ -606,14 +598,20 @@ def fp8_quantize(x: torch.Tensor, *, block_rows: int = 1, pow2_scale: bool = Fal
     x2, ld = _rows_of(x)
     rows, cols = x2.shape
     groups = -(-cols // _FP8_GROUP)
-    q = torch.empty(x.shape, dtype=_F8, device=x.device)
+    index = x.device.index
+    if _current_device() != index:
+        with _on_device(x.device):
+            return fp8_quantize(x, block_rows=block_rows, pow2_scale=pow2_scale)
+    q = x.new_empty(x.shape, dtype=_F8)
     if block_rows == 1:
         shape = (rows, groups) if x.dim() == 2 else (*x.shape[:-1], groups)
     else:
         shape = (-(-rows // _FP8_GROUP), groups)
-    scale = torch.empty(shape, dtype=torch.float32, device=x.device)
-    _c_call(x.device.index, _lib.load().exl3_fp8_quantize, x2.data_ptr(), code, rows, cols, ld, q.data_ptr(), cols,
-            scale.data_ptr(), block_rows, 1 if pow2_scale else 0)
+    scale = x.new_empty(shape, dtype=torch.float32)
+    rc = _lib.load().exl3_fp8_quantize(x2.data_ptr(), code, rows, cols, ld, q.data_ptr(), cols, scale.data_ptr(),
+                                       block_rows, 1 if pow2_scale else 0, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
     return q, scale
 
 
@@ -646,15 +644,16 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
 
 class _Fp8Weight:
     """An e4m3 weight as the C ABI takes it, checked once."""
-    __slots__ = ("weight", "scale", "n", "k", "groups", "device", "args")
+    __slots__ = ("weight", "scale", "n", "k", "groups", "device", "index", "ptr", "ldw", "scale_ptr")
 
     def __init__(self, weight: torch.Tensor, weight_scale: torch.Tensor):
         _fp8_weight_checks(weight, weight_scale)
         self.weight, self.scale, self.device = weight, weight_scale, weight.device
         self.n, self.k = (int(v) for v in weight.shape)
         self.groups = -(-self.k // _FP8_GROUP)
-        ldw = weight.stride(0) if self.n > 1 else -(-self.k // 16) * 16
-        self.args = (weight.data_ptr(), ldw, weight_scale.data_ptr())
+        self.index = weight.device.index
+        self.ldw = weight.stride(0) if self.n > 1 else -(-self.k // 16) * 16
+        self.ptr, self.scale_ptr = weight.data_ptr(), weight_scale.data_ptr()
 
 
 def _fp8_linear(x, w: _Fp8Weight, x_scale, bias, out_dtype, pow2_scale) -> torch.Tensor:
@@ -666,10 +665,13 @@ def _fp8_linear(x, w: _Fp8Weight, x_scale, bias, out_dtype, pow2_scale) -> torch
         _check(x_code is not None, "fp8_linear: x must be fp16, bf16, fp32 or float8_e4m3fn")
         _check(x.device == device, "fp8_linear: x and weight on different devices")
         _check(False, "fp8_linear: x feature dimension does not match weight")
+    if _current_device() != w.index:
+        with _on_device(device):
+            return _fp8_linear(x, w, x_scale, bias, out_dtype, pow2_scale)
     x2, ld = _rows_of(x)
     rows = x2.size(0)
     xs_ptr = None
-    if x_code == _lib.DT_E4M3:
+    if x_code == 3:                                  # e4m3
         _check(x_scale is not None and x_scale.device == device and x_scale.dtype == torch.float32
                and x_scale.shape == (*x.shape[:-1], w.groups),
                "fp8_linear: an e4m3 x needs x_scale fp32 [..., ceil(in / 128)]")
@@ -678,7 +680,7 @@ def _fp8_linear(x, w: _Fp8Weight, x_scale, bias, out_dtype, pow2_scale) -> torch
     elif x_scale is not None:
         _check(False, "fp8_linear: x_scale goes with an e4m3 x only")
     if out_dtype is None:
-        out_dtype = torch.bfloat16 if x_code == _lib.DT_E4M3 else x.dtype
+        out_dtype = torch.bfloat16 if x_code == 3 else x.dtype
     y_code = _DT.get(out_dtype)
     if y_code is None:
         _check(False, "fp8_linear: out_dtype must be fp16, bf16 or fp32")
@@ -689,7 +691,7 @@ def _fp8_linear(x, w: _Fp8Weight, x_scale, bias, out_dtype, pow2_scale) -> torch
                and (n == 1 or bias.stride(0) == 1),
                "fp8_linear: bias must be contiguous fp16, bf16 or fp32 [out_features]")
         bias_ptr = bias.data_ptr()
-    y = torch.empty((rows, n) if dim == 2 else (*x.shape[:-1], n), dtype=out_dtype, device=device)
+    y = x2.new_empty((rows, n) if dim == 2 else (*x.shape[:-1], n), dtype=out_dtype)
     if rows == 0:
         return y
     lib = _lib.load()
@@ -698,10 +700,13 @@ def _fp8_linear(x, w: _Fp8Weight, x_scale, bias, out_dtype, pow2_scale) -> torch
         need = lib.exl3_fp8_linear_scratch_bytes(rows, k, n, x_code)
         if need > 0:
             # from the allocator each time: a captured graph owns its own, and streams share none
-            scratch = torch.empty(need, dtype=torch.uint8, device=device)
+            scratch = x2.new_empty(need, dtype=torch.uint8)
             scratch_ptr = scratch.data_ptr()
-    _c_call(device.index, lib.exl3_fp8_linear, x2.data_ptr(), x_code, ld, xs_ptr, rows, k, n, *w.args, bias_ptr,
-            bias_code, y.data_ptr(), y_code, n, 1 if pow2_scale else 0, scratch_ptr, need)
+    rc = lib.exl3_fp8_linear(x2.data_ptr(), x_code, ld, xs_ptr, rows, k, n, w.ptr, w.ldw, w.scale_ptr, bias_ptr,
+                             bias_code, y.data_ptr(), y_code, n, 1 if pow2_scale else 0, scratch_ptr, need,
+                             _raw_stream(w.index))
+    if rc:
+        _lib.check(rc)
     return y
 
 
@@ -769,12 +774,12 @@ def fp8_moe_decode(x: torch.Tensor, out: torch.Tensor, gate_up: torch.Tensor, ga
 
 class _Fp8Experts:
     """A layer's e4m3 experts as the C ABI takes them, checked once."""
-    __slots__ = ("tensors", "E", "H", "I", "device", "args", "need")
+    __slots__ = ("tensors", "E", "H", "I", "device", "index", "args", "need")
 
     def __init__(self, gate_up, gate_up_scale, down, down_scale):
         self.E, self.H, self.I = _fp8_moe_weight_checks(gate_up, gate_up_scale, down, down_scale)
         self.tensors = (gate_up, gate_up_scale, down, down_scale)
-        self.device = gate_up.device
+        self.device, self.index = gate_up.device, gate_up.device.index
         self.args = (*(t.data_ptr() for t in self.tensors), self.E)
         self.need = {}
 
@@ -788,9 +793,11 @@ class _Fp8Experts:
 def _fp8_moe_decode(x, x_scale, out, w: _Fp8Experts, expert_ids, routing_weights, swiglu_limit, scratch, expert_map,
                     pow2_scale, check_status) -> torch.Tensor:
     """fp8_moe_decode behind the checks of the weights, which Fp8MoeState makes once."""
-    import ctypes
-
     device, H = w.device, w.H
+    if _current_device() != w.index:
+        with _on_device(device):
+            return _fp8_moe_decode(x, x_scale, out, w, expert_ids, routing_weights, swiglu_limit, scratch, expert_map,
+                                   pow2_scale, check_status)
     x_code = _DT_X8.get(x.dtype)
     _check(x.device == device and x_code is not None and x.dim() == 2 and x.size(1) == H and x.is_contiguous(),
            "fp8_moe_decode: x must be contiguous fp16, bf16, fp32 or float8_e4m3fn [m, hidden] on the weights' device")
@@ -830,10 +837,11 @@ def _fp8_moe_decode(x, x_scale, out, w: _Fp8Experts, expert_ids, routing_weights
                "EXL3 expert_map must be a contiguous CUDA int64 [n_global] on the hidden-state device")
         map_ptr, n_global = expert_map.data_ptr(), expert_map.numel()
     route = _lib.MoeRoute(expert_ids.data_ptr(), ids_code, routing_weights.data_ptr(), w_code, map_ptr, n_global)
-    _c_call(device.index, _lib.load().exl3_fp8_moe_decode, x.data_ptr(), x_code, xs_ptr, out.data_ptr(), out_code, m,
-            H, w.I, *w.args, ctypes.addressof(route), topk, limit, 1 if pow2_scale else 0, scratch.data_ptr(),
-            scratch.numel())
+    rc = _lib.load().exl3_fp8_moe_decode(x.data_ptr(), x_code, xs_ptr, out.data_ptr(), out_code, m, H, w.I, *w.args,
+                                         ctypes.addressof(route), topk, limit, 1 if pow2_scale else 0,
+                                         scratch.data_ptr(), scratch.numel(), _raw_stream(w.index))
+    if rc:
+        _lib.check(rc)
     if check_status_default() if check_status is None else check_status:
-        with _on_device(device):
-            _raise_on_status(scratch)
+        _raise_on_status(scratch)
     return out

@@ -71,8 +71,8 @@ def test_linear_argument_checks(buf):
     _err(call(xs=p), "x_scale")
     _err(call(xd=3), "x_scale")
     assert call(rows=0, x=None, w=None, ws=None, y=None) == 0
-    sizes = [lib.exl3_fp8_linear_scratch_bytes(r, 1000, 256, d) for r in (0, 1, 16, 17, 4096) for d in (1, 3)]
-    assert all(v >= 0 for v in sizes) and sizes[-2] >= 4096 * 1000 and sizes[2] == 0
+    sizes = [lib.exl3_fp8_linear_scratch_bytes(r, 1000, 256, d) for r in (0, 1, 8, 17, 4096) for d in (1, 3)]
+    assert all(v >= 0 for v in sizes) and sizes[-2] >= 4096 * 1000 and sizes[2] == 0 and sizes[0] == 0
     assert lib.exl3_fp8_linear_scratch_bytes(-1, 1000, 256, 1) == -1
     assert lib.exl3_fp8_linear_scratch_bytes(4, 1000, 256, 4) == -1
 
