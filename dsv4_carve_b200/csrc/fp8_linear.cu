@@ -303,9 +303,13 @@ struct FgParams {
 
 template <int NW>
 struct FgLayout {
-    static constexpr int kA = 128 * 128, kB = NW / 2 * 128, kStage = kA + kB;
-    static constexpr int kStages = NW == 256 ? 5 : 6;
-    static constexpr int kBufs = kFgTmemCols / NW;
+    // Groups of 128 columns in a step.  Two with the narrow tile: a step's barriers
+    // and its commit cost the issuing warp about as much as four MMAs of 256 x 128
+    // (512 x 4096 x 4096: 15.2 us with one).
+    static constexpr int kKS = NW == 256 ? 1 : 2;
+    static constexpr int kA = 128 * 128, kB = NW / 2 * 128, kGroup = kA + kB, kStage = kKS * kGroup;
+    static constexpr int kStages = NW == 256 ? 5 : 3;
+    static constexpr int kBufs = kFgTmemCols / (NW * kKS);
     static constexpr int kCols = NW / 2;                   // columns of a thread
     static constexpr int kOut = 32 * 256;                  // 256 bytes of a warp's rows on their way out
     static constexpr int kSmem = 1024 + kStages * kStage + kFgEpiWarps * kOut + 512;
@@ -334,6 +338,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const uint32_t rank = cluster_rank();
     const int pair = (int) blockIdx.x >> 1, pairs = (int) gridDim.x >> 1;
+    const int steps = (p.groups + L::kKS - 1) / L::kKS;                       // of a tile
+    const int total = ((p.tiles - pair + pairs - 1) / pairs) * steps;         // of this pair
+    auto groups_of = [&](int step) { return min(L::kKS, p.groups - step * L::kKS); };
     uint32_t* status = &g_fp8_status;
 
     if (tid == 0) {
@@ -352,16 +359,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
         regs_down();
         if (lane == 0) {
             int it = 0, ahead = 0;
-            const int total = ((p.tiles - pair + pairs - 1) / pairs) * p.groups;     // steps of this pair
-            auto weights = [&](int st, int nt, int kb) {
-                if (rank == 0) mbar_arrive_expect_tx(&H.full[st], 2 * L::kStage);
-                tma_load_2d_pair(ring + st * L::kStage + L::kA, &p.wmap, kb * 128, nt * NW + (int) rank * (NW / 2),
-                                 mapa_u32(smem_u32(&H.full[st]), 0));
+            auto weights = [&](int st, int nt, int step) {
+                const int n = groups_of(step);
+                if (rank == 0) mbar_arrive_expect_tx(&H.full[st], 2 * n * L::kGroup);
+                for (int q = 0; q < n; ++q)
+                    tma_load_2d_pair(ring + st * L::kStage + q * L::kGroup + L::kA, &p.wmap, (step * L::kKS + q) * 128,
+                                     nt * NW + (int) rank * (NW / 2), mapa_u32(smem_u32(&H.full[st]), 0));
             };
             if (p.early) {
                 // weights ahead of the quantiser's end (it began after everything before this call)
                 const int nt = pair % p.ntiles;
-                for (; ahead < min(L::kStages, p.groups); ++ahead) weights(ahead, nt, ahead);
+                for (; ahead < min(L::kStages, steps); ++ahead) weights(ahead, nt, ahead);
             }
             pdl_wait();
             pdl_launch_dependents();
@@ -369,14 +377,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
             bool ok = true;
             for (int t = pair; t < p.tiles && ok; t += pairs) {
                 const int nt = t % p.ntiles, row = t / p.ntiles * 256 + (int) rank * 128;
-                for (int kb = 0; kb < p.groups; ++kb, ++it) {
+                for (int step = 0; step < steps; ++step, ++it) {
                     const int st = it % L::kStages;
                     if (it >= L::kStages) {
                         ok = mbar_poll(&H.done[st], ((it / L::kStages) + 1u) & 1u, status);
                         if (!ok) break;
                     }
-                    if (it >= ahead) weights(st, nt, kb);
-                    tma_load_2d_pair(ring + st * L::kStage, &p.xmap, kb * 128, row, mapa_u32(smem_u32(&H.full[st]), 0));
+                    if (it >= ahead) weights(st, nt, step);
+                    for (int q = 0; q < groups_of(step); ++q)
+                        tma_load_2d_pair(ring + st * L::kStage + q * L::kGroup, &p.xmap, (step * L::kKS + q) * 128, row,
+                                         mapa_u32(smem_u32(&H.full[st]), 0));
                 }
             }
             // no copy may still be in flight when the CTA retires: the pair's last MMAs have read every stage
@@ -391,15 +401,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
         if (rank == 0) {
             const uint32_t id = idesc_f16(256, NW);
             const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
-            const int total = ((p.tiles - pair + pairs - 1) / pairs) * p.groups;     // steps of this pair
-            for (int it = 0; it < total; ++it) {
+            for (int it = 0, step = 0; it < total; ++it, step = step + 1 == steps ? 0 : step + 1) {
                 const int st = it % L::kStages, b = it % L::kBufs;
                 if (!mbar_poll2_lanes(&H.full[st], (it / L::kStages) & 1u, &H.tempty[b], ((it / L::kBufs) + 1u) & 1u, status)) break;
                 tc_fence_after();
                 const uint64_t ad = desc0 + (uint64_t) (st * (L::kStage >> 4)), bd = ad + (L::kA >> 4);
+                const int n = groups_of(step);
                 if (elect_lane()) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) tc_mma_f8_pair(tmem + b * NW, ad + 2 * q, bd + 2 * q, id, q);
+                    for (int g = 0; g < L::kKS; ++g) {
+                        if (g >= n) break;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            tc_mma_f8_pair(tmem + (b * L::kKS + g) * NW, ad + g * (L::kGroup >> 4) + 2 * q, bd + g * (L::kGroup >> 4) + 2 * q, id, q);
+                    }
                     tc_commit_pair(&H.done[st]);
                 }
             }
@@ -426,32 +441,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
 #pragma unroll
             for (int j = 0; j < L::kCols; ++j) acc[j] = 0.f;
             // scales two steps ahead: a step is shorter than a load from L2
-            auto scales = [&](int kb) { return live && wlive && kb < p.groups ? make_float2(__ldcg(xs + kb * p.xsg), __ldg(ws + kb)) : make_float2(0.f, 0.f); };
-            float2 s0 = scales(0), s1 = scales(1);
-            for (int kb = 0; kb < p.groups; ++kb, ++it) {
-                const int b = it % L::kBufs;
-                const float f = s0.x * s0.y;
+            struct Scales { float x[L::kKS], w[L::kKS]; };
+            auto scales = [&](int step) {
+                Scales v;
+#pragma unroll
+                for (int g = 0; g < L::kKS; ++g) {
+                    const int kb = step * L::kKS + g;
+                    const bool on = live && wlive && kb < p.groups;
+                    v.x[g] = on ? __ldcg(xs + kb * p.xsg) : 0.f;
+                    v.w[g] = on ? __ldg(ws + kb) : 0.f;
+                }
+                return v;
+            };
+            Scales s0 = scales(0), s1 = scales(1);
+            for (int step = 0; step < steps; ++step, ++it) {
+                const int b = it % L::kBufs, n = groups_of(step);
+                float f[L::kKS];
+#pragma unroll
+                for (int g = 0; g < L::kKS; ++g) f[g] = s0.x[g] * s0.w[g];
                 s0 = s1;
-                s1 = scales(kb + 2);
+                s1 = scales(step + 2);
                 ok = mbar_poll_lanes(&H.done[it % L::kStages], (it / L::kStages) & 1u, status);
                 if (!ok) break;
                 tc_fence_after();
                 // the next 32 columns are on their way while these are scaled
                 constexpr int NC = L::kCols / 32;
                 uint32_t v[2][32];
-                tc_ld32_issue(tcol + (uint32_t) (b * NW), v[0]);
+                auto col_of = [&](int i) { return tcol + (uint32_t) ((b * L::kKS + i / NC) * NW + i % NC * 32); };
+                tc_ld32_issue(col_of(0), v[0]);
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    tc_ld32_wait(v[c & 1]);
-                    if (c + 1 < NC) {
-                        tc_ld32_issue(tcol + (uint32_t) (b * NW + (c + 1) * 32), v[(c + 1) & 1]);
+                for (int i = 0; i < NC * L::kKS; ++i) {
+                    const int c = i % NC;
+                    if (i / NC >= n) break;
+                    tc_ld32_wait(v[i & 1]);
+                    if (i + 1 < NC * n) {
+                        tc_ld32_issue(col_of(i + 1), v[(i + 1) & 1]);
                     } else {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * (uint32_t) b);
                     }
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[c & 1][j]), f, acc[c * 32 + j]);
+                    for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[i & 1][j]), f[i / NC], acc[c * 32 + j]);
                 }
             }
             if (!ok) break;

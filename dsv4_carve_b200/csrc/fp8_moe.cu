@@ -380,6 +380,7 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
             pdl_wait();
         }
     } else if (warp == kFmMmaWarp) {
+        pdl_wait();                                                   // the bounded waits begin behind it
         const uint64_t wdesc0 = sdesc_sw128(smem_u32(ring));
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
         int slot = 0;
@@ -475,8 +476,8 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[mat][j] = 0.f;
         };
+        pdl_wait();
         if (PH == 1) {
-            pdl_wait();
             if (total == 0)
                 for (int64_t i = (int64_t) cta * 128 + tid; i < (int64_t) p.m * p.H; i += (int64_t) C * 128)
                     store_out(p.out, p.out_dtype, i, 0.f);
