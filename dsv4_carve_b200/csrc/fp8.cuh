@@ -344,12 +344,17 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(addr) : "memory");
 }
 
-// fp32 at shared-memory address `addr` (of this CTA's layout) in CTA `rank` of the cluster.
+// fp32 / four fp32 at shared-memory address `addr` (of this CTA's layout) in CTA `rank` of the cluster.
 __device__ __forceinline__ float ld_dsmem(uint32_t addr, uint32_t rank) {
-    uint32_t a;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_u32(addr, rank)) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float4 ld_dsmem4(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_u32(addr, rank)) : "memory");
     return v;
 }
 

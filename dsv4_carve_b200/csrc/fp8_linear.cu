@@ -8,7 +8,7 @@
 // columns are one accumulation in TMEM that is read back, scaled and added to
 // fp32 registers while the next group's runs into another TMEM buffer.
 //
-// Few rows (fp8_stream_kernel): bound by the weights' bytes.  The weights are
+// Few rows (fp8_stream_kernel, fp8_rows_kernel): bound by the weights' bytes.  The weights are
 // the M operand -- a 128-row tile of W is exactly one row of scale blocks, and
 // it goes from HBM through TMA into swizzled shared memory and from there to
 // the tensor core without touching a register -- and the rows of x are N.
@@ -40,12 +40,11 @@ constexpr int kFsProducerWarp = 8;
 constexpr int kFsMmaWarp = 9;
 constexpr int kFsThreads = 320;
 constexpr int kFsMaxStages = 12;
-constexpr int kFsMaxBufs = 8;
 constexpr int kFsMaxCluster = 8;
 
 struct FsParams {
     CUtensorMap wmap;            // W [n][k] bytes, box [128 k, 128 n], 128-byte swizzle
-    CUtensorMap xmap;            // PRE: e4m3 x [rows][k], box [128 k, NT]
+    CUtensorMap xmap;            // e4m3 x [rows][k], box [128 k, NT] (fp8_rows_kernel)
     const void* x;
     int64_t ldx;
     const float* xs;             // scales of an e4m3 x: xs[row * xsr + group * xsg], else null
@@ -60,32 +59,62 @@ struct FsParams {
     int early;                   // nothing still running can write the weights
 };
 
-template <int NT>
+// Sums of a cluster's partial tiles part[rows][128], in rank order; this CTA's
+// share of the outputs goes to `put`, four columns a thread or, where that would
+// leave most threads idle, one.
+template <bool WIDE, typename Put>
+__device__ __forceinline__ void cluster_reduce(const float* part, int rows, int S, int rank, int tid, int threads, Put&& put) {
+    cluster_sync_all();
+    constexpr int V = WIDE ? 4 : 1;
+    const int total = rows * 128 / V, per = (total + S - 1) / S;
+    for (int i = rank * per + tid; i < min(total, (rank + 1) * per); i += threads) {
+        const uint32_t at = smem_u32(part + V * i);
+        if constexpr (WIDE) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f), w[kFsMaxCluster];
+#pragma unroll
+            for (int c = 0; c < kFsMaxCluster; ++c) w[c] = c < S ? ld_dsmem4(at, (uint32_t) c) : v;
+#pragma unroll
+            for (int c = 0; c < kFsMaxCluster; ++c) { v.x += w[c].x; v.y += w[c].y; v.z += w[c].z; v.w += w[c].w; }
+            put(i >> 5, (i & 31) * 4, v.x);
+            put(i >> 5, (i & 31) * 4 + 1, v.y);
+            put(i >> 5, (i & 31) * 4 + 2, v.z);
+            put(i >> 5, (i & 31) * 4 + 3, v.w);
+        } else {
+            float v = 0.f;
+            for (int c = 0; c < S; ++c) v += ld_dsmem(at, (uint32_t) c);
+            put(i >> 7, i & 127, v);
+        }
+    }
+    cluster_sync_all();                                    // no CTA leaves while its sums are being read
+}
+
+// ------------------------------------------------------------------ up to 8 rows
+// x is quantised inside the kernel: warps 4-7 write it into the ring beside the
+// weights.  One launch, 6.4 us for one row x 4096 x 4096 back to back (2.6 TB/s);
+// what it takes is the chain of one launch (x from L2, quantising, MMA, the
+// cluster's sum), not the weights' time.
 struct FsLayout {
-    static constexpr int kXBytes = NT * 128;
-    static constexpr int kStage = (int) kFp8WTile + kXBytes;
-    static constexpr int kBufs = NT <= 16 ? 8 : NT <= 32 ? 4 : 2;
-    static constexpr int kTmemCols = NT * kBufs;           // 128
+    static constexpr int NT = 16;                          // MMA N
+    static constexpr int kStage = (int) kFp8WTile + NT * 128;
+    static constexpr int kBufs = 8;
+    static constexpr int kTmemCols = NT * kBufs;
 };
 
-template <int NT>
 struct FsHead {
     uint64_t full[kFsMaxStages];
     uint64_t empty[kFsMaxStages];
-    uint64_t tfull[kFsMaxBufs];
-    uint64_t tempty[kFsMaxBufs];
+    uint64_t tfull[FsLayout::kBufs];
+    uint64_t tempty[FsLayout::kBufs];
     uint32_t tmem;
-    uint32_t pad[3];
-    float fac[kFsMaxStages][NT];          // s_x * s_w of the stage's rows
+    alignas(16) float fac[kFsMaxStages][FsLayout::NT];     // s_x * s_w of the stage's rows
 };
 
-// PRE: x comes as e4m3 through TMA; otherwise warps 4-7 quantise it into the ring.
-template <int NT, bool PRE>
-__global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kernel(const __grid_constant__ FsParams p) {
-    using L = FsLayout<NT>;
+__global__ void __launch_bounds__(kFsThreads, 2) fp8_stream_kernel(const __grid_constant__ FsParams p) {
+    using L = FsLayout;
+    constexpr int NT = L::NT;
     extern __shared__ uint8_t fs_raw[];
     uint8_t* ring = fs_raw + ((1024u - (smem_u32(fs_raw) & 1023u)) & 1023u);
-    FsHead<NT>& H = *reinterpret_cast<FsHead<NT>*>(ring + p.stages * L::kStage);
+    FsHead& H = *reinterpret_cast<FsHead*>(ring + p.stages * L::kStage);
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const int S = p.cluster, rank = S > 1 ? (int) cluster_rank() : 0;
     const int tile = (int) blockIdx.x / S;
@@ -97,7 +126,7 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(&H.full[s], PRE ? 2 : 1 + (rows + 3) / 4);
+            mbar_init(&H.full[s], 1 + (rows + 3) / 4);
             mbar_init(&H.empty[s], 1 + kFsEpiWarps);
         }
         for (int b = 0; b < L::kBufs; ++b) { mbar_init(&H.tfull[b], 1); mbar_init(&H.tempty[b], kFsEpiWarps); }
@@ -117,31 +146,19 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
         const int ahead = min(nsteps, p.stages);
         auto weights = [&](int s) {
             const int st = s % p.stages;
-            mbar_arrive_expect_tx(&H.full[st], kFp8WTile + (PRE ? L::kXBytes : 0));
+            mbar_arrive_expect_tx(&H.full[st], kFp8WTile);
             tma_load_2d(ring + st * L::kStage, &p.wmap, (kbeg + s) * 128, n0, &H.full[st]);
         };
-        auto inputs = [&](int s) {
-            const int st = s % p.stages;
-            tma_load_2d(ring + st * L::kStage + kFp8WTile, &p.xmap, (kbeg + s) * 128, row0, &H.full[st]);
-        };
-        // Ahead of the wait for the previous kernel: the weights themselves
-        // when it is the quantiser of this call, which began after everything
-        // before it; otherwise it may write them, and only a prefetch into L2,
-        // which brings no value into this SM, is ahead.
-        if (p.early) {
-            if (lane == 0) for (int s = 0; s < ahead; ++s) weights(s);
-        } else if (lane < ahead) {
-            tma_prefetch_2d(&p.wmap, (kbeg + lane) * 128, n0);
-        }
+        // Ahead of the wait for the previous kernel, which may write the weights:
+        // a prefetch into L2, which brings no value into this SM.
+        if (lane < ahead) tma_prefetch_2d(&p.wmap, (kbeg + lane) * 128, n0);
         pdl_wait();
         if (lane == 0) {
             pdl_launch_dependents();
-            if (PRE) fence_proxy_async_global();
             int issued = 0;
             for (int s = 0; s < nsteps; ++s) {
                 if (s >= p.stages && !mbar_wait(&H.empty[s % p.stages], ((s / p.stages) + 1u) & 1u, status)) break;
-                if (s >= ahead || !p.early) weights(s);
-                if (PRE) inputs(s);
+                weights(s);
                 ++issued;
             }
             // no copy may still be in flight when the CTA retires
@@ -163,25 +180,6 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
                 tc_commit(&H.empty[st]);
                 tc_commit(&H.tfull[b]);
             }
-        }
-    } else if (warp >= kFsEpiWarps && PRE) {
-        // the factors of a step's rows, one warp a step
-        pdl_wait();
-        for (int s = warp - kFsEpiWarps; s < nsteps; s += kFsXWarps) {
-            const int st = s % p.stages;
-            const float ws = __ldg(p.ws + (int64_t) tile * p.groups + kbeg + s);
-            float f[(NT + 31) / 32];
-#pragma unroll
-            for (int h = 0; h < (NT + 31) / 32; ++h) {
-                const int j = h * 32 + lane;
-                f[h] = j < rows ? __ldcg(p.xs + (row0 + j) * p.xsr + (kbeg + s) * p.xsg) * ws : 0.f;
-            }
-            if (!mbar_wait_lanes(&H.empty[st], ((s / p.stages) + 1u) & 1u, status)) break;
-#pragma unroll
-            for (int h = 0; h < (NT + 31) / 32; ++h)
-                if (h * 32 + lane < NT) H.fac[st][h * 32 + lane] = f[h];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&H.full[st]);
         }
     } else if (warp >= kFsEpiWarps) {
         // x: one warp for each step and four rows.  Rows of the B operand behind
@@ -266,16 +264,213 @@ __global__ void __launch_bounds__(kFsThreads, NT <= 32 ? 2 : 1) fp8_stream_kerne
             for (int j = 0; j < NT; ++j)
                 if (j < rows) part[j * 128 + tid] = acc[j];
         }
-        cluster_sync_all();
-        const int total = rows * 128, per = (total + S - 1) / S;
-        for (int i = rank * per + tid; i < min(total, (rank + 1) * per); i += kFsThreads) {
-            float v = 0.f;
-            for (int c = 0; c < S; ++c) v += ld_dsmem(smem_u32(part + i), (uint32_t) c);
-            put(i >> 7, i & 127, v);
-        }
-        cluster_sync_all();                                // no CTA leaves while its sums are being read
+        cluster_reduce<false>(part, rows, S, rank, tid, kFsThreads, put);
     }
     if (warp == kFsMmaWarp) {
+        tc_fence_after();
+        tmem_free(tmem, L::kTmemCols);
+    }
+}
+
+// ------------------------------------------------------------------ up to some hundred rows
+// x comes in e4m3 through TMA beside the weights.  Eight epilogue warps (four for
+// 16 rows) share the columns, i.e. the rows of x; each keeps its columns' factors
+// in shared memory of its own, loaded two steps ahead.
+constexpr int kFrProducerWarp = 8;
+constexpr int kFrMmaWarp = 9;
+constexpr int kFrThreads = 320;
+
+template <int NT>
+struct FrLayout {
+    static constexpr int kHalves = NT >= 32 ? 2 : 1;
+    static constexpr int kCols = NT / kHalves;             // columns of an epilogue warp: 16, 16, 32, 64
+    static constexpr int kStage = (int) kFp8WTile + NT * 128;
+    static constexpr int kBufs = NT <= 32 ? 4 : 2;
+    static constexpr int kTmemCols = NT * kBufs;           // 64 .. 256
+    static constexpr int kCtas = NT <= 64 ? 2 : 1;         // that share an SM
+};
+
+template <int NT>
+struct FrHead {
+    uint64_t full[kFsMaxStages];
+    uint64_t done[kFsMaxStages];                           // the stage's MMAs: it may be refilled, and its sums be read
+    uint64_t tempty[4];
+    uint32_t tmem;
+    alignas(16) float fac[8][2][FrLayout<NT>::kCols];
+};
+
+template <int NT>
+__global__ void __launch_bounds__(kFrThreads, FrLayout<NT>::kCtas) fp8_rows_kernel(const __grid_constant__ FsParams p) {
+    using L = FrLayout<NT>;
+    extern __shared__ uint8_t fr_raw[];
+    uint8_t* ring = fr_raw + ((1024u - (smem_u32(fr_raw) & 1023u)) & 1023u);
+    FrHead<NT>& H = *reinterpret_cast<FrHead<NT>*>(ring + p.stages * L::kStage);
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
+    const int S = p.cluster, rank = S > 1 ? (int) cluster_rank() : 0;
+    const int tile = (int) blockIdx.x / S;
+    const int n0 = tile * 128, row0 = (int) blockIdx.y * NT;
+    const int rows = min(NT, p.rows - row0);
+    const int ncols = (rows + 15) & ~15;                   // MMA N
+    const int kbeg = rank * p.groups / S, nsteps = (rank + 1) * p.groups / S - kbeg;
+    uint32_t* status = &g_fp8_status;
+
+    if (tid == 0) {
+        for (int s = 0; s < p.stages; ++s) { mbar_init(&H.full[s], 1); mbar_init(&H.done[s], 1); }
+        for (int b = 0; b < L::kBufs; ++b) mbar_init(&H.tempty[b], 4 * L::kHalves);
+        fence_barrier_init();
+    }
+    if (warp == kFrMmaWarp) tmem_alloc(&H.tmem, L::kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, H.tmem, 0);
+    const int half = warp >> 2, lg = warp & 3, j0 = half * L::kCols;   // epilogue warps
+    float acc[L::kCols];
+#pragma unroll
+    for (int j = 0; j < L::kCols; ++j) acc[j] = 0.f;
+
+    if (warp == kFrProducerWarp) {
+        const int ahead = min(nsteps, p.stages);
+        auto weights = [&](int s) {
+            const int st = s % p.stages;
+            mbar_arrive_expect_tx(&H.full[st], L::kStage);
+            tma_load_2d(ring + st * L::kStage, &p.wmap, (kbeg + s) * 128, n0, &H.full[st]);
+        };
+        // Ahead of the wait for the previous kernel: the weights themselves when it
+        // is the quantiser of this call, which began after everything before it;
+        // otherwise it may write them, and a prefetch into L2 has to do.
+        if (p.early) {
+            if (lane == 0) for (int s = 0; s < ahead; ++s) weights(s);
+        } else if (lane < ahead) {
+            tma_prefetch_2d(&p.wmap, (kbeg + lane) * 128, n0);
+        }
+        pdl_wait();
+        if (lane == 0) {
+            pdl_launch_dependents();
+            fence_proxy_async_global();
+            int issued = 0;
+            for (int s = 0; s < nsteps; ++s) {
+                const int st = s % p.stages;
+                if (s >= p.stages && !mbar_wait(&H.done[st], ((s / p.stages) + 1u) & 1u, status)) break;
+                if (s >= ahead || !p.early) weights(s);
+                tma_load_2d(ring + st * L::kStage + kFp8WTile, &p.xmap, (kbeg + s) * 128, row0, &H.full[st]);
+                ++issued;
+            }
+            // no copy may still be in flight when the CTA retires
+            for (int i = max(0, issued - p.stages); i < issued; ++i)
+                if (!mbar_wait(&H.full[i % p.stages], (i / p.stages) & 1u, status)) break;
+        }
+    } else if (warp == kFrMmaWarp) {
+        pdl_wait();
+        const uint32_t id = idesc_f16(128, ncols);
+        const uint64_t desc0 = sdesc_sw128(smem_u32(ring));
+        for (int s = 0; s < nsteps; ++s) {
+            const int st = s % p.stages, b = s % L::kBufs;
+            if (!mbar_poll2_lanes(&H.full[st], (s / p.stages) & 1u, &H.tempty[b], ((s / L::kBufs) + 1u) & 1u, status)) break;
+            tc_fence_after();
+            const uint64_t wd = desc0 + (uint64_t) (st * (L::kStage >> 4)), xd = wd + (kFp8WTile >> 4);
+            if (elect_lane()) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) tc_mma_f8(tmem + b * NT, wd + 2 * q, xd + 2 * q, id, q);
+                tc_commit(&H.done[st]);
+            }
+        }
+    } else if (half < L::kHalves) {
+        // scale and add: thread = weight row, registers = rows of x
+        pdl_wait();
+        constexpr int NF = (L::kCols + 31) / 32;
+        struct Fac { float f[NF], w; };
+        auto load = [&](int s) {
+            Fac v;
+            v.w = s < nsteps ? __ldg(p.ws + (int64_t) tile * p.groups + kbeg + s) : 0.f;
+#pragma unroll
+            for (int h = 0; h < NF; ++h) {
+                const int j = h * 32 + lane;
+                v.f[h] = s < nsteps && j < L::kCols && j0 + j < rows ? __ldcg(p.xs + (row0 + j0 + j) * p.xsr + (kbeg + s) * p.xsg) : 0.f;
+            }
+            return v;
+        };
+        Fac v0 = load(0), v1 = load(1);
+        const uint32_t tcol = tmem + ((uint32_t) (lg * 32) << 16) + (uint32_t) j0;
+        for (int s = 0; s < nsteps; ++s) {
+            const int st = s % p.stages, b = s % L::kBufs;
+            float* fac = H.fac[warp][s & 1];               // the other one may still be read by slower lanes
+#pragma unroll
+            for (int h = 0; h < NF; ++h)
+                if (h * 32 + lane < L::kCols) fac[h * 32 + lane] = v0.f[h] * v0.w;
+            v0 = v1;
+            v1 = load(s + 2);
+            __syncwarp();
+            if (!mbar_wait_lanes(&H.done[st], (s / p.stages) & 1u, status)) break;
+            tc_fence_after();
+            const float4* f4 = reinterpret_cast<const float4*>(fac);
+            if constexpr (L::kCols == 16) {
+                if (j0 < ncols) {
+                    float v[16];
+                    tc_ld16(tcol + (uint32_t) (b * NT), v);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 f = f4[q];
+                        acc[4 * q] = fmaf(v[4 * q], f.x, acc[4 * q]);
+                        acc[4 * q + 1] = fmaf(v[4 * q + 1], f.y, acc[4 * q + 1]);
+                        acc[4 * q + 2] = fmaf(v[4 * q + 2], f.z, acc[4 * q + 2]);
+                        acc[4 * q + 3] = fmaf(v[4 * q + 3], f.w, acc[4 * q + 3]);
+                    }
+                }
+            } else {
+                constexpr int NC = L::kCols / 32;
+                if (j0 < ncols) {
+                    uint32_t v[NC][32];
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) tc_ld32_issue(tcol + (uint32_t) (b * NT + c * 32), v[c]);
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        tc_ld32_wait(v[c]);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            const float4 f = f4[c * 8 + q];
+                            float* o = &acc[c * 32 + 4 * q];
+                            o[0] = fmaf(__uint_as_float(v[c][4 * q]), f.x, o[0]);
+                            o[1] = fmaf(__uint_as_float(v[c][4 * q + 1]), f.y, o[1]);
+                            o[2] = fmaf(__uint_as_float(v[c][4 * q + 2]), f.z, o[2]);
+                            o[3] = fmaf(__uint_as_float(v[c][4 * q + 3]), f.w, o[3]);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&H.tempty[b]);
+        }
+    } else {
+        pdl_wait();
+    }
+
+    auto put = [&](int j, int i, float v) {
+        const int col = n0 + i;
+        if (col >= p.n) return;
+        if (p.bias != nullptr) v += load_f32(p.bias, p.bias_dtype, col);
+        store_out(p.y, p.y_dtype, (int64_t) (row0 + j) * p.ldy + col, v);
+    };
+    const bool epi = half < L::kHalves;
+    if (S == 1) {
+        if (epi) {
+#pragma unroll
+            for (int j = 0; j < L::kCols; ++j)
+                if (j0 + j < rows) put(j0 + j, lg * 32 + lane, acc[j]);
+        }
+        __syncthreads();
+    } else {
+        __syncthreads();                                   // every stage has been read: the ring is free
+        float* part = reinterpret_cast<float*>(ring);       // [rows][128]
+        if (epi) {
+#pragma unroll
+            for (int j = 0; j < L::kCols; ++j)
+                if (j0 + j < rows) part[(j0 + j) * 128 + lg * 32 + lane] = acc[j];
+        }
+        cluster_reduce<true>(part, rows, S, rank, tid, kFrThreads, put);
+    }
+    if (warp == kFrMmaWarp) {
         tc_fence_after();
         tmem_free(tmem, L::kTmemCols);
     }
@@ -627,34 +822,28 @@ int fs_cluster(int64_t tiles, int groups, int resident) {
     return s;
 }
 
-template <int NT, bool PRE>
-int fs_launch(FsParams& p, cudaStream_t stream) {
-    using L = FsLayout<NT>;
-    const int64_t tiles = ((int64_t) p.n + 127) / 128, rtiles = ((int64_t) p.rows + NT - 1) / NT;
-    p.cluster = fs_cluster(tiles * rtiles, p.groups, NT <= 32 ? 296 : 148);
-    const int steps = (p.groups + p.cluster - 1) / p.cluster;
-    // two CTAs share an SM up to 32 rows: at most about 112 KB each; at least the partial sums' room
-    constexpr int kBudget = (NT <= 32 ? 112 : 200) * 1024;
-    const int head = 1024 + (int) sizeof(FsHead<NT>);
-    int stages = (kBudget - head) / L::kStage;
+// Launches one of the kernels whose clusters split k: `nt` rows a tile, `stage`
+// bytes a stage, `head` bytes beside the ring, `ctas` that share an SM.
+int fs_launch(void (*kern)(FsParams), std::once_flag (&once)[64], FsParams& p, int nt, int stage, int head, int ctas, cudaStream_t stream) {
+    const int64_t tiles = ((int64_t) p.n + 127) / 128, rtiles = ((int64_t) p.rows + nt - 1) / nt;
+    p.cluster = fs_cluster(tiles * rtiles, p.groups, 148 * ctas);
+    const int steps = (p.groups + p.cluster - 1) / p.cluster, budget = (ctas == 2 ? 112 : 200) * 1024;
+    int stages = (budget - 1024 - head) / stage;
     if (stages > kFsMaxStages) stages = kFsMaxStages;
-    const int least = (NT * 512 + L::kStage - 1) / L::kStage;
+    const int least = (nt * 512 + stage - 1) / stage;      // the partial sums' room
     if (stages > steps) stages = steps < least ? least : steps;
+    if (stages < 4) stages = 4;                            // not fewer than TMEM buffers
     p.stages = stages;
-    const int smem = head + stages * L::kStage;
-    static std::once_flag once[64];
     int dev = 0;
     EXL3_CUDA(cudaGetDevice(&dev));
     cudaError_t attr = cudaSuccess;
-    std::call_once(once[dev & 63], [&] {
-        attr = cudaFuncSetAttribute(fp8_stream_kernel<NT, PRE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
-    });
+    std::call_once(once[dev & 63], [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); });
     EXL3_CUDA(attr);
     EXL3_REQUIRE(tiles * p.cluster <= INT32_MAX && rtiles <= 65535, EXL3_ERR_UNSUPPORTED, "exl3_fp8_linear: matrix too large");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned) (tiles * p.cluster), (unsigned) rtiles);
     cfg.blockDim = dim3(kFsThreads);
-    cfg.dynamicSmemBytes = (size_t) smem;
+    cfg.dynamicSmemBytes = (size_t) (1024 + head + stages * stage);
     cfg.stream = stream;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -665,8 +854,15 @@ int fs_launch(FsParams& p, cudaStream_t stream) {
     at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    EXL3_CUDA(cudaLaunchKernelEx(&cfg, fp8_stream_kernel<NT, PRE>, p));
+    EXL3_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
     return EXL3_OK;
+}
+
+template <int NT>
+int fr_launch(FsParams& p, cudaStream_t stream) {
+    static std::once_flag once[64];
+    static_assert(kFrThreads == kFsThreads, "one launch shape");
+    return fs_launch(fp8_rows_kernel<NT>, once, p, NT, FrLayout<NT>::kStage, (int) sizeof(FrHead<NT>), FrLayout<NT>::kCtas, stream);
 }
 
 template <int NW>
@@ -702,7 +898,7 @@ int fg_launch(FgParams& p, int sms, cudaStream_t stream) {
 // Rows up to which the weights are the M operand and k is split: below, the
 // 256-row tiles of the pair kernel are too few to fill the GPU.
 constexpr int kFsInlineRows = 8;     // x quantised inside the kernel (16 rows x 4096 x 4096: 11.6 us so, 9.6 by a launch before)
-constexpr int kFsMaxRows = 192;
+constexpr int kFsMaxRows = 128;
 
 int64_t fp8_ldq(int64_t k) { return (k + 15) / 16 * 16; }
 
@@ -738,7 +934,10 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
     p.rows = (int) rows; p.n = (int) n; p.k = (int) k; p.groups = groups;
     p.xvec = k % 16 == 0 && ldx * es % 16 == 0 && aligned16(x);
     if (rows <= kFsMaxRows && (rc = fp8_map(&p.wmap, w, n, k, ldw, 128, "exl3_fp8_linear")) != EXL3_OK) return rc;
-    if (rows <= kFsInlineRows) return fs_launch<16, false>(p, s);
+    if (rows <= kFsInlineRows) {
+        static std::once_flag once[64];
+        return fs_launch(fp8_stream_kernel, once, p, FsLayout::NT, FsLayout::kStage, (int) sizeof(FsHead), 2, s);
+    }
 
     // e4m3 rows that TMA can load: the caller's, or a copy / the quantised rows in the scratch
     const void* xq = x;
@@ -768,7 +967,7 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
         if ((rc = fp8_map(&p.xmap, xq, rows, k, ldq, nt, "exl3_fp8_linear")) != EXL3_OK) return rc;
         p.xs = xs; p.xsr = xsr; p.xsg = xsg;
         p.early = early;
-        return nt == 16 ? fs_launch<16, true>(p, s) : nt == 32 ? fs_launch<32, true>(p, s) : nt == 64 ? fs_launch<64, true>(p, s) : fs_launch<128, true>(p, s);
+        return nt == 16 ? fr_launch<16>(p, s) : nt == 32 ? fr_launch<32>(p, s) : nt == 64 ? fr_launch<64>(p, s) : fr_launch<128>(p, s);
     }
     int dev = 0;
     EXL3_CUDA(cudaGetDevice(&dev));
