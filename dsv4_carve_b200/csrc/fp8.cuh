@@ -32,25 +32,59 @@ __device__ __forceinline__ float fp8_scale(uint32_t amax_bits, bool pow2) {
 // x / s to within the e4m3 rounding that follows, i.e. RN_e4m3 of the result
 // is RN_e4m3 of the real quotient.  q = x * (1 / s) is off by at most two units
 // in its last place (two roundings of 2^-24), which moves the e4m3 rounding
-// only next to a midpoint of two e4m3 values.  There the sign of x - midpoint
-// * s, which one FMA has exactly, decides.  16-bit inputs meet midpoints often
-// (amax divides many of their multiples by 448), so this costs no division: a
-// slow path with one took 33 instructions a value in all, 2.5 times as long.
-//
-// Near a midpoint: 0x80000 +- 2 in the low 20 bits of a normal e4m3 value.
-// Values below 2^-6, where e4m3 steps stay 2^-9 wide, are moved up by 2^-6 into
-// the binade with that step first.
-__device__ __forceinline__ float fp8_quotient(float x, float s, float inv, bool pow2) {
-    const float q = x * inv;                       // exact for a power of two
-    if (pow2) return q;
-    const float a = fabsf(q), m = a < 0x1p-6f ? a + 0x1p-6f : a;
-    if (((__float_as_uint(m) + 0x80002u) & 0xFFFFFu) > 4u) return q;
-    // the midpoint has 5 significant bits at most: the nearest number whose low 19 bits are zero
-    const uint32_t mid = (__float_as_uint(q) + 0x40000u) & 0xFFF80000u;
-    const float up = s < 0x1p-60f ? 0x1p64f : 1.f; // keeps the remainder clear of the subnormal numbers
-    const float r = __fmaf_rn(-__uint_as_float(mid), s * up, x * up);
-    if (r == 0.f) return __uint_as_float(mid);     // a tie: to even, by the conversion
-    return __uint_as_float((r > 0.f) == (q > 0.f) ? mid + 1u : mid - 1u);
+// only next to a midpoint of two e4m3 values.  Those have at most 5 significant
+// bits, as the values themselves do, i.e. 19 low bits that are zero.  Where q is
+// within two units of such a number v, the remainder r = x - v * s, which one FMA
+// has exactly, says on which side of v the real quotient v + r / s lies; v + 64 r
+// / s keeps that side, does not round back to v (r is a multiple of 2^-27 of v *
+// s at least, so 64 r / s is a unit in the last place) and is still 2^-15 of v at
+// most, far from the next boundary.  A tie (r = 0) stays v, for the conversion to
+// round to even.  All of it is arithmetic without a branch: 16-bit inputs meet
+// midpoints often, because amax divides many of their multiples by 448, and a
+// branch for each value, predicated or voted, was slower (8192 x 4096: 28 us).
+__device__ __forceinline__ float fp8_quotient_fast(float x, float s, float inv) {
+    const float q = x * inv;
+    const uint32_t b = __float_as_uint(q);
+    const float v = __uint_as_float((b + 0x40000u) & 0xFFF80000u);
+    const float side = __fmaf_rn(__fmaf_rn(-v, s, x), 64.f * inv, v);
+    return ((b + 2u) & 0x7FFFFu) <= 4u ? side : q;
+}
+
+// The same for any scale: a remainder clear of the subnormal numbers for tiny
+// ones, and nothing multiplied by an infinite one.
+static __device__ __noinline__ void fp8_quotients_any(float* x, int n, float s, float inv) {
+    const float up = s < 0x1p-60f ? 0x1p64f : 1.f;
+    for (int i = 0; i < n; ++i) {
+        const float q = x[i] * inv;
+        const uint32_t b = __float_as_uint(q), v = (b + 0x40000u) & 0xFFF80000u;
+        float o = q;
+        if (((b + 2u) & 0x7FFFFu) <= 4u && s < INFINITY) {
+            const float r = __fmaf_rn(-__uint_as_float(v), s * up, x[i] * up);
+            o = __uint_as_float(r == 0.f || q == 0.f ? v : (r > 0.f) == (q > 0.f) ? v + 1u : v - 1u);
+        }
+        x[i] = o;
+    }
+}
+
+__device__ __forceinline__ bool fp8_easy(float s) { return s >= 0x1p-60f && s < 0x1p100f; }
+
+// N quotients by one scale, with one branch for all of them.
+template <int N>
+__device__ __forceinline__ void fp8_quotients(float (&v)[N], float s, float inv, bool pow2) {
+    if (pow2 || s == 0x1p-126f) {                  // exact; the latter: rows of zeros, and lanes without a row
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= inv;
+    } else if (fp8_easy(s)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = fp8_quotient_fast(v[i], s, inv);
+    } else {
+        float t[N];                                // its address keeps `v` itself in registers
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = v[i];
+        fp8_quotients_any(t, N, s, inv);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = t[i];
+    }
 }
 
 // Two fp32 -> two e4m3 bytes (nearest, ties to even, finite values saturate),
@@ -180,11 +214,15 @@ struct XRows {
         }
         s = fp8_scale(m, pow2);
         const float inv = __frcp_rn(s);
+        if (cnt == 1) {
+            float t[4] = {v[0], v[1], v[2], v[3]};
+            fp8_quotients(t, s, inv, pow2);
+            q[0] = e4m3x2(t[0], t[1]) | (e4m3x2(t[2], t[3]) << 16);
+            return make_uint4(q[0], 0u, 0u, 0u);
+        }
+        fp8_quotients(v, s, inv, pow2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (i > 0 && cnt == 1) break;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * i + j] = fp8_quotient(v[4 * i + j], s, inv, pow2);
             q[i] = e4m3x2(v[4 * i], v[4 * i + 1]) | (e4m3x2(v[4 * i + 2], v[4 * i + 3]) << 16);
         }
         return make_uint4(q[0], q[1], q[2], q[3]);

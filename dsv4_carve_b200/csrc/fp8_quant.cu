@@ -64,8 +64,7 @@ struct QuantVec {
         const float inv = __frcp_rn(s);
         float v[VEC];
         values(v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = fp8_quotient(v[i], s, inv, POW2);
+        fp8_quotients(v, s, inv, POW2);
         uint32_t o[VEC / 4];
 #pragma unroll
         for (int i = 0; i < VEC / 4; ++i)

@@ -42,7 +42,8 @@ def test_quantize_midpoints_and_borders(cuda, pow2):
     mids = torch.tensor([(m + 0.5) / 8 * 2.0 ** -6 for m in range(8)] +
                         [(1 + (m + 0.5) / 8) * 2.0 ** e for e in range(-6, 9) for m in range(8)][:-2], dtype=torch.float64)
     rows = []
-    for amax in (448.0, 448.0 * 0.7, 448.0 * 1.0000001, 447.99997, 448.00003, 1.0, 3.0, 1e-30, 2e30):
+    for amax in (448.0, 448.0 * 0.7, 448.0 * 1.0000001, 447.99997, 448.00003, 1.0, 3.0, 1e-30, 2e30, 7e-36, 1e-37, 3.3e38,
+                 1.3e-15, 2.7e33):
         s = float(R.scale_of(torch.tensor([amax], dtype=torch.float64).float().double(), pow2))
         v = (mids * s).float()
         v = torch.cat([v, torch.nextafter(v, torch.zeros_like(v)), torch.nextafter(v, torch.full_like(v, 1e38)), -v])
