@@ -95,6 +95,14 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
+// Four values by one scale -> e4m3 bytes; one copy of the code, for places that
+// run it a few times only.
+static __device__ __noinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float s, bool pow2) {
+    float v[4] = {a, b, c, d};
+    fp8_quotients(v, s, __frcp_rn(s), pow2);
+    return e4m3x2(v[0], v[1]) | (e4m3x2(v[2], v[3]) << 16);
+}
+
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // ---------------------------------------------------------------- loads

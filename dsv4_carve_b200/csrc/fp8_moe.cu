@@ -315,10 +315,9 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
                     float v[4] = {fm_swiglu(g4.x, u4.x, p.limit), fm_swiglu(g4.y, u4.y, p.limit),
                                   fm_swiglu(g4.z, u4.z, p.limit), fm_swiglu(g4.w, u4.w, p.limit)};
                     const uint32_t mx = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
-                    const float sa = fp8_scale(__reduce_max_sync(0xffffffffu, mx), p.pow2), inv = __frcp_rn(sa);
-                    fp8_quotients(v, sa, inv, p.pow2 != 0);
+                    const float sa = fp8_scale(__reduce_max_sync(0xffffffffu, mx), p.pow2);
                     *reinterpret_cast<uint32_t*>(p.aq + (int64_t) (pr + h) * p.I + ib * 128 + lane * 4) =
-                        e4m3x2(v[0], v[1]) | (e4m3x2(v[2], v[3]) << 16);
+                        fp8_pack4(v[0], v[1], v[2], v[3], sa, p.pow2 != 0);
                     if (lane == 0) p.as[(int64_t) (pr + h) * NBI + ib] = sa;
                 }
             }
@@ -584,9 +583,7 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
                         for (int j = c * kCh; j < (c + 1) * kCh; ++j) {
                             const uint32_t mx = max(max(S.wmax[0][j], S.wmax[1][j]), max(S.wmax[2][j], S.wmax[3][j]));
                             const float sa = fp8_scale(mx, p.pow2);
-                            float v[1] = {acc[0][j]};
-                            fp8_quotients(v, sa, __frcp_rn(sa), p.pow2 != 0);
-                            const uint32_t q = e4m3x2(v[0], 0.f);
+                            const uint32_t q = fp8_pack4(acc[0][j], 0.f, 0.f, 0.f, sa, p.pow2 != 0);
                             if (have >> j & 1ull) {
                                 // an expert listed twice for a token has two pairs next to each other
                                 int pr = S.tokpair[j];
