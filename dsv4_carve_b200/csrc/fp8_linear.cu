@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kFrThreads, FrLayout<NT>::kCtas) fp8_rows_kern
             tma_load_2d(ring + st * L::kStage, &p.wmap, (kbeg + s) * 128, n0, &H.full[st]);
         };
         // Ahead of the wait for the previous kernel: the weights themselves when it
-        // is the quantiser of this call, which began after everything before it;
+        // is the quantiser of this call, behind whose own wait this kernel started;
         // otherwise it may write them, and a prefetch into L2 has to do.
         if (p.early) {
             if (lane == 0) for (int s = 0; s < ahead; ++s) weights(s);
@@ -562,7 +562,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
                                      nt * NW + (int) rank * (NW / 2), mapa_u32(smem_u32(&H.full[st]), 0));
             };
             if (p.early) {
-                // weights ahead of the quantiser's end (it began after everything before this call)
+                // weights ahead of the quantiser's end: this kernel started behind its wait for all before
                 const int nt = pair % p.ntiles;
                 for (; ahead < min(L::kStages, steps); ++ahead) weights(ahead, nt, ahead);
             }

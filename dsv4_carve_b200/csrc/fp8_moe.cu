@@ -272,9 +272,9 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
     if (warp == kFmMmaWarp) tmem_alloc(&S.tmem, L::kTmemCols);
     if (PH == 0) {
         // Kernel 2 may start once what came before the layer (the routes among
-        // it) is complete: at once where the quantiser, an ordinary launch, ran in
-        // between -- only x is waited for then, by those who read it -- otherwise
-        // behind this kernel's own wait.
+        // it) is complete: at once where the quantiser, which waits for that before it
+        // lets this kernel start, ran in between -- only x is waited for then, by
+        // those who read it -- otherwise behind this kernel's own wait.
         if (!p.early) pdl_wait();
         pdl_launch_dependents();
     }

@@ -96,6 +96,8 @@ struct QuantArgs {
 template <int DT, bool POW2, bool FAST, int RP>
 __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(const __grid_constant__ QuantArgs p) {
     using V = QuantVec<DT, FAST>;
+    // Whoever starts early behind this kernel finds all that came before it complete.
+    pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const uint32_t item = blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
@@ -126,6 +128,7 @@ __global__ void __launch_bounds__(512) fp8_quant_blocks_kernel(const __grid_cons
     constexpr int RP = 512 / V::LANES;                     // rows in a pass
     constexpr int N = kFp8Block / RP;                      // passes
     __shared__ uint32_t wmax[16];
+    pdl_wait();
     const int tid = threadIdx.x;
     const int64_t row0 = (int64_t) blockIdx.y * kFp8Block + tid / V::LANES;
     const int col = blockIdx.x * kFp8Block + (tid % V::LANES) * V::VEC, left = p.cols - col;
@@ -146,6 +149,21 @@ __global__ void __launch_bounds__(512) fp8_quant_blocks_kernel(const __grid_cons
     if (tid == 0) p.scale[(int64_t) blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 
+// Programmatic launch: the grid is set up while the previous kernel ends.
+int quant_pdl(void (*kern)(QuantArgs), dim3 grid, int threads, const QuantArgs& a, cudaStream_t s) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned) threads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    EXL3_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+    return EXL3_OK;
+}
+
 template <int DT, bool POW2, bool FAST>
 int quant_launch(QuantArgs& a, int block_rows, cudaStream_t s) {
     if (block_rows == 1) {
@@ -155,15 +173,12 @@ int quant_launch(QuantArgs& a, int block_rows, cudaStream_t s) {
         const int rp = a.rows * a.spans < 4 * 2 * 148 * kQuantWarps ? 1 : 4;
         const int64_t items = (a.rows + rp - 1) / rp * a.spans, grid = (items + kQuantWarps - 1) / kQuantWarps;
         EXL3_REQUIRE(items <= INT32_MAX, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: too many elements for one launch");
-        if (rp == 1) fp8_quant_rows_kernel<DT, POW2, FAST, 1><<<(unsigned) grid, kQuantWarps * 32, 0, s>>>(a);
-        else fp8_quant_rows_kernel<DT, POW2, FAST, 4><<<(unsigned) grid, kQuantWarps * 32, 0, s>>>(a);
-    } else {
-        const int64_t rb = (a.rows + kFp8Block - 1) / kFp8Block;
-        EXL3_REQUIRE(rb <= 65535, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: more than 65535 blocks of 128 rows");
-        fp8_quant_blocks_kernel<DT, POW2, FAST><<<dim3((unsigned) a.groups, (unsigned) rb), 512, 0, s>>>(a);
+        return quant_pdl(rp == 1 ? fp8_quant_rows_kernel<DT, POW2, FAST, 1> : fp8_quant_rows_kernel<DT, POW2, FAST, 4>,
+                         dim3((unsigned) grid), kQuantWarps * 32, a, s);
     }
-    EXL3_CUDA(cudaGetLastError());
-    return EXL3_OK;
+    const int64_t rb = (a.rows + kFp8Block - 1) / kFp8Block;
+    EXL3_REQUIRE(rb <= 65535, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: more than 65535 blocks of 128 rows");
+    return quant_pdl(fp8_quant_blocks_kernel<DT, POW2, FAST>, dim3((unsigned) a.groups, (unsigned) rb), 512, a, s);
 }
 
 template <int DT>
