@@ -10,52 +10,61 @@
 
 namespace exl3 {
 
-// A lane holds VEC = 16 bytes / es elements of one row; 128 / VEC lanes hold a
-// group.  FAST: rows start and end on VEC-element boundaries, so whole vectors
-// are inside or outside; otherwise elements are moved one by one.
+// A lane holds VEC = 32 bytes / es elements of one row; 128 / VEC lanes hold a
+// group.  (With 16 bytes a lane the scale, its reciprocal and the addresses cost
+// as much as the values: 15 instructions a value with power-of-two scales.)
+// FAST: rows start and end on VEC-element boundaries, so whole vectors are
+// inside or outside; otherwise elements are moved one by one.
 template <int DT, bool FAST>
 struct QuantVec {
-    static constexpr int VEC = DT == 2 ? 4 : 8;
-    static constexpr int LANES = kFp8Block / VEC;          // 32 (fp32) or 16
-    uint32_t w[4];
+    static constexpr int VEC = DT == 2 ? 8 : 16;
+    static constexpr int LANES = kFp8Block / VEC;          // 16 (fp32) or 8
+    uint32_t w[8];
     __device__ __forceinline__ void load(const void* x, int64_t at, int left) {
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (left > 0) {
-            if (FAST) {
-                raw = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + at * (DT == 2 ? 4 : 2)));
-            } else if (DT == 2) {
-                raw = load_raw4_tail(x, DT, at, left);
-            } else {
-                const uint4 a = load_raw4_tail(x, DT, at, left), b = load_raw4_tail(x, DT, at + 4, left - 4);
-                raw = make_uint4(a.x, a.y, b.x, b.y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 0u;
+        if (left <= 0) return;
+        if (FAST) {
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + at * (DT == 2 ? 4 : 2));
+            const uint4 a = __ldcs(src), b = __ldcs(src + 1);
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+            w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+        } else {
+            constexpr int PER = DT == 2 ? 4 : 2;           // words of four elements
+#pragma unroll
+            for (int i = 0; i < VEC / 4; ++i) {
+                const uint4 t = load_raw4_tail(x, DT, at + 4 * i, left - 4 * i);
+                w[PER * i] = t.x;
+                w[PER * i + 1] = t.y;
+                if constexpr (DT == 2) {
+                    w[PER * i + 2] = t.z;
+                    w[PER * i + 3] = t.w;
+                }
             }
         }
-        w[0] = raw.x; w[1] = raw.y; w[2] = raw.z; w[3] = raw.w;
     }
     // Bits of the largest magnitude as fp32, NaN kept; 16-bit types two at a time.
     __device__ __forceinline__ uint32_t amax() const {
-        if (DT == 2) return max(max(w[0] & 0x7FFFFFFFu, w[1] & 0x7FFFFFFFu), max(w[2] & 0x7FFFFFFFu, w[3] & 0x7FFFFFFFu));
-        uint32_t a[4];
+        if constexpr (DT == 2) {
+            uint32_t m = 0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = w[i] & 0x7FFF7FFFu;
-        if (DT == 1) {
-            auto h = [&](int i) { return *reinterpret_cast<const __nv_bfloat162*>(&a[i]); };
-            const float2 f = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h(0), h(1)), __hmax2_nan(h(2), h(3))));
+            for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+            return m;
+        } else {
+            uint32_t a[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = w[i] & 0x7FFF7FFFu;
+            float2 f;
+            if constexpr (DT == 1) {
+                auto h = [&](int i) { return *reinterpret_cast<const __nv_bfloat162*>(&a[i]); };
+                auto m = [&](int i) { return __hmax2_nan(h(i), h(i + 1)); };
+                f = __bfloat1622float2(__hmax2_nan(__hmax2_nan(m(0), m(2)), __hmax2_nan(m(4), m(6))));
+            } else {
+                auto h = [&](int i) { return *reinterpret_cast<const __half2*>(&a[i]); };
+                auto m = [&](int i) { return __hmax2_nan(h(i), h(i + 1)); };
+                f = __half22float2(__hmax2_nan(__hmax2_nan(m(0), m(2)), __hmax2_nan(m(4), m(6))));
+            }
             return max(abs_bits(f.x), abs_bits(f.y));
-        }
-        auto h = [&](int i) { return *reinterpret_cast<const __half2*>(&a[i]); };
-        const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(h(0), h(1)), __hmax2_nan(h(2), h(3))));
-        return max(abs_bits(f.x), abs_bits(f.y));
-    }
-    __device__ __forceinline__ void values(float (&v)[VEC]) const {
-        float t[4];
-        unpack4(make_uint4(w[0], w[1], w[2], w[3]), DT, t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = t[i];
-        if constexpr (DT != 2) {
-            unpack4(make_uint4(w[2], w[3], 0u, 0u), DT, t);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 + i] = t[i];
         }
     }
     template <bool POW2>
@@ -63,15 +72,22 @@ struct QuantVec {
         if (left <= 0) return;
         const float inv = __frcp_rn(s);
         float v[VEC];
-        values(v);
+#pragma unroll
+        for (int i = 0; i < VEC / 4; ++i) {
+            float t[4];
+            if constexpr (DT == 2) unpack4(make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]), DT, t);
+            else unpack4(make_uint4(w[2 * i], w[2 * i + 1], 0u, 0u), DT, t);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * i + j] = t[j];
+        }
         fp8_quotients(v, s, inv, POW2);
         uint32_t o[VEC / 4];
 #pragma unroll
         for (int i = 0; i < VEC / 4; ++i)
             o[i] = e4m3x2(v[4 * i], v[4 * i + 1]) | (e4m3x2(v[4 * i + 2], v[4 * i + 3]) << 16);
         if (FAST) {
-            if constexpr (DT == 2) *reinterpret_cast<uint32_t*>(q + at) = o[0];
-            else *reinterpret_cast<uint2*>(q + at) = make_uint2(o[0], o[1]);
+            if constexpr (DT == 2) *reinterpret_cast<uint2*>(q + at) = make_uint2(o[0], o[1]);
+            else *reinterpret_cast<uint4*>(q + at) = make_uint4(o[0], o[1], o[2], o[3]);
         } else {
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
@@ -91,7 +107,7 @@ struct QuantArgs {
 };
 
 // One scale for each row and group of 128 columns.  A warp takes one span of a
-// row -- one group (fp32) or two neighbours (16-bit) -- in RP consecutive
+// row -- two neighbouring groups (fp32) or four (16-bit) -- in RP consecutive
 // rows, all loads first.
 template <int DT, bool POW2, bool FAST, int RP>
 __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(const __grid_constant__ QuantArgs p) {
@@ -120,8 +136,8 @@ __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(const 
     }
 }
 
-// One scale for each 128 x 128 block, held in registers: 512 threads of four
-// 16-byte pieces (16-bit types) or eight (fp32).
+// One scale for each 128 x 128 block, held in registers: 512 threads of two
+// 32-byte pieces (16-bit types) or four (fp32).
 template <int DT, bool POW2, bool FAST>
 __global__ void __launch_bounds__(512) fp8_quant_blocks_kernel(const __grid_constant__ QuantArgs p) {
     using V = QuantVec<DT, FAST>;
@@ -167,9 +183,9 @@ int quant_pdl(void (*kern)(QuantArgs), dim3 grid, int threads, const QuantArgs& 
 template <int DT, bool POW2, bool FAST>
 int quant_launch(QuantArgs& a, int block_rows, cudaStream_t s) {
     if (block_rows == 1) {
-        a.spans = DT == 2 ? a.groups : (a.groups + 1) / 2;
-        // Four rows a warp keep 2 KB a warp in flight; with fewer than about
-        // two warps an SM that way, one row a warp spreads a small batch wider.
+        a.spans = DT == 2 ? (a.groups + 1) / 2 : (a.groups + 3) / 4;
+        // Four rows a warp keep 4 KB a warp in flight; where that leaves an SM
+        // fewer than 16 warps, one row a warp spreads a small batch wider.
         const int rp = a.rows * a.spans < 4 * 2 * 148 * kQuantWarps ? 1 : 4;
         const int64_t items = (a.rows + rp - 1) / rp * a.spans, grid = (items + kQuantWarps - 1) / kQuantWarps;
         EXL3_REQUIRE(items <= INT32_MAX, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: too many elements for one launch");
@@ -191,8 +207,8 @@ int quant_dispatch(QuantArgs& a, int block_rows, bool pow2, bool fast, cudaStrea
 // scales lie at scale[row * sr + group * sg].
 int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
                         float* scale, int64_t sr, int64_t sg, int block_rows, bool pow2, cudaStream_t s) {
-    const int vec = dtype == 2 ? 4 : 8;
-    const bool fast = cols % vec == 0 && ldx % vec == 0 && ldq % vec == 0 && aligned16(x) &&
+    const int vec = dtype == 2 ? 8 : 16;
+    const bool fast = cols % vec == 0 && ldx % (vec / 2) == 0 && ldq % vec == 0 && aligned16(x) &&
                       (reinterpret_cast<uintptr_t>(q) % (uintptr_t) vec) == 0;
     QuantArgs a{x, static_cast<uint8_t*>(q), scale, ldx, ldq, sr, sg, rows, (int) cols, (int) ((cols + kFp8Block - 1) / kFp8Block), 0};
     if (dtype == 0) return quant_dispatch<0>(a, block_rows, pow2, fast, s);
