@@ -13,9 +13,9 @@ namespace exl3 {
 // A lane holds VEC = 32 bytes / es elements of one row; 128 / VEC lanes hold a
 // group.  (With 16 bytes a lane the scale, its reciprocal and the addresses cost
 // as much as the values: 15 instructions a value with power-of-two scales.)
-// FAST: rows start and end on VEC-element boundaries, so whole vectors are
-// inside or outside; otherwise elements are moved one by one.
-template <int DT, bool FAST>
+// FAST 2: rows start and end on VEC-element boundaries, so whole vectors are
+// inside or outside; 1: the same for half vectors; 0: elements are moved one by one.
+template <int DT, int FAST>
 struct QuantVec {
     static constexpr int VEC = DT == 2 ? 8 : 16;
     static constexpr int LANES = kFp8Block / VEC;          // 16 (fp32) or 8
@@ -24,9 +24,9 @@ struct QuantVec {
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = 0u;
         if (left <= 0) return;
-        if (FAST) {
+        if constexpr (FAST != 0) {
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + at * (DT == 2 ? 4 : 2));
-            const uint4 a = __ldcs(src), b = __ldcs(src + 1);
+            const uint4 a = __ldcs(src), b = FAST == 2 || left > VEC / 2 ? __ldcs(src + 1) : make_uint4(0u, 0u, 0u, 0u);
             w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
             w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
         } else {
@@ -85,9 +85,17 @@ struct QuantVec {
 #pragma unroll
         for (int i = 0; i < VEC / 4; ++i)
             o[i] = e4m3x2(v[4 * i], v[4 * i + 1]) | (e4m3x2(v[4 * i + 2], v[4 * i + 3]) << 16);
-        if (FAST) {
+        if constexpr (FAST == 2) {
             if constexpr (DT == 2) *reinterpret_cast<uint2*>(q + at) = make_uint2(o[0], o[1]);
             else *reinterpret_cast<uint4*>(q + at) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else if constexpr (FAST == 1) {
+            if constexpr (DT == 2) {
+                *reinterpret_cast<uint32_t*>(q + at) = o[0];
+                if (left > VEC / 2) *reinterpret_cast<uint32_t*>(q + at + 4) = o[1];
+            } else {
+                *reinterpret_cast<uint2*>(q + at) = make_uint2(o[0], o[1]);
+                if (left > VEC / 2) *reinterpret_cast<uint2*>(q + at + 8) = make_uint2(o[2], o[3]);
+            }
         } else {
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
@@ -109,7 +117,7 @@ struct QuantArgs {
 // One scale for each row and group of 128 columns.  A warp takes one span of a
 // row -- two neighbouring groups (fp32) or four (16-bit) -- in RP consecutive
 // rows, all loads first.
-template <int DT, bool POW2, bool FAST, int RP>
+template <int DT, bool POW2, int FAST, int RP>
 __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(const __grid_constant__ QuantArgs p) {
     using V = QuantVec<DT, FAST>;
     // Whoever starts early behind this kernel finds all that came before it complete.
@@ -138,7 +146,7 @@ __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quant_rows_kernel(const 
 
 // One scale for each 128 x 128 block, held in registers: 512 threads of two
 // 32-byte pieces (16-bit types) or four (fp32).
-template <int DT, bool POW2, bool FAST>
+template <int DT, bool POW2, int FAST>
 __global__ void __launch_bounds__(512) fp8_quant_blocks_kernel(const __grid_constant__ QuantArgs p) {
     using V = QuantVec<DT, FAST>;
     constexpr int RP = 512 / V::LANES;                     // rows in a pass
@@ -180,7 +188,7 @@ int quant_pdl(void (*kern)(QuantArgs), dim3 grid, int threads, const QuantArgs& 
     return EXL3_OK;
 }
 
-template <int DT, bool POW2, bool FAST>
+template <int DT, bool POW2, int FAST>
 int quant_launch(QuantArgs& a, int block_rows, cudaStream_t s) {
     if (block_rows == 1) {
         a.spans = DT == 2 ? (a.groups + 1) / 2 : (a.groups + 3) / 4;
@@ -197,23 +205,23 @@ int quant_launch(QuantArgs& a, int block_rows, cudaStream_t s) {
     return quant_pdl(fp8_quant_blocks_kernel<DT, POW2, FAST>, dim3((unsigned) a.groups, (unsigned) rb), 512, a, s);
 }
 
-template <int DT>
-int quant_dispatch(QuantArgs& a, int block_rows, bool pow2, bool fast, cudaStream_t s) {
-    if (fast) return pow2 ? quant_launch<DT, true, true>(a, block_rows, s) : quant_launch<DT, false, true>(a, block_rows, s);
-    return pow2 ? quant_launch<DT, true, false>(a, block_rows, s) : quant_launch<DT, false, false>(a, block_rows, s);
+template <int DT, bool POW2>
+int quant_dispatch(QuantArgs& a, int block_rows, int fast, cudaStream_t s) {
+    return fast == 2 ? quant_launch<DT, POW2, 2>(a, block_rows, s) : fast == 1 ? quant_launch<DT, POW2, 1>(a, block_rows, s)
+                                                                              : quant_launch<DT, POW2, 0>(a, block_rows, s);
 }
 
 // Arguments are checked by the callers.  rows >= 1, cols in 1..2^30.  Rows'
 // scales lie at scale[row * sr + group * sg].
 int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
                         float* scale, int64_t sr, int64_t sg, int block_rows, bool pow2, cudaStream_t s) {
-    const int vec = dtype == 2 ? 8 : 16;
-    const bool fast = cols % vec == 0 && ldx % (vec / 2) == 0 && ldq % vec == 0 && aligned16(x) &&
-                      (reinterpret_cast<uintptr_t>(q) % (uintptr_t) vec) == 0;
+    const int half = dtype == 2 ? 4 : 8;                   // elements of 16 bytes
+    auto on = [&](int n) { return cols % n == 0 && ldx % half == 0 && ldq % n == 0 && aligned16(x) && reinterpret_cast<uintptr_t>(q) % (uintptr_t) n == 0; };
+    const int fast = on(2 * half) ? 2 : on(half) ? 1 : 0;
     QuantArgs a{x, static_cast<uint8_t*>(q), scale, ldx, ldq, sr, sg, rows, (int) cols, (int) ((cols + kFp8Block - 1) / kFp8Block), 0};
-    if (dtype == 0) return quant_dispatch<0>(a, block_rows, pow2, fast, s);
-    if (dtype == 1) return quant_dispatch<1>(a, block_rows, pow2, fast, s);
-    return quant_dispatch<2>(a, block_rows, pow2, fast, s);
+    if (dtype == 0) return pow2 ? quant_dispatch<0, true>(a, block_rows, fast, s) : quant_dispatch<0, false>(a, block_rows, fast, s);
+    if (dtype == 1) return pow2 ? quant_dispatch<1, true>(a, block_rows, fast, s) : quant_dispatch<1, false>(a, block_rows, fast, s);
+    return pow2 ? quant_dispatch<2, true>(a, block_rows, fast, s) : quant_dispatch<2, false>(a, block_rows, fast, s);
 }
 
 }  // namespace exl3

@@ -26,7 +26,7 @@ def _same(q, want):
 @pytest.mark.parametrize("pow2", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("block_rows", [1, 128])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 128), (3, 257), (130, 520), (128, 1000), (65, 4096)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 128), (3, 257), (130, 520), (128, 1000), (65, 4096), (9, 1036), (300, 4008)])
 def test_quantize_bits(cuda, rows, cols, block_rows, dtype, pow2):
     x = R.activations(rows, cols, rows + cols, dtype, cuda)
     q, s = ext.fp8_quantize(x, block_rows=block_rows, pow2_scale=pow2)
