@@ -104,7 +104,7 @@ struct QuantVec {
     }
 };
 
-constexpr int kQuantWarps = 8;
+constexpr int kQuantWarps = 4;         // 8192 x 4096, powers of two: 14.5 us with 4 warps a CTA, 17.3 with 8
 
 struct QuantArgs {
     const void* x;
@@ -192,9 +192,10 @@ template <int DT, bool POW2, int FAST>
 int quant_launch(QuantArgs& a, int block_rows, cudaStream_t s) {
     if (block_rows == 1) {
         a.spans = DT == 2 ? (a.groups + 1) / 2 : (a.groups + 3) / 4;
-        // Four rows a warp keep 4 KB a warp in flight; where that leaves an SM
-        // fewer than 16 warps, one row a warp spreads a small batch wider.
-        const int rp = a.rows * a.spans < 4 * 2 * 148 * kQuantWarps ? 1 : 4;
+        // Four rows a warp keep 4 KB a warp in flight (8192 rows x 4096: 14.5 us,
+        // with one row 18.6); below some 32768 spans the other way round, since the
+        // grid is a few waves then (1024 rows: 5.2 us with four, 4.4 with one).
+        const int rp = a.rows * a.spans < 32768 ? 1 : 4;
         const int64_t items = (a.rows + rp - 1) / rp * a.spans, grid = (items + kQuantWarps - 1) / kQuantWarps;
         EXL3_REQUIRE(items <= INT32_MAX, EXL3_ERR_UNSUPPORTED, "exl3_fp8_quantize: too many elements for one launch");
         return quant_pdl(rp == 1 ? fp8_quant_rows_kernel<DT, POW2, FAST, 1> : fp8_quant_rows_kernel<DT, POW2, FAST, 4>,
