@@ -3,9 +3,10 @@
 //   G = x . Wgate_e^T, U = x . Wup_e^T      (x in e4m3, scales by row and 128 columns)
 //   a = silu(min(G, L)) * clamp(U, -L, L)   (fp32; quantised the same way)
 //   out[t] = sum over the valid slots of weight * (a . Wdown_e^T)   (fp32, one cast)
-// An x in 16 or 32 bits goes through the quantiser's kernel first.  (Quantising
-// it inside kernel 1, for every output tile anew, cost one warp about 2000
-// clocks a row and block: four tokens took 232 us.)
+// An x in 16 or 32 bits is quantised by kernel 1, once in every CTA while its first
+// weights are on their way, up to four rows; above that by the quantiser's kernel
+// before it.  (Quantising it inside kernel 1 for every output tile anew cost one
+// warp about 2000 clocks a row and block: four tokens took 232 us.)
 //
 // Bound: the routed experts' weights, 3 * H * I bytes each, read once.  So both
 // kernels do nothing but stream weight blocks: a 128 x 128 block is one TMA box
@@ -50,6 +51,12 @@ constexpr int kFmThreads = 256;
 constexpr int kFmProducerWarp = 4;
 constexpr int kFmMmaWarp = 5;
 constexpr int kFmFacWarp = 6;
+// Rows and width of an x that kernel 1 quantises itself, once a CTA and into its
+// own shared memory (a launch less: 1 token of 4096 takes 20.8 us for 21.4, 4 tokens
+// 138.4 for 139.1); above, the quantiser's launch comes first.  Four rows are what
+// a warp quantises at once; a wider x would leave the ring fewer than three blocks.
+constexpr int kFmInlineRows = 4;
+constexpr int kFmInlineHidden = 6144;
 constexpr int kFmMaxSlotsW = 12;             // weight blocks in the ring
 constexpr int kFmMaxBufs = 4;                // steps whose sums and inputs are held
 // Control region (uint32 words): [2] status; counters of kernel 1's output
@@ -67,7 +74,9 @@ struct FmParams {
     void* out;
     const float* w13s;           // [E][2 I / 128][H / 128]
     const float* w2s;            // [E][H / 128][I / 128]
-    const float* xs;             // its scales: xs[token * xsr + block * xsg]
+    const void* x;               // an x that kernel 1 quantises: fp16 / bf16 / fp32 [m][H]
+    int x_dtype, xvec;
+    const float* xs;             // scales of an e4m3 x: xs[token * xsr + block * xsg]
     int64_t xsr, xsg;
     uint8_t* aq;                 // [slots][I] e4m3
     float* as;                   // [slots][I / 128]
@@ -98,13 +107,17 @@ struct FmPlan {
 // head, kernel 2's output rows.  A step is one block of k: kernel 1 multiplies
 // the gate and the up block, each into TMEM columns of its own, kernel 2 the down
 // block.  D's columns are all tokens in kernel 1 -- those that are not the
-// expert's are never used -- and the group's pairs in kernel 2.
-template <int NT, int PH>
+// expert's are never used -- and the group's pairs in kernel 2.  INL: kernel 1's x
+// lies beside the ring, 8 rows x 128 bytes a block of k and then its scales; the
+// tensor core reads 16 rows, the second half being the next block's, whose columns
+// are never used.
+template <int NT, int PH, bool INL = false>
 struct FmLayout {
+    static_assert(!INL || (NT == 16 && PH == 0), "");
     static constexpr int kMats = PH == 0 ? 2 : 1;
     static constexpr int kBufs = NT <= 16 ? 4 : PH == 0 ? 2 : NT <= 32 ? 4 : 2;
     static constexpr int kTmemCols = NT * kMats * kBufs;             // 64 .. 256
-    static constexpr int kSlot = (int) kFp8WTile + NT * 128;
+    static constexpr int kSlot = (int) kFp8WTile + (INL ? 0 : NT * 128);
 };
 
 template <int NT>
@@ -124,6 +137,10 @@ struct FmHead {
     uint32_t tmem;
     uint32_t last;
 };
+
+// The head's bytes, so that what follows it starts on a swizzle atom.
+template <int NT>
+__host__ __device__ constexpr int fm_head_bytes() { return ((int) sizeof(FmHead<NT>) + 1023) / 1024 * 1024; }
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 // The epilogue hands a part that it has stored to the finisher and goes on.
@@ -244,19 +261,21 @@ __device__ __forceinline__ float fm_swiglu(float g, float u, float lim) {
     return g / (1.f + expf(-g)) * u;
 }
 
-template <int NT, int PH>
+template <int NT, int PH, bool INL>
 __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(const __grid_constant__ FmParams p) {
-    using L = FmLayout<NT, PH>;
+    using L = FmLayout<NT, PH, INL>;
     constexpr int kMats = L::kMats, kBufs = L::kBufs, kFacs = 2 * L::kBufs;
     constexpr int kCh = NT < 32 ? 4 : 8;                              // columns handled together at a tile's end
     extern __shared__ uint8_t fm_raw[];
     uint8_t* ring = fm_raw + ((1024u - (smem_u32(fm_raw) & 1023u)) & 1023u);
     FmHead<NT>& S = *reinterpret_cast<FmHead<NT>*>(ring + p.slots * L::kSlot);
     float* oacc = reinterpret_cast<float*>(ring + p.slots * L::kSlot + sizeof(FmHead<NT>));    // PH 1: [m][128]
+    uint8_t* xres = ring + p.slots * L::kSlot + fm_head_bytes<NT>();                           // INL: [KB + 1][1024]
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const int C = (int) gridDim.x, cta = (int) blockIdx.x;
     const int NBI = p.I / 128, NBH = p.H / 128, KB = PH == 0 ? NBH : NBI;
     const int W = p.slots;
+    float* xsc = reinterpret_cast<float*>(xres + (KB + 1) * 1024);                             // INL: [KB][8]
     uint32_t* status = p.ctrl + 2;
 
     if (tid == 0) {
@@ -339,6 +358,24 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
         }
     };
 
+    if (INL && warp != kFmProducerWarp) {
+        // x's blocks of this CTA's range, while the first weights are on their way
+        const int w = warp < kFmProducerWarp ? warp : warp - 1;
+        for (int i = w; i < min(nsteps, KB); i += 7) {
+            const int kb = (beg + i) % KB, lr = XRows::row(p.m, lane);
+            XRows r;
+            r.load(p.m, p.x, p.x_dtype, (int64_t) lr * p.H + kb * 128 + XRows::col(p.m, lane), lr < p.m ? 16 : 0, p.xvec != 0);
+            float sx;
+            const uint4 q = r.quantize(p.m, p.x_dtype, p.pow2 != 0, sx);
+            if (lr < p.m) {
+                XRows::store(p.m, xres + kb * 1024, lr, lane, q);
+                if (p.m == 1 ? lane == 0 : (lane & 7) == 0) xsc[kb * 8 + lr] = sx;
+            }
+        }
+        fence_proxy_async_smem();
+        asm volatile("bar.sync 3, 224;" ::: "memory");
+    }
+
     if (warp == kFmProducerWarp) {
         if (lane == 0 && nsteps > 0) {
             const int nblk = nsteps * kMats;
@@ -359,15 +396,17 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
             FmAt<PH> a0 = a;
             int t = 0;
             for (; t < min(W, nblk); ++t) { weights(a, mat_of(t), t); next(a, t); }
-            pdl_wait();
-            fence_proxy_async_global();
-            for (int i = 0; i < t; ++i) { inputs(a0, i); next(a0, i); }
+            if (!INL) {
+                pdl_wait();
+                fence_proxy_async_global();
+                for (int i = 0; i < t; ++i) { inputs(a0, i); next(a0, i); }
+            }
             int issued = t;
             for (; t < nblk; ++t) {
                 const int slot = t % W;
                 if (t >= W && !mbar_wait(&S.wdone[slot], ((t / W) + 1u) & 1u, status)) break;
                 weights(a, mat_of(t), slot);
-                inputs(a, slot);
+                if (!INL) inputs(a, slot);
                 next(a, t);
                 ++issued;
             }
@@ -379,7 +418,7 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
         }
     } else if (warp == kFmMmaWarp) {
         pdl_wait();                                                   // the bounded waits begin behind it
-        const uint64_t wdesc0 = sdesc_sw128(smem_u32(ring));
+        const uint64_t wdesc0 = sdesc_sw128(smem_u32(ring)), xdesc0 = sdesc_sw128(smem_u32(xres));
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
         int slot = 0;
         uint32_t wpar = 0;
@@ -394,7 +433,8 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
                 ok = ok && mbar_poll_lanes(&S.wfull[slot], wpar, status);
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t wd = wdesc0 + (uint64_t) (slot * (L::kSlot >> 4)), xd = wd + (kFp8WTile >> 4);
+                const uint64_t wd = wdesc0 + (uint64_t) (slot * (L::kSlot >> 4));
+                const uint64_t xd = INL ? xdesc0 + (uint64_t) (a.kb * 64) : wd + (kFp8WTile >> 4);
                 if (elect_lane()) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) tc_mma_f8(tmem + (b * kMats + mat) * NT, wd + 2 * q, xd + 2 * q, id, q);
@@ -426,7 +466,7 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
 #pragma unroll
             for (int h = 0; h < (NT + 31) / 32; ++h) {
                 const int j = h * 32 + lane;
-                if (j < n) v.f[h] = PH == 0 ? __ldcg(p.xs + j * p.xsr + at.kb * p.xsg) : __ldcg(p.as + (int64_t) (p0 + j) * NBI + at.kb);
+                if (j < n) v.f[h] = INL ? xsc[at.kb * 8 + j] : PH == 0 ? __ldcg(p.xs + j * p.xsr + at.kb * p.xsg) : __ldcg(p.as + (int64_t) (p0 + j) * NBI + at.kb);
             }
             at.next();
             return v;
@@ -641,13 +681,14 @@ FmGeom fm_geom(int64_t m, int64_t topk, int64_t H, int64_t I) {
     return g;
 }
 
-template <int NT, int PH>
+template <int NT, int PH, bool INL>
 int fm_launch(FmParams p, int sms, cudaStream_t stream) {
-    using L = FmLayout<NT, PH>;
+    using L = FmLayout<NT, PH, INL>;
     // The two kernels share an SM while kernel 2 waits: 120 + 104 KB of its memory.
     constexpr int kBudget = (PH == 0 ? 120 : 104) * 1024;
-    const int extra = 1024 + (int) sizeof(FmHead<NT>) + (PH == 1 ? p.m * 512 : 0);
     static_assert(sizeof(FmHead<64>) + 64 * 512 + 1024 + 2 * FmLayout<64, 1>::kSlot <= 104 * 1024, "room for two blocks");
+    const int extra = INL ? 1024 + fm_head_bytes<NT>() + (p.H / 128 + 1) * 1024 + p.H / 128 * 32
+                          : 1024 + (int) sizeof(FmHead<NT>) + (PH == 1 ? p.m * 512 : 0);
     int slots = (kBudget - extra) / L::kSlot;
     if (slots > kFmMaxSlotsW) slots = kFmMaxSlotsW;
     p.slots = slots;
@@ -657,9 +698,9 @@ int fm_launch(FmParams p, int sms, cudaStream_t stream) {
     EXL3_CUDA(cudaGetDevice(&dev));
     cudaError_t attr = cudaSuccess;
     std::call_once(once[dev & 63], [&] {
-        attr = cudaFuncSetAttribute(fp8_moe_kernel<NT, PH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
+        attr = cudaFuncSetAttribute(fp8_moe_kernel<NT, PH, INL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
         if (attr == cudaSuccess)   // all of it, or the SM's split made for one CTA keeps the other kernel's out
-            attr = cudaFuncSetAttribute(fp8_moe_kernel<NT, PH>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+            attr = cudaFuncSetAttribute(fp8_moe_kernel<NT, PH, INL>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     });
     EXL3_CUDA(attr);
     cudaLaunchConfig_t cfg{};
@@ -672,14 +713,14 @@ int fm_launch(FmParams p, int sms, cudaStream_t stream) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    EXL3_CUDA(cudaLaunchKernelEx(&cfg, fp8_moe_kernel<NT, PH>, p));
+    EXL3_CUDA(cudaLaunchKernelEx(&cfg, fp8_moe_kernel<NT, PH, INL>, p));
     return EXL3_OK;
 }
 
-template <int NT>
+template <int NT, bool INL = false>
 int fm_run(const FmParams& p, int sms, cudaStream_t s) {
-    const int rc = fm_launch<NT, 0>(p, sms, s);
-    return rc != EXL3_OK ? rc : fm_launch<NT, 1>(p, sms, s);
+    const int rc = fm_launch<NT, 0, INL>(p, sms, s);
+    return rc != EXL3_OK ? rc : fm_launch<NT, 1, false>(p, sms, s);
 }
 
 }  // namespace
@@ -745,6 +786,12 @@ extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, const float* x_sc
     auto s = static_cast<cudaStream_t>(stream);
     const void* xq = x;
     p.xs = x_scale; p.xsr = hidden / 128; p.xsg = 1;
+    if (x_dtype != EXL3_DTYPE_E4M3 && m <= kFmInlineRows && hidden <= kFmInlineHidden) {
+        p.x = x;
+        p.x_dtype = x_dtype;
+        p.xvec = aligned16(x);
+        return fm_run<16, true>(p, di.sms, s);
+    }
     if (x_dtype != EXL3_DTYPE_E4M3) {
         float* xs = reinterpret_cast<float*>(sb + g.off_xs);
         xq = sb + g.off_xq;

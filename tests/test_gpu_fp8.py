@@ -294,6 +294,24 @@ def test_moe_prequantised(cuda, T):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 2, 3, 4])
+def test_moe_few_tokens_quantised_inside(cuda, T, dtype):
+    """Up to four tokens are quantised by the experts' kernel: the bits of a call on
+    an e4m3 x, from a start off 16 bytes too, on either side of its width limit."""
+    for H, I, E in ((128, 128, 3), (640, 384, 8), (6144, 128, 4), (6272, 128, 4)):
+        layer = _layer(cuda, E, H, I, 13)
+        ids, rw = _route(T, E, 3, T, cuda)
+        flat = R.activations(1, T * H + 1, T, dtype, cuda).view(-1)
+        for x in (flat[:-1].view(T, H), flat[1:].view(T, H)):
+            for pow2 in (False, True):
+                scratch = torch.zeros(ext.fp8_moe_scratch_bytes(T, 3, H, I), dtype=torch.uint8, device=cuda)
+                q, s = ext.fp8_quantize(x, pow2_scale=pow2)
+                a = ext.fp8_moe_decode(q, torch.empty_like(x), *layer, ids, rw, 10.0, scratch, x_scale=s, pow2_scale=pow2)
+                b = ext.fp8_moe_decode(x, torch.empty_like(x), *layer, ids, rw, 10.0, scratch, pow2_scale=pow2)
+                assert torch.equal(a, b)
+
+
 def test_moe_many_rows_in_pieces(cuda):
     layer = _layer(cuda, 4, 256, 128, 6)
     ids, rw = _route(150, 4, 2, 9, cuda)
