@@ -299,7 +299,7 @@ def test_moe_prequantised(cuda, T):
 def test_moe_few_tokens_quantised_inside(cuda, T, dtype):
     """Up to four tokens are quantised by the experts' kernel: the bits of a call on
     an e4m3 x, from a start off 16 bytes too, on either side of its width limit."""
-    for H, I, E in ((128, 128, 3), (640, 384, 8), (6144, 128, 4), (6272, 128, 4)):
+    for H, I, E in ((128, 128, 3), (640, 384, 8), (4096, 128, 4), (4224, 128, 4)):
         layer = _layer(cuda, E, H, I, 13)
         ids, rw = _route(T, E, 3, T, cuda)
         flat = R.activations(1, T * H + 1, T, dtype, cuda).view(-1)
