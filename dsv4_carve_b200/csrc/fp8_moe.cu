@@ -52,7 +52,7 @@ constexpr int kFmProducerWarp = 4;
 constexpr int kFmMmaWarp = 5;
 constexpr int kFmFacWarp = 6;
 // Rows and width of an x that kernel 1 quantises itself, once a CTA and into its
-// own shared memory (a launch less: 1 token of 4096 takes 20.8 us for 21.4, 4 tokens
+// own shared memory (a launch less: 1 token of 4096 takes 20.4 us for 21.4, 4 tokens
 // 138.4 for 139.1); above, the quantiser's launch comes first.  Four rows are what
 // a warp quantises at once.  A wider x takes too much of the ring: with 8 experts of
 // 2048 a token takes 33.3 us for 34.7 at 2048 columns, 49.7 for 51.1 at 4096, but
@@ -109,11 +109,11 @@ struct FmPlan {
 // head, kernel 2's output rows.  A step is one block of k: kernel 1 multiplies
 // the gate and the up block, each into TMEM columns of its own, kernel 2 the down
 // block.  D's columns are all tokens in kernel 1 -- those that are not the
-// expert's are never used -- and the group's pairs in kernel 2.  INL: kernel 1's x
-// lies beside the ring, 8 rows x 128 bytes a block of k and then its scales; the
-// tensor core reads 16 rows, the second half being the next block's, whose columns
-// are never used.
-template <int NT, int PH, bool INL = false>
+// expert's are never used -- and the group's pairs in kernel 2.  INL (rows that a
+// warp quantises at once, 1 or 4): kernel 1's x lies beside the ring, 8 rows x 128
+// bytes a block of k and then its scales; the tensor core reads 16 rows, the second
+// half being the next block's, whose columns are never used.
+template <int NT, int PH, int INL = 0>
 struct FmLayout {
     static_assert(!INL || (NT == 16 && PH == 0), "");
     static constexpr int kMats = PH == 0 ? 2 : 1;
@@ -263,7 +263,7 @@ __device__ __forceinline__ float fm_swiglu(float g, float u, float lim) {
     return g / (1.f + expf(-g)) * u;
 }
 
-template <int NT, int PH, bool INL>
+template <int NT, int PH, int INL>
 __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(const __grid_constant__ FmParams p) {
     using L = FmLayout<NT, PH, INL>;
     constexpr int kMats = L::kMats, kBufs = L::kBufs, kFacs = 2 * L::kBufs;
@@ -362,16 +362,17 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
 
     if (INL && warp != kFmProducerWarp) {
         // x's blocks of this CTA's range, while the first weights are on their way
-        const int w = warp < kFmProducerWarp ? warp : warp - 1;
+        const int w = warp < kFmProducerWarp ? warp : warp - 1, lr = XRows::row(INL, lane);
+#pragma unroll 1
         for (int i = w; i < min(nsteps, KB); i += 7) {
-            const int kb = (beg + i) % KB, lr = XRows::row(p.m, lane);
+            const int kb = (beg + i) % KB;
             XRows r;
-            r.load(p.m, p.x, p.x_dtype, (int64_t) lr * p.H + kb * 128 + XRows::col(p.m, lane), lr < p.m ? 16 : 0, p.xvec != 0);
+            r.load(INL, p.x, p.x_dtype, (int64_t) lr * p.H + kb * 128 + XRows::col(INL, lane), lr < p.m ? 16 : 0, p.xvec != 0);
             float sx;
-            const uint4 q = r.quantize(p.m, p.x_dtype, p.pow2 != 0, sx);
+            const uint4 q = r.quantize(INL, p.x_dtype, p.pow2 != 0, sx);
             if (lr < p.m) {
-                XRows::store(p.m, xres + kb * 1024, lr, lane, q);
-                if (p.m == 1 ? lane == 0 : (lane & 7) == 0) xsc[kb * 8 + lr] = sx;
+                XRows::store(INL, xres + kb * 1024, lr, lane, q);
+                if (INL == 1 ? lane == 0 : (lane & 7) == 0) xsc[kb * 8 + lr] = sx;
             }
         }
         fence_proxy_async_smem();
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
                 const int e = P.pexp[P.gstart[a.g]];
                 mbar_arrive_expect_tx(&S.wfull[slot], (uint32_t) L::kSlot);
                 const int row = PH == 0 ? e * 2 * p.I + mat * p.I + (a.tile % NBI) * 128 : e * p.H + a.tile * 128;
-                tma_load_2d(ring + slot * L::kSlot, PH == 0 ? &p.w13 : &p.w2, a.kb * 128, row, &S.wfull[slot]);
+                tma_load_2d_once(ring + slot * L::kSlot, PH == 0 ? &p.w13 : &p.w2, a.kb * 128, row, &S.wfull[slot]);
             };
             auto inputs = [&](const FmAt<PH>& a, int slot) {
                 if (PH == 0) tma_load_2d(ring + slot * L::kSlot + kFp8WTile, &p.xmap, a.kb * 128, 0, &S.wfull[slot]);
@@ -683,7 +684,7 @@ FmGeom fm_geom(int64_t m, int64_t topk, int64_t H, int64_t I) {
     return g;
 }
 
-template <int NT, int PH, bool INL>
+template <int NT, int PH, int INL>
 int fm_launch(FmParams p, int sms, cudaStream_t stream) {
     using L = FmLayout<NT, PH, INL>;
     // The two kernels share an SM while kernel 2 waits: 120 + 104 KB of its memory.
@@ -719,10 +720,10 @@ int fm_launch(FmParams p, int sms, cudaStream_t stream) {
     return EXL3_OK;
 }
 
-template <int NT, bool INL = false>
+template <int NT, int INL = 0>
 int fm_run(const FmParams& p, int sms, cudaStream_t s) {
     const int rc = fm_launch<NT, 0, INL>(p, sms, s);
-    return rc != EXL3_OK ? rc : fm_launch<NT, 1, false>(p, sms, s);
+    return rc != EXL3_OK ? rc : fm_launch<NT, 1, 0>(p, sms, s);
 }
 
 }  // namespace
@@ -792,7 +793,7 @@ extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, const float* x_sc
         p.x = x;
         p.x_dtype = x_dtype;
         p.xvec = aligned16(x);
-        return fm_run<16, true>(p, di.sms, s);
+        return m == 1 ? fm_run<16, 1>(p, di.sms, s) : fm_run<16, kFmInlineRows>(p, di.sms, s);
     }
     if (x_dtype != EXL3_DTYPE_E4M3) {
         float* xs = reinterpret_cast<float*>(sb + g.off_xs);
