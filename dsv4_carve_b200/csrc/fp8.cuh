@@ -103,6 +103,12 @@ static __device__ __noinline__ uint32_t fp8_pack4(float a, float b, float c, flo
     return e4m3x2(v[0], v[1]) | (e4m3x2(v[2], v[3]) << 16);
 }
 
+static __device__ __noinline__ uint32_t fp8_pack1(float a, float s, float inv, bool pow2) {
+    float v[1] = {a};
+    fp8_quotients(v, s, inv, pow2);
+    return e4m3x2(v[0], 0.f) & 0xFFu;
+}
+
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // ---------------------------------------------------------------- loads
