@@ -55,7 +55,7 @@ constexpr int kFmMmaWarp = 5;
 constexpr int kFmFacWarp = 6;
 // Rows and width of an x that kernel 1 quantises itself, once a CTA and into its
 // own shared memory (a launch less: 1 token of 4096 takes 20.4 us for 21.4, 4 tokens
-// 138.4 for 139.1); above, the quantiser's launch comes first.  Four rows are what
+// 130.5 for 133.1); above, the quantiser's launch comes first.  Four rows are what
 // a warp quantises at once.  A wider x takes too much of the ring: with 8 experts of
 // 2048 a token takes 33.3 us for 34.7 at 2048 columns, 49.7 for 51.1 at 4096, but
 // 60.5 for 59.5 at 5120 and 72.2 for 67.4 at 6144.
