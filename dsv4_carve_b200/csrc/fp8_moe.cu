@@ -512,7 +512,9 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
                 part_wait();
                 uint32_t done = 0u;
                 if (lane == 0) done = atom_add_acq_rel_gpu(&p.ctrl[(PH == 0 ? kFmCntA : kFmCntB) + first / per_tile], (uint32_t) steps) + (uint32_t) steps;
-                if (__shfl_sync(0xffffffffu, done, 0) == (uint32_t) per_tile) finish_shared(first / per_tile, 0, 1);
+                done = __shfl_sync(0xffffffffu, done, 0);
+                __syncwarp();                                         // a shuffle orders no memory: lane 0's acquire before all lanes' loads
+                if (done == (uint32_t) per_tile) finish_shared(first / per_tile, 0, 1);
             }
         }
     } else {
