@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import logging
 import os
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -252,23 +253,42 @@ class Fp8MoeState:
         self.pow2_scale = bool(pow2_scale)
 
 
-_FP8_SCRATCH: dict[tuple, torch.Tensor] = {}
+class _Fp8Scratch:
+    """Zeroed scratch of one stream.  A call is two or three launches that hand
+    their sums on through it, so a host thread holds the lock from taking the
+    buffer to its last launch: another thread's call on the same stream comes
+    behind it whole."""
+    __slots__ = ("lock", "buf")
+
+    def __init__(self):
+        self.lock = threading.Lock()
+        self.buf = None
+
+    def take(self, device: torch.device, nbytes: int) -> torch.Tensor:
+        if self.buf is None or self.buf.numel() < nbytes:
+            self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        return self.buf
 
 
-def _fp8_moe_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Zeroed scratch of one stream (calls on different streams may overlap).
-    A capture gets its own, from the graph's memory, so that graphs which are
-    replayed side by side share nothing."""
-    if torch.cuda.is_current_stream_capturing():
+class _Fp8CaptureScratch(_Fp8Scratch):
+    """Scratch of one captured call, from the graph's memory, so that graphs
+    which are replayed side by side share nothing."""
+    __slots__ = ()
+
+    def take(self, device: torch.device, nbytes: int) -> torch.Tensor:
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
         scratch[:_ext._lib.FP8_MOE_CTRL_BYTES].zero_()
         return scratch
+
+
+_FP8_SCRATCH: dict[tuple, _Fp8Scratch] = {}
+
+
+def _fp8_moe_scratch(device: torch.device) -> _Fp8Scratch:
+    if torch.cuda.is_current_stream_capturing():
+        return _Fp8CaptureScratch()
     key = (device.index, _ext._raw_stream(device.index))
-    buf = _FP8_SCRATCH.get(key)
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-        _FP8_SCRATCH[key] = buf
-    return buf
+    return _FP8_SCRATCH.get(key) or _FP8_SCRATCH.setdefault(key, _Fp8Scratch())
 
 
 def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, state: Fp8MoeState,
@@ -294,14 +314,16 @@ def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, s
     if _ext._current_device() != w.index:      # captures are asked of the current device's stream
         with _ext._on_device(x.device):
             return apply_fp8_moe(x, ids2, route_w, state, expert_map, limit, out)
-    scratch = _fp8_moe_scratch(x.device, w.scratch_bytes(min(T, step), topk))
-    if T <= step:
-        _ext._fp8_moe_decode(x, None, out, w, ids2, route_w, limit, scratch, expert_map, state.pow2_scale, None)
-    else:
-        for t in range(0, T, step):
-            part = slice(t, min(T, t + step))
-            _ext._fp8_moe_decode(x[part], None, out[part], w, ids2[part], route_w[part], limit, scratch, expert_map,
-                                 state.pow2_scale, None)
+    held = _fp8_moe_scratch(x.device)
+    with held.lock:
+        scratch = held.take(x.device, w.scratch_bytes(min(T, step), topk))
+        if T <= step:
+            _ext._fp8_moe_decode(x, None, out, w, ids2, route_w, limit, scratch, expert_map, state.pow2_scale, None)
+        else:
+            for t in range(0, T, step):
+                part = slice(t, min(T, t + step))
+                _ext._fp8_moe_decode(x[part], None, out[part], w, ids2[part], route_w[part], limit, scratch, expert_map,
+                                     state.pow2_scale, None)
     _CALLS["b200"] += 1
     return out
 

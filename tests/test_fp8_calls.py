@@ -1,0 +1,85 @@
+"""Calls of the e4m3 layers as the host makes them, without a GPU: tensors that
+pass as CUDA ones, and recorded launches."""
+from __future__ import annotations
+
+import threading
+import time
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from dsv4_carve_b200 import moe
+from dsv4_carve_b200 import vllm_exl3_c as ext
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that says it is on a CUDA device."""
+    index = 0
+
+    is_cuda = property(lambda self: True)
+    device = property(lambda self: torch.device("cuda", self.index))
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        kwargs = {k: v for k, v in (kwargs or {}).items() if k != "device"}
+        return super().__torch_function__(func, types, args, kwargs)
+
+
+class OnDevice1(OnDevice):
+    index = 1
+
+
+@pytest.fixture
+def layer(monkeypatch):
+    """An Fp8MoeState of 8 experts, 256 x 128, on device 0 whose launches are recorded in `launched`."""
+    state = object.__new__(moe.Fp8MoeState)
+    launched = []
+    state.__dict__.update(experts=SimpleNamespace(index=0, device=torch.device("cuda", 0), E=8, H=256, I=128,
+                                                  scratch_bytes=lambda m, topk: ext.fp8_moe_scratch_bytes(m, topk, 256, 128)),
+                          n_experts=8, hidden=256, inter=128, pow2_scale=False, launched=launched)
+    current = [0]
+    monkeypatch.setattr(ext, "_current_device", lambda: current[0])
+    monkeypatch.setattr(ext, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "set_device", lambda i: current.__setitem__(0, i))
+    monkeypatch.setattr(moe, "_FP8_SCRATCH", {})
+    monkeypatch.setattr(ext, "_fp8_moe_decode", lambda *a: launched.append(a))
+    real_zeros, real_empty = torch.zeros, torch.empty
+    host = lambda f: lambda *a, device=None, **k: f(*a, **k).as_subclass(OnDevice)  # noqa: E731
+    monkeypatch.setattr(torch, "zeros", host(real_zeros))
+    monkeypatch.setattr(torch, "empty", host(real_empty))
+    return state
+
+
+def _call(T=3, topk=2, kind=OnDevice, dtype=torch.bfloat16, **kw):
+    x = torch.ones((T, 256)).to(dtype).as_subclass(kind)
+    return dict(x2d=x, ids=torch.ones((T, topk), dtype=torch.int32).as_subclass(kind),
+                weights=torch.ones((T, topk)).as_subclass(kind), **kw)
+
+
+def test_moe_launches_once_up_to_the_ceiling_and_in_pieces_above(layer):
+    moe.apply_moe(**_call(32, 8), state=layer)
+    assert len(layer.launched) == 1
+    moe.apply_moe(**_call(33, 8), state=layer)
+    assert [a[0].shape[0] for a in layer.launched] == [32, 32, 1]
+
+
+def test_moe_host_threads_on_one_stream_take_turns(layer, monkeypatch):
+    """One call at a time holds a stream's scratch, from its first launch to its last."""
+    inside, most = [0], [0]
+
+    def launch(*a):
+        inside[0] += 1
+        most[0] = max(most[0], inside[0])
+        time.sleep(0.005)                      # the other threads run meanwhile, as during a C call
+        inside[0] -= 1
+
+    monkeypatch.setattr(ext, "_fp8_moe_decode", launch)
+    threads = [threading.Thread(target=lambda: [moe.apply_moe(**_call(), state=layer) for _ in range(5)]) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert most[0] == 1

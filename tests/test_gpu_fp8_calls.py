@@ -1,0 +1,47 @@
+"""Calls of the e4m3 operators that a serving program makes: from several host
+threads, on slices, with signed zeros."""
+from __future__ import annotations
+
+import threading
+
+import pytest
+import torch
+
+from dsv4_carve_b200 import moe
+from tests import fp8_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def _layer(cuda, E, H, I, seed):
+    return (*R.e4m3_weight((E, 2 * I, H), 100 + seed, cuda), *R.e4m3_weight((E, H, I), 200 + seed, cuda))
+
+
+def _route(T, E, topk, seed, cuda):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.stack([torch.randperm(E, generator=g)[:topk] for _ in range(T)]).to(torch.int32)
+    return ids.to(cuda), torch.softmax(torch.randn((T, topk), generator=g), dim=1).to(cuda)
+
+
+def test_moe_two_host_threads_on_one_stream(cuda):
+    """Layers of different sizes from two threads whose current stream is the same."""
+    work = []
+    for i, (T, H, I) in enumerate(((8, 512, 256), (3, 256, 512))):
+        state = moe.Fp8MoeState(*_layer(cuda, 8, H, I, i))
+        ids, rw = _route(T, 8, 4, i, cuda)
+        x = R.activations(T, H, i, torch.bfloat16, cuda)
+        work.append((x, ids, rw, state, moe.apply_moe(x, ids, rw, state, None, 10.0)))
+    torch.cuda.synchronize()
+    wrong = [None, None]
+
+    def run(i):
+        x, ids, rw, state, want = work[i]
+        wrong[i] = sum(((moe.apply_moe(x, ids, rw, state, None, 10.0) != want).any() for _ in range(400)),
+                       torch.zeros((), dtype=torch.int64, device=cuda))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert [int(w) for w in wrong] == [0, 0]
