@@ -536,11 +536,15 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
         clear();
         FmAt<PH> a(beg, max(G, 1), NBI, KB);
         int seg = 0;                                                  // steps of the current tile so far
-        bool handed = false;
+        // The four warps meet at barriers of a fixed count at tile ends, and each has
+        // a verdict of its own on every wait.  So a warp whose wait gave up walks on
+        // through its steps and meets them all, without waiting, reading TMEM or
+        // arriving any more; what it leaves is in bounds, and the status marks it.
+        bool ok = true;
         for (int s = 0; s < nsteps; ++s) {
             const int b = s % kBufs;
             const int p0 = P.gstart[a.g], pairs = P.gstart[a.g + 1] - p0, n = PH == 0 ? p.m : pairs;   // n: D's columns
-            if (!mbar_wait_lanes(&S.tfull[b], (s / kBufs) & 1u, status)) break;
+            ok = ok && mbar_wait_lanes(&S.tfull[b], (s / kBufs) & 1u, status);
             tc_fence_after();
 #pragma unroll
             for (int mat = 0; mat < kMats; ++mat) {
@@ -548,7 +552,7 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
                 const float4* f4 = reinterpret_cast<const float4*>(S.fac[s % kFacs]);
 #pragma unroll
                 for (int c = 0; c < NT / 16; ++c) {
-                    if (c * 16 >= n) break;
+                    if (c * 16 >= n || !ok) break;
                     float v[16];
                     tc_ld16(tmem + ((uint32_t) (warp * 32) << 16) + (uint32_t) ((b * kMats + mat) * NT + c * 16), v);
 #pragma unroll
@@ -564,7 +568,7 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&S.tempty[b]);
+            if (ok && lane == 0) mbar_arrive(&S.tempty[b]);
             ++seg;
             const bool tile_end = (PH == 0 ? a.kb + 1 == KB : (a.kb + 1 == KB && a.g + 1 == G)) || s + 1 == nsteps;
             if (PH == 1 && (a.kb + 1 == KB || s + 1 == nsteps)) {
@@ -599,7 +603,6 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
                     }
                     if (s + 1 < nsteps) {
                         part_ready();
-                        handed = true;
                     } else {
                         epi_sync();
                         if (tid == 0)
@@ -661,11 +664,6 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
                 seg = 0;
             }
             a.next();
-        }
-        // after a wait that gave up: the finisher's barrier is met all the same
-        if (nsteps > 0 && !handed) {
-            const int steps = min(end, (beg / per_tile + 1) * per_tile) - beg;
-            if (steps != per_tile && beg + steps < end) part_ready();
         }
     }
     tc_fence_before();
