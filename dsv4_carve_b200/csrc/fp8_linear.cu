@@ -907,6 +907,7 @@ int64_t fp8_ldq(int64_t k) { return (k + 15) / 16 * 16; }
 
 int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
                         float* scale, int64_t sr, int64_t sg, int block_rows, bool pow2, cudaStream_t s);
+int fp8_moe_status(int clear, uint32_t* status, cudaStream_t s);
 
 }  // namespace exl3
 
@@ -1009,5 +1010,8 @@ extern "C" int exl3_fp8_status(int clear, uint32_t* status, void* stream) {
         EXL3_CUDA(cudaMemcpyToSymbolAsync(g_fp8_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s));
         EXL3_CUDA(cudaStreamSynchronize(s));
     }
-    return EXL3_OK;
+    uint32_t moe = 0u;
+    const int rc = fp8_moe_status(clear, &moe, s);
+    *status |= moe;
+    return rc;
 }

@@ -40,6 +40,11 @@ int fp8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int6
 int fp8_quantize_launch(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
                         float* scale, int64_t sr, int64_t sg, int block_rows, bool pow2, cudaStream_t s);
 
+// Status bits of this file's kernels on this device, whatever scratch they ran with
+// (exl3_fp8_status): a captured call's scratch belongs to its graph and its control
+// words are cleared with every replay.
+__device__ uint32_t g_fp8_moe_status = 0u;
+
 constexpr int kFmMaxRows = 64;
 constexpr int kFmMaxSlots = 256;             // m * topk
 constexpr int kFmMaxTopk = 16;
@@ -140,6 +145,7 @@ struct FmHead {
     short tokpair[NT];                   // a token's first pair in the group
     uint32_t tmem;
     uint32_t last;
+    uint32_t fail;                       // status bits of this CTA's waits
 };
 
 // The head's bytes, so that what follows it starts on a swizzle atom.
@@ -284,7 +290,7 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
     const int NBI = p.I / 128, NBH = p.H / 128, KB = PH == 0 ? NBH : NBI;
     const int W = p.slots;
     float* xsc = reinterpret_cast<float*>(xres + (KB + 1) * 1024);                             // INL: [KB][8]
-    uint32_t* status = p.ctrl + 2;
+    uint32_t* status = &S.fail;
 
     if (tid == 0) {
         tmap_prefetch(PH == 0 ? &p.w13 : &p.w2);
@@ -295,6 +301,7 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
             mbar_init(&S.tempty[b], 4);
         }
         S.last = 0u;
+        S.fail = 0u;
         fence_barrier_init();
     }
     if (warp == kFmMmaWarp) tmem_alloc(&S.tmem, L::kTmemCols);
@@ -668,6 +675,10 @@ __global__ void __launch_bounds__(kFmThreads, NT <= 32 ? 2 : 1) fp8_moe_kernel(c
     }
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && S.fail != 0u) {
+        set_error(p.ctrl + 2, S.fail);
+        set_error(&g_fp8_moe_status, S.fail);
+    }
     if (kAllFinish && S.last) finish_shared((end - 1) / per_tile, warp, kFmThreads / 32);
     if (warp == kFmMmaWarp) {
         tc_fence_after();
@@ -740,6 +751,19 @@ int fm_run(const FmParams& p, int sms, cudaStream_t s) {
 }
 
 }  // namespace
+
+// Reads the word into `status` (host memory) and clears it on request; synchronizes.
+int fp8_moe_status(int clear, uint32_t* status, cudaStream_t s) {
+    EXL3_CUDA(cudaMemcpyFromSymbolAsync(status, g_fp8_moe_status, sizeof(uint32_t), 0, cudaMemcpyDeviceToHost, s));
+    EXL3_CUDA(cudaStreamSynchronize(s));
+    if (clear) {
+        const uint32_t zero = 0u;
+        EXL3_CUDA(cudaMemcpyToSymbolAsync(g_fp8_moe_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s));
+        EXL3_CUDA(cudaStreamSynchronize(s));
+    }
+    return EXL3_OK;
+}
+
 }  // namespace exl3
 
 extern "C" int64_t exl3_fp8_moe_max_rows(void) { return exl3::kFmMaxRows; }

@@ -711,10 +711,9 @@ def _fp8_linear(x, w: _Fp8Weight, x_scale, bias, out_dtype, pow2_scale) -> torch
 
 
 def fp8_status(device: torch.device | None = None, clear: bool = False) -> int:
-    """Status word of the fp8 linear kernels on a device (0 = healthy; bit 3: a
-    ring wait timed out).  Synchronizes; sticky until cleared."""
-    import ctypes
-
+    """Status word of the fp8 linear and MoE kernels on a device (0 = healthy;
+    bit 3: a ring wait timed out), those of replayed graphs among them.
+    Synchronizes; sticky until cleared."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     word = ctypes.c_uint32(0)
     with _on_device(dev):

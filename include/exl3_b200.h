@@ -347,9 +347,9 @@ int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const float* x_scal
                     const void* w, int64_t ldw, const float* w_scale, const void* bias, int bias_dtype,
                     void* y, int y_dtype, int64_t ldy, int pow2, void* scratch, int64_t scratch_bytes, void* stream);
 
-/* Status word of the fp8 linear kernels on the current device (bit 3: a ring
- * wait timed out), sticky until cleared.  Synchronizes `stream`; not for use
- * during graph capture. */
+/* Status word of the fp8 linear and MoE kernels on the current device (bit 3: a
+ * ring wait timed out), sticky until cleared, for calls from a graph and for any
+ * scratch.  Synchronizes `stream`; not for use during graph capture. */
 int exl3_fp8_status(int clear, uint32_t* status, void* stream);
 
 /* Routed-expert MoE layer for a few tokens over e4m3 experts, two kernels
@@ -372,7 +372,7 @@ int exl3_fp8_status(int clear, uint32_t* status, void* stream);
  * whose first EXL3_FP8_MOE_CTRL_BYTES are zero before first use (calls reset
  * what they need of them, whatever sizes follow); one call at a time per
  * scratch.  Its status word is read by
- * exl3_scratch_status.  No kernel waits for another CTA, so calls on different
+ * exl3_scratch_status; exl3_fp8_status has the same bits for the device.  No kernel waits for another CTA, so calls on different
  * streams with scratches of their own may overlap. */
 #define EXL3_FP8_MOE_CTRL_BYTES 131072
 int64_t exl3_fp8_moe_scratch_bytes(int64_t m, int64_t topk, int64_t hidden, int64_t inter);

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from dsv4_carve_b200 import moe
+from dsv4_carve_b200 import vllm_exl3_c as ext
 from tests import fp8_reference as R
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +46,19 @@ def test_moe_two_host_threads_on_one_stream(cuda):
     for t in threads:
         t.join()
     assert [int(w) for w in wrong] == [0, 0]
+
+
+def test_status_covers_replayed_moe_layers(cuda):
+    """One word for the device, read and cleared outside captures; eager and replayed calls leave it at 0."""
+    state = moe.Fp8MoeState(*_layer(cuda, 8, 512, 256, 3))
+    ids, rw = _route(4, 8, 2, 3, cuda)
+    x = R.activations(4, 512, 3, torch.bfloat16, cuda)
+    want = moe.apply_moe(x, ids, rw, state, None, 10.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = moe.apply_moe(x, ids, rw, state, None, 10.0)
+    for _ in range(3):
+        graph.replay()
+        assert ext.fp8_status(cuda) == 0
+    assert torch.equal(y, want)
+    assert ext.fp8_status(cuda, clear=True) == 0 and ext.fp8_status() == 0
