@@ -39,14 +39,16 @@ __device__ __forceinline__ float fp8_scale(uint32_t amax_bits, bool pow2) {
 // / s keeps that side, does not round back to v (r is a multiple of 2^-27 of v *
 // s at least, so 64 r / s is a unit in the last place) and is still 2^-15 of v at
 // most, far from the next boundary.  A tie (r = 0) stays v, for the conversion to
-// round to even.  All of it is arithmetic without a branch: 16-bit inputs meet
+// round to even.  Both FMAs are taken with the sign turned (v * s - x, times
+// -64 / s), so that -0 stays -0: (-0) * s + 0 is +0, times a negative number -0,
+// plus v = -0 is -0.  All of it is arithmetic without a branch: 16-bit inputs meet
 // midpoints often, because amax divides many of their multiples by 448, and a
 // branch for each value, predicated or voted, was slower (8192 x 4096: 28 us).
 __device__ __forceinline__ float fp8_quotient_fast(float x, float s, float inv) {
     const float q = x * inv;
     const uint32_t b = __float_as_uint(q);
     const float v = __uint_as_float((b + 0x40000u) & 0xFFF80000u);
-    const float side = __fmaf_rn(__fmaf_rn(-v, s, x), 64.f * inv, v);
+    const float side = __fmaf_rn(__fmaf_rn(v, s, -x), -64.f * inv, v);
     return ((b + 2u) & 0x7FFFFu) <= 4u ? side : q;
 }
 

@@ -62,3 +62,29 @@ def test_status_covers_replayed_moe_layers(cuda):
         assert ext.fp8_status(cuda) == 0
     assert torch.equal(y, want)
     assert ext.fp8_status(cuda, clear=True) == 0 and ext.fp8_status() == 0
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [128, 136, 131])
+def test_quantize_keeps_the_sign_of_zero(cuda, cols, dtype, pow2):
+    """The bytes, not the values: -0.0 gives 0x80 in each kind of group, beside
+    ordinary values, alone, and where the scale is tiny or huge; so do negative
+    values that round to zero."""
+    x = R.activations(7, cols, 3, torch.float32, cuda)
+    x[:, ::3] = -0.0
+    x[:, 1::5] = 0.0
+    x[1] = -0.0
+    x[2, 2], x[2, 4] = -1e-7, 1e-7
+    if dtype == torch.float32:
+        x[3] *= 1e-30
+        x[4] *= 1e32
+        x[5, 2] = -1e-44
+    x = x.to(dtype)
+    for rows in (1, 128):
+        q, _ = ext.fp8_quantize(x, block_rows=rows, pow2_scale=pow2)
+        wq, _ = R.quantize(x, rows, pow2)
+        sign = torch.signbit(x)
+        assert torch.equal(q.double(), wq)
+        assert torch.equal((q.view(torch.uint8) & 128) != 0, sign)
+        assert bool(((q.view(torch.uint8) == 128) == (sign & (wq == 0))).all())
