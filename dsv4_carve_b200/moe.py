@@ -301,6 +301,9 @@ def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, s
             or not 1 <= ids.size(-1) <= 16:
         _decline(f"fp8 geometry x={tuple(x2d.shape)} topk={int(ids.shape[-1])}")
         return None
+    w = state.experts
+    if x2d.device != w.device:
+        raise RuntimeError(f"apply_moe: x is on {x2d.device}, the layer's experts are on {w.device}")
     T, topk = x2d.size(0), ids.size(-1)
     ids2, route_w = _router_outputs(ids, weights, expert_map)
     x = x2d if x2d.dtype in _ext._DT else x2d.to(torch.float16)
@@ -310,9 +313,8 @@ def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, s
         out = torch.empty(x.shape, dtype=out_dtype or (x.dtype if x.dtype != torch.float32 else torch.float16),
                           device=x.device)
     step = min(64, 256 // topk)
-    w = state.experts
     if _ext._current_device() != w.index:      # captures are asked of the current device's stream
-        with _ext._on_device(x.device):
+        with _ext._on_device(w.device):
             return apply_fp8_moe(x, ids2, route_w, state, expert_map, limit, out)
     held = _fp8_moe_scratch(x.device)
     with held.lock:

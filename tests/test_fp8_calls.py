@@ -83,3 +83,13 @@ def test_moe_host_threads_on_one_stream_take_turns(layer, monkeypatch):
     for t in threads:
         t.join()
     assert most[0] == 1
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_moe_of_another_device_than_the_current_one(layer, current):
+    """A layer of device 0 runs there whatever is current; rows of device 1 are refused."""
+    torch.cuda.set_device(current)
+    moe.apply_moe(**_call(), state=layer)
+    assert len(layer.launched) == 1 and torch.cuda.current_device() == current
+    with pytest.raises(RuntimeError, match="x is on cuda:1, the layer's experts are on cuda:0"):
+        moe.apply_moe(**_call(kind=OnDevice1), state=layer)
