@@ -304,9 +304,11 @@ def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, s
     w = state.experts
     if x2d.device != w.device:
         raise RuntimeError(f"apply_moe: x is on {x2d.device}, the layer's experts are on {w.device}")
+    if x2d.dtype == torch.float8_e4m3fn:
+        raise RuntimeError("apply_moe: x in e4m3 comes without its scales here; fp8_moe_decode takes both (x_scale)")
     T, topk = x2d.size(0), ids.size(-1)
     ids2, route_w = _router_outputs(ids, weights, expert_map)
-    x = x2d if x2d.dtype in _ext._DT else x2d.to(torch.float16)
+    x = x2d if x2d.dtype in _ext._DT else x2d.to(torch.float32)     # fp16 would overflow ahead of the quantiser
     if not x.is_contiguous():
         x = x.contiguous()
     if out is None:

@@ -93,3 +93,15 @@ def test_moe_of_another_device_than_the_current_one(layer, current):
     assert len(layer.launched) == 1 and torch.cuda.current_device() == current
     with pytest.raises(RuntimeError, match="x is on cuda:1, the layer's experts are on cuda:0"):
         moe.apply_moe(**_call(kind=OnDevice1), state=layer)
+
+
+def test_moe_types_of_x(layer):
+    """e4m3 rows are refused, because their scales have no way in; fp64 ones keep their range."""
+    with pytest.raises(RuntimeError, match="x_scale"):
+        moe.apply_moe(**_call(dtype=torch.float8_e4m3fn), state=layer)
+    assert not layer.launched
+    call = _call(dtype=torch.float64)
+    call["x2d"] = call["x2d"] * 1e6
+    moe.apply_moe(**call, state=layer)
+    x, out = layer.launched[0][0], layer.launched[0][2]
+    assert x.dtype == torch.float32 and float(x[0, 0]) == 1e6 and out.dtype == torch.float16
