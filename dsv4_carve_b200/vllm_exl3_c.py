@@ -744,6 +744,8 @@ def _fp8_moe_weight_checks(gate_up, gate_up_scale, down, down_scale) -> tuple:
            "fp8_moe_decode: gate_up must be [experts, 2 * intermediate, hidden], down [experts, hidden, intermediate]")
     _check(H >= 128 and H % 128 == 0 and I >= 128 and I % 128 == 0,
            "fp8_moe_decode: hidden and intermediate must be multiples of 128")
+    _check(fp8_moe_scratch_bytes(1, 1, H, I) > 0,
+           f"fp8_moe_decode: hidden up to 16384 and intermediate up to 8192 are served, got {H} and {I}")
     _check(gate_up.data_ptr() % 16 == 0 and down.data_ptr() % 16 == 0, "fp8_moe_decode: weights must be 16-byte aligned")
     _check(gate_up_scale.dtype == torch.float32 and gate_up_scale.shape == (E, I2 // 128, H // 128)
            and down_scale.dtype == torch.float32 and down_scale.shape == (E, H // 128, I // 128),

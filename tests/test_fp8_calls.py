@@ -105,3 +105,19 @@ def test_moe_types_of_x(layer):
     moe.apply_moe(**call, state=layer)
     x, out = layer.launched[0][0], layer.launched[0][2]
     assert x.dtype == torch.float32 and float(x[0, 0]) == 1e6 and out.dtype == torch.float16
+
+
+@pytest.mark.parametrize("H,I", [(16512, 128), (128, 8320)])
+def test_moe_state_refuses_sizes_past_the_limits(H, I):
+    """The layer's own message, where the state is built."""
+    def of(shape, dtype):
+        return torch.empty(shape, dtype=dtype).as_subclass(OnDevice)
+
+    def state(H, I):
+        f8 = torch.float8_e4m3fn
+        return moe.Fp8MoeState(of((1, 2 * I, H), f8), of((1, 2 * I // 128, H // 128), torch.float32),
+                               of((1, H, I), f8), of((1, H // 128, I // 128), torch.float32))
+
+    with pytest.raises(RuntimeError, match="16384 and intermediate up to 8192"):
+        state(H, I)
+    assert state(H - 128, I).hidden == H - 128 if H > I else state(H, I - 128).inter == I - 128
