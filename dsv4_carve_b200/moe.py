@@ -297,8 +297,7 @@ def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, s
     """The routed experts of an e4m3 layer: fp8_moe_decode, the rows in pieces
     above its row ceiling.  Returns the [T, hidden] output, or None when the
     call is declined."""
-    if not x2d.is_cuda or x2d.dim() != 2 or x2d.size(0) < 1 or x2d.size(1) != state.hidden \
-            or not 1 <= ids.size(-1) <= 16:
+    if not x2d.is_cuda or x2d.dim() != 2 or x2d.size(0) < 1 or x2d.size(1) != state.hidden:
         _decline(f"fp8 geometry x={tuple(x2d.shape)} topk={int(ids.shape[-1])}")
         return None
     w = state.experts
@@ -306,8 +305,16 @@ def apply_fp8_moe(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, s
         raise RuntimeError(f"apply_moe: x is on {x2d.device}, the layer's experts are on {w.device}")
     if x2d.dtype == torch.float8_e4m3fn:
         raise RuntimeError("apply_moe: x in e4m3 comes without its scales here; fp8_moe_decode takes both (x_scale)")
-    T, topk = x2d.size(0), ids.size(-1)
     ids2, route_w = _router_outputs(ids, weights, expert_map)
+    T, topk = x2d.size(0), ids2.size(1)
+    if not 1 <= topk <= 16:
+        _decline(f"fp8 geometry x={tuple(x2d.shape)} topk={topk}")
+        return None
+    # of the whole call, ahead of the first piece's launch
+    if ids2.size(0) != T:
+        raise RuntimeError(f"apply_moe: ids of {ids2.size(0)} rows for {T} rows of x")
+    if out is not None and (out.shape != x2d.shape or not out.is_contiguous()):
+        raise RuntimeError("apply_moe: out must be contiguous and of x's shape")
     x = x2d if x2d.dtype in _ext._DT else x2d.to(torch.float32)     # fp16 would overflow ahead of the quantiser
     if not x.is_contiguous():
         x = x.contiguous()

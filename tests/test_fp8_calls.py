@@ -121,3 +121,30 @@ def test_moe_state_refuses_sizes_past_the_limits(H, I):
     with pytest.raises(RuntimeError, match="16384 and intermediate up to 8192"):
         state(H, I)
     assert state(H - 128, I).hidden == H - 128 if H > I else state(H, I - 128).inter == I - 128
+
+
+@pytest.mark.parametrize("T", [5, 80])
+def test_moe_checks_the_whole_call_ahead_of_its_pieces(layer, T):
+    """ids or out of another number of rows are refused, in one piece or several, before a launch."""
+    more = _call(T + 3, 8)
+    call = _call(T, 8)
+    with pytest.raises(RuntimeError, match="ids of"):
+        moe.apply_moe(**{**call, "ids": more["ids"], "weights": more["weights"]}, state=layer)
+    less = _call(T - 1, 8)
+    with pytest.raises(RuntimeError, match="ids of"):
+        moe.apply_moe(**{**call, "ids": less["ids"], "weights": less["weights"]}, state=layer)
+    for out in (torch.empty((T + 3, 256)), torch.empty((T, 512))[:, ::2], torch.empty((T - 1, 256))):
+        with pytest.raises(RuntimeError, match="out must be"):
+            moe.apply_moe(**call, state=layer, out=out.as_subclass(OnDevice))
+    assert not layer.launched
+
+
+@pytest.mark.parametrize("shape,topk", [((20,), 1), ((20, 2, 4), 8), ((20, 4), 4)])
+def test_moe_ids_of_other_ranks(layer, shape, topk):
+    """ids [rows] are one slot a row, more dimensions are slots too; the scratch is asked for what is launched."""
+    call = _call(20, 1)
+    call["ids"] = torch.ones(shape, dtype=torch.int32).as_subclass(OnDevice)
+    call["weights"] = torch.ones(shape).as_subclass(OnDevice)
+    moe.apply_moe(**call, state=layer)
+    assert [tuple(a[4].shape) for a in layer.launched] == [(20, topk)]
+    assert layer.launched[0][7].numel() == ext.fp8_moe_scratch_bytes(20, topk, 256, 128)
