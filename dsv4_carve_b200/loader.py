@@ -329,15 +329,15 @@ def load_linear(ckpt: Checkpoint, prefix: str, device="cuda", config: Exl3QuantC
     """A dense module (attention / shared expert): the LinearEXL3 that the
     plugin's dense branch calls, K checked against non_routed_exl3 when the
     config lists the module; or LinearFP8 where the pack leaves the module in
-    e4m3 with block scales."""
-    if has_fp8(ckpt, prefix):
-        weight, scale, pow2 = load_fp8_weight(ckpt, prefix, device)
-        bias = ckpt.get(f"{prefix}.bias", device) if ckpt.has(f"{prefix}.bias") else None
-        return LinearFP8(weight, scale, bias=bias, pow2_scale=pow2, key=prefix)
+    e4m3 with block scales and the config does not list it."""
     config = config or ckpt.config
     bits = None
     if config is not None and config.matches_non_routed(prefix):
         bits = config.bits_for_non_routed(prefix)
+    elif has_fp8(ckpt, prefix):
+        weight, scale, pow2 = load_fp8_weight(ckpt, prefix, device)
+        bias = ckpt.get(f"{prefix}.bias", device) if ckpt.has(f"{prefix}.bias") else None
+        return LinearFP8(weight, scale, bias=bias, pow2_scale=pow2, key=prefix)
     w = load_dense(ckpt, prefix, device, bits)
     mcg = ckpt.get(f"{prefix}.mcg", device) if w.cb == synth.CB_MCG else None
     mul1 = ckpt.get(f"{prefix}.mul1", device) if w.cb == synth.CB_MUL1 else None
