@@ -111,14 +111,16 @@ class LinearFP8:
                 padded = torch.zeros((weight.size(0), -(-k // 16) * 16), dtype=torch.uint8, device=weight.device)
                 padded[:, :k] = weight.view(torch.uint8)
                 weight = padded.view(torch.float8_e4m3fn)[:, :k]
-        self.weight = weight
-        self.weight_scale = weight_scale.to(torch.float32).contiguous()
-        self._w = _ext._Fp8Weight(self.weight, self.weight_scale)
+        self._w = _ext._Fp8Weight(weight, weight_scale.to(torch.float32).contiguous())
         self.out_features, self.in_features = (int(v) for v in weight.shape)
         self.bias = bias
         self.default_out_dtype = out_dtype or torch.half
         self.pow2_scale = bool(pow2_scale)
         self.key = key
+
+    # Checked and taken by address once, so not to be assigned (writes into them are seen).
+    weight = property(lambda self: self._w.weight)
+    weight_scale = property(lambda self: self._w.scale)
 
     @classmethod
     def from_weight(cls, weight: torch.Tensor, **kw) -> "LinearFP8":

@@ -245,12 +245,16 @@ class Fp8MoeState:
 
     def __init__(self, gate_up: torch.Tensor, gate_up_scale: torch.Tensor, down: torch.Tensor,
                  down_scale: torch.Tensor, pow2_scale: bool = False):
-        self.gate_up, self.down = gate_up, down
-        self.gate_up_scale = gate_up_scale.to(torch.float32).contiguous()
-        self.down_scale = down_scale.to(torch.float32).contiguous()
-        self.experts = _ext._Fp8Experts(self.gate_up, self.gate_up_scale, self.down, self.down_scale)
+        self.experts = _ext._Fp8Experts(gate_up, gate_up_scale.to(torch.float32).contiguous(),
+                                        down, down_scale.to(torch.float32).contiguous())
         self.n_experts, self.hidden, self.inter = self.experts.E, self.experts.H, self.experts.I
         self.pow2_scale = bool(pow2_scale)
+
+    # Checked and taken by address once, so not to be assigned (writes into them are seen).
+    gate_up = property(lambda self: self.experts.tensors[0])
+    gate_up_scale = property(lambda self: self.experts.tensors[1])
+    down = property(lambda self: self.experts.tensors[2])
+    down_scale = property(lambda self: self.experts.tensors[3])
 
 
 class _Fp8Scratch:

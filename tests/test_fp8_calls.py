@@ -11,6 +11,7 @@ import torch
 
 from dsv4_carve_b200 import moe
 from dsv4_carve_b200 import vllm_exl3_c as ext
+from dsv4_carve_b200.linear import LinearFP8
 
 
 class OnDevice(torch.Tensor):
@@ -148,3 +149,18 @@ def test_moe_ids_of_other_ranks(layer, shape, topk):
     moe.apply_moe(**call, state=layer)
     assert [tuple(a[4].shape) for a in layer.launched] == [(20, topk)]
     assert layer.launched[0][7].numel() == ext.fp8_moe_scratch_bytes(20, topk, 256, 128)
+
+
+def test_weights_of_a_built_layer_are_not_assigned():
+    """What the kernels read was taken when the layer was built; another tensor needs another layer."""
+    def of(shape, dtype=torch.float32):
+        return torch.zeros(shape).to(dtype).as_subclass(OnDevice)
+
+    f8 = torch.float8_e4m3fn
+    lin = LinearFP8(of((256, 128), f8), of((2, 1)))
+    state = moe.Fp8MoeState(of((2, 256, 128), f8), of((2, 2, 1)), of((2, 128, 128), f8), of((2, 1, 1)))
+    assert lin.weight.shape == (256, 128) and lin.weight_scale.shape == (2, 1) and state.down_scale.shape == (2, 1, 1)
+    for layer_, names in ((lin, ("weight", "weight_scale")), (state, ("gate_up", "gate_up_scale", "down", "down_scale"))):
+        for name in names:
+            with pytest.raises(AttributeError):
+                setattr(layer_, name, getattr(layer_, name).clone())
