@@ -926,6 +926,9 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, int64_t ldx, const fl
     EXL3_REQUIRE((x_dtype == EXL3_DTYPE_E4M3) == (x_scale != nullptr), EXL3_ERR_ARG,
                  "exl3_fp8_linear: x_scale goes with an e4m3 x, and only with one");
     EXL3_REQUIRE(aligned16(w) && ldw % 16 == 0, EXL3_ERR_ARG, "exl3_fp8_linear: weight rows must be 16-byte aligned");
+    EXL3_REQUIRE(aligned_to(x, dtype_bytes(x_dtype)) && aligned_to(y, dtype_bytes(y_dtype)) && aligned_to(x_scale, 4) &&
+                     aligned_to(w_scale, 4) && aligned_to(bias, dtype_bytes(bias_dtype)),
+                 EXL3_ERR_ARG, "exl3_fp8_linear: x, y, bias and the scales must be aligned to their elements");
     auto s = static_cast<cudaStream_t>(stream);
     const int groups = (int) ((k + 127) / 128);
     const int es = x_dtype == 2 ? 4 : x_dtype == 3 ? 1 : 2;

@@ -801,6 +801,10 @@ extern "C" int exl3_fp8_moe_decode(const void* x, int x_dtype, const float* x_sc
     EXL3_REQUIRE(swiglu_limit > 0.f, EXL3_ERR_ARG, "exl3_fp8_moe_decode: the SwiGLU limit must be positive");
     EXL3_REQUIRE(aligned16(gate_up) && aligned16(down) && aligned16(scratch), EXL3_ERR_ARG,
                  "exl3_fp8_moe_decode: weights and scratch must be 16-byte aligned");
+    EXL3_REQUIRE(aligned_to(x, dtype_bytes(x_dtype)) && aligned_to(out, dtype_bytes(out_dtype)) && aligned_to(x_scale, 4) &&
+                     aligned_to(gate_up_scale, 4) && aligned_to(down_scale, 4) && aligned_to(route->ids, route->ids_dtype ? 8 : 4) &&
+                     aligned_to(route->weights, dtype_bytes(route->weights_dtype)) && aligned_to(route->expert_map, 8),
+                 EXL3_ERR_ARG, "exl3_fp8_moe_decode: x, out, scales, ids, routing weights and map must be aligned to their elements");
     const FmGeom g = fm_geom(m, topk, hidden, inter);
     EXL3_REQUIRE(scratch_bytes >= g.bytes, EXL3_ERR_ARG, "exl3_fp8_moe_decode: scratch too small (%lld < %lld bytes)",
                  (long long) scratch_bytes, (long long) g.bytes);

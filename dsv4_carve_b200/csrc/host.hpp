@@ -45,4 +45,10 @@ inline int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// To elements of `bytes`; a null pointer is.
+inline bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t) bytes == 0; }
+
+// Bytes of an element: fp16, bf16, fp32, e4m3.
+inline int dtype_bytes(int dtype) { return dtype == EXL3_DTYPE_F32 ? 4 : dtype == EXL3_DTYPE_E4M3 ? 1 : 2; }
+
 }  // namespace exl3
