@@ -88,3 +88,23 @@ def test_quantize_keeps_the_sign_of_zero(cuda, cols, dtype, pow2):
         assert torch.equal(q.double(), wq)
         assert torch.equal((q.view(torch.uint8) & 128) != 0, sign)
         assert bool(((q.view(torch.uint8) == 128) == (sign & (wq == 0))).all())
+
+
+@pytest.mark.parametrize("rows", [1, 5, 20, 129, 300])
+def test_linear_e4m3_rows_at_any_offset(cuda, rows):
+    """e4m3 x whose rows start off 16 bytes or lie apart, eager and captured: the bits of an aligned one."""
+    w, ws = R.e4m3_weight((384, 528), 5, cuda)
+    q, s = ext.fp8_quantize(R.activations(rows, 528, 6, torch.bfloat16, cuda))
+    want = ext.fp8_linear(q, w, ws, x_scale=s, out_dtype=torch.float32)
+    for off, width in ((0, 529), (3, 560), (4, 576), (16, 592), (1, 529)):
+        wide = torch.zeros((rows, width), dtype=torch.uint8, device=cuda)
+        wide[:, off:off + 528] = q.view(torch.uint8)
+        x = wide.view(R.F8)[:, off:off + 528]
+        assert torch.equal(ext.fp8_linear(x, w, ws, x_scale=s, out_dtype=torch.float32), want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = ext.fp8_linear(x, w, ws, x_scale=s, out_dtype=torch.float32)
+        y.zero_()
+        for _ in range(2):
+            graph.replay()
+        assert torch.equal(y, want)
