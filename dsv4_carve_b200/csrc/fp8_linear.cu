@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(kFrThreads, FrLayout<NT>::kCtas) fp8_rows_kern
                     for (int c = 0; c < NC; ++c) tc_ld32_issue(tcol + (uint32_t) (b * NT + c * 32), v[c]);
 #pragma unroll
                     for (int c = 0; c < NC; ++c) {
-                        tc_ld32_wait(v[c]);
+                        tc_ld_wait(v[c]);
 #pragma unroll
                         for (int q = 0; q < 8; ++q) {
                             const float4 f = f4[c * 8 + q];
@@ -669,7 +669,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFgThreads, 1) fp8_g
                 for (int i = 0; i < NC * L::kKS; ++i) {
                     const int c = i % NC;
                     if (i / NC >= n) break;
-                    tc_ld32_wait(v[i & 1]);
+                    tc_ld_wait(v[i & 1]);
                     if (i + 1 < NC * n) {
                         tc_ld32_issue(col_of(i + 1), v[(i + 1) & 1]);
                     } else {
