@@ -108,3 +108,54 @@ def test_linear_e4m3_rows_at_any_offset(cuda, rows):
         for _ in range(2):
             graph.replay()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_inputs_from_another_stream(cuda, captured):
+    """Rows, ids and weights that a side stream makes while the calls' stream is at
+    other work, joined by an event directly ahead of each call."""
+    H = 1024
+    w, ws = R.e4m3_weight((512, H), 50, cuda)
+    state = moe.Fp8MoeState(*_layer(cuda, 8, H, 256, 51))
+    side = torch.cuda.Stream()
+    src = torch.zeros((300, H), device=cuda)
+    lst = torch.zeros((32, 4), dtype=torch.int32, device=cuda)
+    waste = torch.ones((2048, 2048), device=cuda)
+    calls = {"quantize": lambda x, i: ext.fp8_quantize(x)[0].view(torch.uint8),
+             "linear 4": lambda x, i: ext.fp8_linear(x[:4], w, ws), "linear 40": lambda x, i: ext.fp8_linear(x[:40], w, ws),
+             "linear 300": lambda x, i: ext.fp8_linear(x, w, ws),
+             "moe 2": lambda x, i: moe.apply_moe(x[:2], i[:2], torch.ones((2, 4), device=cuda), state, None, 10.0),
+             "moe 32": lambda x, i: moe.apply_moe(x[:32], i, torch.ones((32, 4), device=cuda), state, None, 10.0)}
+
+    def step(call):
+        main = torch.cuda.current_stream()
+        call(src, lst)                                       # the kernels that came before, whose end may be overlapped
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            m = waste
+            for _ in range(4):
+                m = m @ waste * 2.0 ** -11                   # 1.0 again, late
+            x = src * m[0, 0]
+            ids = lst + (m[1, 1] - 1.0).to(torch.int32)
+        call(src, lst)
+        main.wait_stream(side)
+        return call(x, ids), x, ids, m
+
+    for name, call in calls.items():
+        if captured:
+            step(call)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                kept = step(call)
+        for seed in range(3):
+            src.copy_(R.activations(300, H, seed, torch.bfloat16, cuda))
+            lst.copy_(_route(32, 8, 4, seed, cuda)[0])
+            if captured:
+                graph.replay()
+            else:
+                kept = step(call)
+            torch.cuda.synchronize()
+            assert torch.equal(kept[1], src) and torch.equal(kept[2], lst)
+            assert torch.equal(kept[0], call(src, lst)), name
+            torch.cuda.synchronize()
