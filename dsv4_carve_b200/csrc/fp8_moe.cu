@@ -24,8 +24,9 @@
 // another one.  Kernel 2 starts while kernel 1 runs (programmatic launch): it
 // builds the same route plan and fills its shared-memory ring with weights, then
 // waits for kernel 1 to complete before it touches what kernel 1 wrote.  4096
-// columns, top-8 of 256: 1 token of I = 256 20.6 us, 4 of 2048 130 us (758 MB, 89 % of
-// the copy rate), 32 of 512 with Zipf routes 114 us (400 MB).
+// columns, top-8 of 256, calls in a CUDA graph: 1 token of I = 256 20.8 us, 4 of 2048
+// 132.7 us (758 MB, 87 % of the copy rate; called one by one 137-148 us), 32 of 512
+// with Zipf routes 110-113 us (400 MB; 105-126, as the routes and the GPU are).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

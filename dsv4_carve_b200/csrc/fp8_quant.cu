@@ -5,7 +5,7 @@
 // Bound: memory, es + 1 bytes for each element (es = 2 or 4) plus the scales.
 // Every value is loaded once, kept in registers while its group's maximum is
 // taken over the lanes that hold it, and stored as e4m3.  8192 x 4096 bf16 with
-// powers of two takes 14 us in a graph (102 MB at the copy rate; 22 us with exact
+// powers of two takes 14 us in a graph (102 MB at the copy rate; 20.6 us with exact
 // quotients, bound by instructions), 4000 x 4080 in
 // blocks 11.2 us (4.4 TB/s: a block is loaded, reduced and stored in turn).
 #include "fp8.cuh"
