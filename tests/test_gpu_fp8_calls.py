@@ -159,3 +159,36 @@ def test_inputs_from_another_stream(cuda, captured):
             assert torch.equal(kept[1], src) and torch.equal(kept[2], lst)
             assert torch.equal(kept[0], call(src, lst)), name
             torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits(cuda):
+    """x, y, its e4m3 copy and the weight with more than 2^31 elements: their last rows."""
+    rows, tail = 530000, 300
+    w, ws = R.e4m3_weight((136, 4096), 60, cuda)
+    x = torch.empty((rows, 4096), dtype=torch.bfloat16, device=cuda).normal_(generator=torch.Generator(device=cuda).manual_seed(1))
+    assert x.numel() > 2 ** 31
+    wq, wscale = R.quantize(x[-tail:])
+    q, s = ext.fp8_quantize(x)
+    assert torch.equal(q[-tail:].double(), wq) and torch.equal(s[-tail:].double(), wscale)
+    del q, s
+    q, s = ext.fp8_quantize(x, block_rows=128)
+    last = rows // 128 * 128
+    wq, wscale = R.quantize(x[last - 128:], 128)
+    assert torch.equal(q[last - 128:].double(), wq) and torch.equal(s[-wscale.shape[0]:].double(), wscale)
+    del q, s
+    want, allowed = R.linear(R.rows_dequant(x[-tail:]), R.weight(w, ws))
+    assert R.worst(ext.fp8_linear(x, w, ws, out_dtype=torch.float32)[-tail:], want, allowed) <= 1.0
+    x = x[:, :128].contiguous()
+    for n in (4096, 4097):
+        w, ws = R.e4m3_weight((n, 128), n, cuda)
+        want, allowed = R.linear(R.rows_dequant(x[-tail:]), R.weight(w, ws), None, torch.bfloat16)
+        y = ext.fp8_linear(x, w, ws)
+        assert y.numel() > 2 ** 31 and R.worst(y[-tail:], want, allowed) <= 1.0
+        del y
+    n = 128 * 4150
+    w = torch.randint(0, 126, (n, 4096), dtype=torch.uint8, device=cuda, generator=torch.Generator(device=cuda).manual_seed(2)).view(R.F8)
+    ws = torch.rand((4150, 32), device=cuda)
+    for m in (3, 20, 140):
+        xm = R.activations(m, 4096, m, torch.bfloat16, cuda)
+        want, allowed = R.linear(R.rows_dequant(xm), R.weight(w[-256:], ws[-2:]))
+        assert R.worst(ext.fp8_linear(xm, w, ws, out_dtype=torch.float32)[:, -256:], want, allowed) <= 1.0
